@@ -21,6 +21,8 @@ EXPORTS = (
     "cet_informer_forward_taps",
     "cet_rnn_blob_size", "cet_rnn_create", "cet_rnn_rollout", "cet_rnn_select", "cet_rnn_rollout_static", "cet_lmmse", "cet_lmmse_direct",
     "cet_lmmse_llr", "cet_lmmse_block", "cet_lmmse_block_llr", "cet_lmmse_grid", "cet_ls_nn", "cet_nmse_sums", "cet_qpsk_bit_errors",
+    "cet_linear_attention_workspace", "cet_linear_attention", "cet_linear_attention_backward",
+    "cet_linear_attention_step",
 )
 
 
@@ -33,6 +35,12 @@ class InformerCfg(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "enc_in", "dec_in", "c_out", "seq_len", "label_len", "pred_len", "d_model", "n_heads",
         "e_layers", "d_layers", "d_ff", "stack", "distil", "activation")]
+
+
+class LinattnDesc(ctypes.Structure):
+    """Mirror of `cet_linattn_desc`."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "T", "H", "K", "V", "lengths64")] + [
+        ("scale", ctypes.c_float)] + [(n, ctypes.c_int64 * 3) for n in ("q", "k", "v", "d_o")]
 
 
 _lib = None
@@ -86,6 +94,12 @@ def lib():
                             ctypes.c_int, vp]
     L.cet_nmse_sums.argtypes = [fp, fp, fp, ctypes.c_long, ctypes.c_int, ctypes.c_int, vp]
     L.cet_qpsk_bit_errors.argtypes = [fp, fp, fp, ctypes.c_long, vp]
+    ip, desc = ctypes.c_int, ctypes.POINTER(LinattnDesc)
+    L.cet_linear_attention_workspace.restype = ctypes.c_size_t
+    L.cet_linear_attention_workspace.argtypes = [desc, vp, vp, vp, vp, ip]
+    L.cet_linear_attention.argtypes = [desc] + [vp] * 9 + [ctypes.c_size_t, vp]
+    L.cet_linear_attention_backward.argtypes = [desc] + [vp] * 13 + [ctypes.c_size_t, vp]
+    L.cet_linear_attention_step.argtypes = [ip] * 5 + [vp] * 7 + [ctypes.c_float, vp, vp, ip, vp, ip, vp, vp]
     for name in EXPORTS:
         getattr(L, name)  # AttributeError here means header and library disagree
     _lib = L

@@ -1,0 +1,387 @@
+// Linear attention with a decay per head: entry points, the join of the segments' states, the copy of
+// operands that wide loads cannot take, and the form for single slots. The chunk kernels are in linattn.h.
+#include <algorithm>
+#include <cmath>
+
+#include "linattn.h"
+
+namespace cet {
+namespace la {
+namespace {
+
+constexpr size_t align_up(size_t n) { return (n + 255) & ~(size_t)255; }
+constexpr int elem_bytes(int dtype) { return dtype == CET_F32 ? 4 : 2; }
+
+// ws[bh][s] holds what segment s adds to the state; afterwards the state behind segment s (the one that
+// segment s + 1 starts from). One thread per state element, segments in order.
+__global__ __launch_bounds__(256) void join_segments(const Args a) {
+  const long states = (long)a.K * a.V, at = (long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= states * a.B * a.H) return;
+  const long bh = at / states, e = at % states;
+  const double dn = exp((double)a.seg_len * (double)a.log_decay[bh % a.H]);
+  const float hi = (float)dn, lo = (float)(dn - (double)hi);
+  float cur = a.init ? a.init[bh * states + e / a.V * a.init_k + e % a.V * a.init_v] : 0.f;
+  float* p = a.ws + bh * (a.nseg - 1) * states + e;
+  for (int s = 0; s < a.nseg - 1; ++s, p += states) {
+    cur = fmaf(cur, hi, cur * lo) + *p;
+    *p = cur;
+  }
+}
+
+// [B,T,H,D] with any strides -> contiguous with D rounded up to a multiple of 16 bytes, zeros behind D
+template <typename E>
+__global__ __launch_bounds__(256) void pack_rows(const E* __restrict__ src, Strides s, E* __restrict__ dst, int T, int H,
+                                                 int D, int per_row, long total) {
+  constexpr int VEC = 16 / sizeof(E);
+  for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long)gridDim.x * 256) {
+    const int c = (int)(at % per_row) * VEC;
+    const long row = at / per_row, h = row % H, t = row / H % T, b = row / H / T;
+    const E* p = src + b * s.b + t * s.t + h * s.h;
+    E e[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = c + j < D ? p[c + j] : E(0);
+    uint4 raw;
+    __builtin_memcpy(&raw, e, 16);
+    reinterpret_cast<uint4*>(dst)[at] = raw;
+  }
+}
+
+// One slot. A workgroup takes 4 TX (or TX, where rows of V are no multiple of four) columns of one head's
+// state of one stream; the rows of K are spread over TY = 256 / TX threads per column group, whose partial
+// sums of q S are added over the lanes of a wave and then over the four waves in LDS.
+template <typename IO>
+struct Step {
+  const IO *q, *k, *v;
+  long qb, qh, kb, kh, vb, vh;
+  const float* log_decay;
+  const float* in;
+  float* out;
+  const void* slots;
+  IO* o;
+  int B, H, K, V, rows, slots64, nslice;
+  float scale;
+};
+
+__device__ inline long slot_of(const void* slots, int wide, int b) {
+  return wide ? static_cast<const long*>(slots)[b] : (long)static_cast<const int*>(slots)[b];
+}
+
+template <typename IO, int TX, int W>
+__global__ __launch_bounds__(256) void step(const Step<IO> a) {
+  constexpr int TY = 256 / TX, COLS = TX * W;
+  __shared__ float ks[256], qs[256], part[4][COLS];
+  const int tid = threadIdx.x, tx = tid % TX, ty = tid / TX;
+  unsigned id = blockIdx.x;
+  const int c = (int)(id % a.nslice) * COLS + tx * W;
+  id /= a.nslice;
+  const int h = (int)(id % a.H), b = (int)(id / a.H);
+  long row = b;
+  float idle = 0.f;
+  bool live = true;
+  if (a.slots) {
+    row = slot_of(a.slots, a.slots64, b);
+    // a slot that an earlier stream of this call has: two workgroups would update one state
+    bool twice = false;
+    if (row >= 0)
+      for (int e = tid; e < b; e += 256) twice |= slot_of(a.slots, a.slots64, e) == row;
+    twice = __syncthreads_or(twice);
+    live = row >= 0 && row < a.rows && !twice;
+    if (row >= 0 && !live) idle = __builtin_nanf("");
+  }
+  if (live) {
+    if (tid < a.K) {
+      ks[tid] = (float)a.k[b * a.kb + h * a.kh + tid];
+      qs[tid] = (float)a.q[b * a.qb + h * a.qh + tid] * a.scale;
+    }
+    const float d = expf(a.log_decay[h]);
+    float v[W], acc[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      v[w] = c + w < a.V ? (float)a.v[b * a.vb + h * a.vh + c + w] : 0.f;
+      acc[w] = 0.f;
+    }
+    __syncthreads();
+    const long base = (row * a.H + h) * a.K * a.V + c;
+    if (c < a.V) {  // V is a multiple of W
+#pragma unroll 4
+      for (int x = ty; x < a.K; x += TY) {
+        const float* p = a.in + base + (long)x * a.V;
+        float* to = a.out + base + (long)x * a.V;
+        float s[W];
+        if constexpr (W == 4) {
+          *reinterpret_cast<f4*>(s) = *reinterpret_cast<const f4*>(p);
+        } else {
+          s[0] = *p;
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          s[w] = fmaf(s[w], d, ks[x] * v[w]);
+          acc[w] = fmaf(qs[x], s[w], acc[w]);
+        }
+        if constexpr (W == 4) {
+          *reinterpret_cast<f4*>(to) = *reinterpret_cast<f4*>(s);
+        } else {
+          *to = s[0];
+        }
+      }
+    }
+#pragma unroll
+    for (int off = TX; off < 64; off *= 2)
+#pragma unroll
+      for (int w = 0; w < W; ++w) acc[w] += __shfl_xor(acc[w], off);
+    if ((tid & 63) < TX)
+#pragma unroll
+      for (int w = 0; w < W; ++w) part[tid >> 6][tx * W + w] = acc[w];
+  }
+  __syncthreads();
+  const int first = (int)(blockIdx.x % a.nslice) * COLS;
+  for (int x = tid; x < COLS; x += 256)
+    if (first + x < a.V) {
+      const float r = live ? part[0][x] + part[1][x] + part[2][x] + part[3][x] : idle;
+      a.o[((long)b * a.H + h) * a.V + first + x] = (IO)r;
+    }
+}
+
+int cu_count() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1)
+    return 256;
+  return n;
+}
+
+struct Operand {
+  const void* p;
+  Strides s;
+  int D;
+  size_t copy = 0;  // bytes of its packed copy, 0 where it is read in place
+
+  Operand(const void* ptr, const int64_t* st, int D, const cet_linattn_desc& d) : p(ptr), s{st[0], st[1], st[2]}, D(D) {
+    const int vec = 16 / elem_bytes(d.dtype);
+    const bool wide = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && D % vec == 0 && (s.b % vec == 0 || d.B == 1) &&
+                      (s.t % vec == 0 || d.T == 1) && (s.h % vec == 0 || d.H == 1);
+    if (!wide) copy = align_up((size_t)d.B * d.T * d.H * ((D + vec - 1) / vec) * 16);
+  }
+  int pack(const cet_linattn_desc& d, char*& ws, hipStream_t stream) {
+    if (!copy) return CET_OK;
+    const int vec = 16 / elem_bytes(d.dtype), per_row = (D + vec - 1) / vec;
+    const long total = (long)d.B * d.T * d.H * per_row;
+    const unsigned blocks = (unsigned)std::min<long>((total + 255) / 256, 1 << 20);
+    if (d.dtype == CET_F32)
+      pack_rows<uint32_t><<<blocks, 256, 0, stream>>>(static_cast<const uint32_t*>(p), s, reinterpret_cast<uint32_t*>(ws), d.T, d.H, D, per_row, total);
+    else
+      pack_rows<uint16_t><<<blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(p), s, reinterpret_cast<uint16_t*>(ws), d.T, d.H, D, per_row, total);
+    CET_HIP(hipGetLastError());
+    const long row = (long)per_row * vec;
+    p = ws;
+    s = Strides{(long)d.T * d.H * row, d.H * row, row};
+    ws += copy;
+    return CET_OK;
+  }
+};
+
+// How a pass over the slots is cut: slices of V, and segments of the time axis where heads, sequences and
+// slices alone are fewer than two workgroups per CU.
+struct Cut {
+  int nslice, nseg, seg_len;
+  size_t ws;  // bytes for the segments' states
+};
+
+Cut cut(const cet_linattn_desc& d, int K, int V, int cus) {
+  Cut c;
+  const int cols = slice_columns(K, V), C = chunk_slots(d.dtype);
+  c.nslice = (V + cols - 1) / cols;
+  const long tasks = (long)d.B * d.H * c.nslice, chunks = (d.T + C - 1) / C;
+  long nseg = tasks ? std::min<long>(2L * cus / tasks, chunks / 4) : 1;
+  nseg = std::max<long>(nseg, 1);
+  const long per = (std::max<long>(chunks, 1) + nseg - 1) / nseg;
+  c.seg_len = (int)(per * C);
+  c.nseg = (int)std::max<long>((chunks + per - 1) / per, 1);
+  c.ws = c.nseg > 1 ? align_up((size_t)d.B * d.H * (c.nseg - 1) * K * V * sizeof(float)) : 0;
+  return c;
+}
+
+int launch(const Args& a, bool out, unsigned blocks, int dtype, hipStream_t s) {
+  if (dtype == CET_F32)
+    launch_f32(a, out, blocks, s);
+  else if (dtype == CET_F16)
+    launch_f16(a, out, blocks, s);
+  else
+    launch_bf16(a, out, blocks, s);
+  CET_HIP(hipGetLastError());
+  return CET_OK;
+}
+
+// One pass of the recurrence over packed operands.
+int pass(Args a, const Cut& c, int dtype, hipStream_t s) {
+  a.nslice = c.nslice;
+  a.nseg = c.nseg;
+  a.seg_len = c.seg_len;
+  a.vec_o = a.V % 4 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
+  const long bh = (long)a.B * a.H;
+  if (c.nseg > 1) {
+    if (const int rc = launch(a, false, (unsigned)(bh * (c.nseg - 1) * c.nslice), dtype, s)) return rc;
+    join_segments<<<(unsigned)((bh * a.K * a.V + 255) / 256), 256, 0, s>>>(a);
+    CET_HIP(hipGetLastError());
+  }
+  return launch(a, true, (unsigned)(bh * c.nseg * c.nslice), dtype, s);
+}
+
+bool bad_desc(const cet_linattn_desc* d) {
+  return !d || d->dtype < CET_F32 || d->dtype > CET_F16 || d->B < 0 || d->T < 0 || d->H < 0 || d->K < 1 || d->V < 1 ||
+         d->T > (1 << 30) || !std::isfinite(d->scale);
+}
+bool too_large(const cet_linattn_desc& d) {
+  return d.K > 256 || d.V > 256 || (double)d.B * d.H * std::max(d.K, d.V) > 2e9 * 4 || (double)d.B * d.H * 16 > 2e9;
+}
+Strides contiguous(const cet_linattn_desc& d, int D) { return Strides{(long)d.T * d.H * D, (long)d.H * D, D}; }
+
+template <typename IO, int W>
+void launch_step(const Step<IO>& a0, int cus, hipStream_t s) {
+  Step<IO> a = a0;
+  const long heads = (long)a.B * a.H;
+  // columns in as few workgroups as keep every CU at two or more
+  int tx = 64;
+  while (tx > 4 && (tx * W / 2 >= a.V || heads * ((a.V + tx * W - 1) / (tx * W)) < 2L * cus)) tx /= 2;
+  a.nslice = (a.V + tx * W - 1) / (tx * W);
+  const unsigned blocks = (unsigned)(heads * a.nslice);
+  switch (tx) {
+    case 64: step<IO, 64, W><<<blocks, 256, 0, s>>>(a); break;
+    case 32: step<IO, 32, W><<<blocks, 256, 0, s>>>(a); break;
+    case 16: step<IO, 16, W><<<blocks, 256, 0, s>>>(a); break;
+    case 8: step<IO, 8, W><<<blocks, 256, 0, s>>>(a); break;
+    default: step<IO, 4, W><<<blocks, 256, 0, s>>>(a);
+  }
+}
+
+template <typename IO>
+void run_step(int B, int H, int K, int V, const int64_t* qs, const int64_t* ks, const int64_t* vs, const void* q,
+              const void* k, const void* v, const float* log_decay, float scale, const float* in, float* out, int rows,
+              const void* slots, int slots64, void* o, hipStream_t s) {
+  const Step<IO> a{static_cast<const IO*>(q), static_cast<const IO*>(k), static_cast<const IO*>(v), qs[0], qs[1], ks[0], ks[1],
+                   vs[0], vs[1], log_decay, in, out, slots, static_cast<IO*>(o), B, H, K, V, rows, slots64, 1, scale};
+  const bool wide = V % 4 == 0 && ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  if (wide)
+    launch_step<IO, 4>(a, cu_count(), s);
+  else
+    launch_step<IO, 1>(a, cu_count(), s);
+}
+
+}  // namespace
+}  // namespace la
+}  // namespace cet
+
+using namespace cet;
+using namespace cet::la;
+
+extern "C" {
+
+size_t cet_linear_attention_workspace(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
+                                      const void* d_o, int backward) {
+  if (bad_desc(d) || too_large(*d)) return 0;
+  const int cus = cu_count();
+  size_t n = Operand(q, d->q, d->K, *d).copy + Operand(k, d->k, d->K, *d).copy + Operand(v, d->v, d->V, *d).copy;
+  size_t states = cut(*d, d->K, d->V, cus).ws;
+  if (backward) {
+    n += Operand(d_o, d->d_o, d->V, *d).copy;
+    states = std::max(states, cut(*d, d->V, d->K, cus).ws);
+  }
+  return n + states;
+}
+
+int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
+                         const float* initial, const void* lengths, void* o, float* final_state, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  if (bad_desc(d)) return CET_ERR_INVALID_ARG;
+  if (too_large(*d)) return CET_ERR_UNSUPPORTED;
+  if ((long)d->B * d->H == 0) return CET_OK;
+  if (!log_decay || (d->T > 0 && (!q || !k || !v || !o))) return CET_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return CET_ERR_INVALID_ARG;
+  const size_t need = cet_linear_attention_workspace(d, q, k, v, nullptr, 0);
+  if (need > workspace_bytes || (need && !workspace)) return CET_ERR_INVALID_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  Operand oq(q, d->q, d->K, *d), ok(k, d->k, d->K, *d), ov(v, d->v, d->V, *d);
+  for (Operand* x : {&oq, &ok, &ov})
+    if (const int rc = x->pack(*d, ws, s)) return rc;
+  Args a{};
+  a.q = oq.p, a.k = ok.p, a.v = ov.p, a.o = o;
+  a.sq = oq.s, a.sk = ok.s, a.sv = ov.s, a.so = contiguous(*d, d->V);
+  a.init = initial, a.fin = final_state;
+  a.init_k = a.fin_k = d->V, a.init_v = a.fin_v = 1;
+  a.log_decay = log_decay, a.lengths = lengths, a.lengths64 = d->lengths64;
+  a.ws = reinterpret_cast<float*>(ws);
+  a.B = d->B, a.T = d->T, a.H = d->H, a.K = d->K, a.V = d->V;
+  a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
+  return pass(a, cut(*d, d->K, d->V, cu_count()), d->dtype, s);
+}
+
+int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
+                                  const float* log_decay, const float* initial, const void* lengths, const void* d_o,
+                                  const float* d_final, void* dq, void* dk, void* dv, float* d_initial, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  if (bad_desc(d)) return CET_ERR_INVALID_ARG;
+  if (too_large(*d)) return CET_ERR_UNSUPPORTED;
+  if ((long)d->B * d->H == 0) return CET_OK;
+  if (!log_decay || (d->T > 0 && (!q || !k || !v || !d_o || !dq || !dk || !dv))) return CET_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return CET_ERR_INVALID_ARG;
+  const size_t need = cet_linear_attention_workspace(d, q, k, v, d_o, 1);
+  if (need > workspace_bytes || (need && !workspace)) return CET_ERR_INVALID_ARG;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  Operand oq(q, d->q, d->K, *d), ok(k, d->k, d->K, *d), ov(v, d->v, d->V, *d), og(d_o, d->d_o, d->V, *d);
+  for (Operand* x : {&oq, &ok, &ov, &og})
+    if (const int rc = x->pack(*d, ws, s)) return rc;
+  const int cus = cu_count();
+  const Cut by_k = cut(*d, d->V, d->K, cus), by_v = cut(*d, d->K, d->V, cus);
+  Args a{};
+  a.log_decay = log_decay, a.lengths = lengths, a.lengths64 = d->lengths64;
+  a.ws = reinterpret_cast<float*>(ws);
+  a.B = d->B, a.T = d->T, a.H = d->H;
+  // dq: (do, v, k) forward in time, states transposed
+  a.q = og.p, a.sq = og.s, a.k = ov.p, a.sk = ov.s, a.v = ok.p, a.sv = ok.s;
+  a.o = dq, a.so = contiguous(*d, d->K);
+  a.K = d->V, a.V = d->K;
+  a.init = initial, a.init_k = 1, a.init_v = d->V;
+  a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
+  if (const int rc = pass(a, by_k, d->dtype, s)) return rc;
+  // dk: (v, do, q) backward in time, states transposed
+  a.q = ov.p, a.sq = ov.s, a.k = og.p, a.sk = og.s, a.v = oq.p, a.sv = oq.s;
+  a.o = dk;
+  a.init = d_final;
+  a.reverse = 1, a.s_inter = 1.f, a.s_intra = a.s_kv = d->scale;
+  if (const int rc = pass(a, by_k, d->dtype, s)) return rc;
+  // dv: (k, q, do) backward in time; the carry at the end is the gradient of the first state
+  a.q = ok.p, a.sq = ok.s, a.k = oq.p, a.sk = oq.s, a.v = og.p, a.sv = og.s;
+  a.o = dv, a.so = contiguous(*d, d->V);
+  a.K = d->K, a.V = d->V;
+  a.init_k = a.fin_k = d->V, a.init_v = a.fin_v = 1;
+  a.fin = d_initial;
+  return pass(a, by_v, d->dtype, s);
+}
+
+int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64_t* q_strides, const int64_t* k_strides,
+                              const int64_t* v_strides, const void* q, const void* k, const void* v,
+                              const float* log_decay, float scale, const float* state_in, float* state_out, int rows,
+                              const void* slots, int slots64, void* o, void* stream) {
+  if (dtype < CET_F32 || dtype > CET_F16 || B < 0 || H < 0 || K < 1 || V < 1 || rows < 0 || !std::isfinite(scale))
+    return CET_ERR_INVALID_ARG;
+  if (K > 256 || V > 256 || (double)B * H * V > 2e9) return CET_ERR_UNSUPPORTED;
+  if ((long)B * H == 0) return CET_OK;
+  if (!q_strides || !k_strides || !v_strides || !q || !k || !v || !log_decay || !o) return CET_ERR_INVALID_ARG;
+  if (rows > 0 && (!state_in || !state_out)) return CET_ERR_INVALID_ARG;
+  if (slots ? state_in != state_out : rows < B) return CET_ERR_INVALID_ARG;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(state_in), z = reinterpret_cast<uintptr_t>(state_out);
+  const uintptr_t bytes = (uintptr_t)B * H * K * V * sizeof(float);
+  if (a != z && (a < z ? z - a : a - z) < bytes) return CET_ERR_INVALID_ARG;  // half overlapping
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dtype == CET_F32)
+    run_step<float>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, o, s);
+  else if (dtype == CET_F16)
+    run_step<_Float16>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, o, s);
+  else
+    run_step<__bf16>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, o, s);
+  CET_HIP(hipGetLastError());
+  return CET_OK;
+}
+
+}  // extern "C"

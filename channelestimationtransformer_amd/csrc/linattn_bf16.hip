@@ -1,0 +1,15 @@
+// Linear attention: the chunk kernels for __bf16 tensors.
+#include "linattn.h"
+
+namespace cet {
+namespace la {
+
+void launch_bf16(const Args& a, bool out, unsigned blocks, hipStream_t s) {
+  if (out)
+    launch<__bf16, true>(a, blocks, s);
+  else
+    launch<__bf16, false>(a, blocks, s);
+}
+
+}  // namespace la
+}  // namespace cet

@@ -5,6 +5,8 @@ never allocates results) and enqueues the HIP kernel on torch's current stream t
 ctypes binding. Handles are created and owned by the host-side model objects.
 """
 import ctypes
+import math
+from typing import Optional
 
 import torch
 
@@ -280,3 +282,199 @@ def lmmse_grid(y: torch.Tensor, h_hat: torch.Tensor, err_var: torch.Tensor, no: 
 def _(y, h_hat, err_var, no, no_scalar, no_mode, data_sym, eff_sc):
     B, Ns, n = y.shape[0], h_hat.shape[2], data_sym.numel() * h_hat.shape[4]
     return y.new_empty((B, Ns, n, 2)), y.new_empty((B, Ns, n))
+
+
+# -- sequence operators -----------------------------------------------------------------------
+
+_SEQ_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _seq_check(name, t, dtype, *shape):
+    """A tensor of the call's type and of this shape (None = any size in that position) whose last axis
+    is contiguous."""
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(s is not None and int(d) != int(s) for d, s in zip(t.shape, shape)):
+        raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _seq_type(t):
+    if t.dtype not in _SEQ_TYPES:
+        raise RuntimeError(f"float32, bfloat16 or float16 tensors are served, got {t.dtype}")
+    return _SEQ_TYPES[t.dtype]
+
+
+def _index(name, t, n):
+    """An int32 / int64 [n] table -> (contiguous, holds int64)."""
+    if t.dtype not in (torch.int32, torch.int64) or t.dim() != 1 or t.shape[0] != n:
+        raise RuntimeError(f"{name} must be int32 or int64 [{n}], got {t.dtype} {list(t.shape)}")
+    return t.contiguous(), int(t.dtype == torch.int64)
+
+
+def _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o=None):
+    """Checked operands of the linear attention calls and their descriptor."""
+    dev = _dev_check(*(t for t in (q, k, v, log_decay, initial_state, lengths, d_o) if t is not None))
+    code = _seq_type(q)
+    q = _seq_check("q", q, q.dtype, None, None, None, None)
+    B, T, H, K = q.shape
+    k = _seq_check("k", k, q.dtype, B, T, H, K)
+    v = _seq_check("v", v, q.dtype, B, T, H, None)
+    V = v.shape[3]
+    if not (1 <= K <= 256 and 1 <= V <= 256):
+        raise RuntimeError(f"head sizes from 1 to 256 are served, got K = {K}, V = {V}")
+    if not math.isfinite(scale):
+        raise RuntimeError(f"scale must be finite, got {scale}")
+    log_decay = _f32("log_decay", log_decay, H)
+    if initial_state is not None:
+        initial_state = _f32("initial_state", initial_state, B, H, K, V)
+    wide = 0
+    if lengths is not None:
+        lengths, wide = _index("lengths", lengths, B)
+    if d_o is not None:
+        d_o = _seq_check("d_o", d_o, q.dtype, B, T, H, V)
+    d = _cabi.LinattnDesc(code, B, T, H, K, V, wide, scale)
+    for name, t in (("q", q), ("k", k), ("v", v), ("d_o", d_o)):
+        if t is not None:
+            getattr(d, name)[:] = t.stride()[:3]
+    return dev, d, q, k, v, log_decay, initial_state, lengths, d_o
+
+
+def _workspace(n, dev):
+    return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+
+
+@torch.library.custom_op("cet::linear_attention", mutates_args=())
+def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
+                     initial_state: Optional[torch.Tensor] = None,
+                     lengths: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """q, k [B,T,H,K], v [B,T,H,V] -> o [B,T,H,V], state float32 [B,H,K,V]."""
+    dev, d, q, k, v, log_decay, s0, lengths, _ = _linattn(q, k, v, log_decay, scale, initial_state, lengths)
+    o = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
+    state = torch.empty((d.B, d.H, d.K, d.V), dtype=torch.float32, device=dev)
+    L = _cabi.lib()
+    with torch.cuda.device(dev):
+        n = L.cet_linear_attention_workspace(d, _ptr(q), _ptr(k), _ptr(v), None, 0)
+        ws = _workspace(n, dev)
+        rc = L.cet_linear_attention(d, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(s0), _ptr(lengths), _ptr(o),
+                                    _ptr(state), _ptr(ws), n, _cabi.current_stream_ptr(dev))
+    _cabi.check(rc, "cet_linear_attention")
+    return o, state
+
+
+@linear_attention.register_fake
+def _(q, k, v, log_decay, scale, initial_state=None, lengths=None):
+    B, T, H, K = q.shape
+    return q.new_empty((B, T, H, v.shape[3])), q.new_empty((B, H, K, v.shape[3]), dtype=torch.float32)
+
+
+@torch.library.custom_op("cet::linear_attention_backward", mutates_args=())
+def linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
+                              initial_state: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
+                              d_o: torch.Tensor, d_state: Optional[torch.Tensor], want_initial: bool
+                              ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> dq, dk, dv, d_initial (empty unless `want_initial`)."""
+    dev, d, q, k, v, log_decay, s0, lengths, d_o = _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o)
+    if d_state is not None:
+        _dev_check(q, d_state)
+        d_state = _f32("d_state", d_state, d.B, d.H, d.K, d.V)
+    dq, dk = (torch.empty((d.B, d.T, d.H, d.K), dtype=q.dtype, device=dev) for _ in range(2))
+    dv = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
+    ds = torch.empty((d.B, d.H, d.K, d.V) if want_initial else (0,), dtype=torch.float32, device=dev)
+    L = _cabi.lib()
+    with torch.cuda.device(dev):
+        n = L.cet_linear_attention_workspace(d, _ptr(q), _ptr(k), _ptr(v), _ptr(d_o), 1)
+        ws = _workspace(n, dev)
+        rc = L.cet_linear_attention_backward(d, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(s0), _ptr(lengths),
+                                             _ptr(d_o), _ptr(d_state), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(ws),
+                                             n, _cabi.current_stream_ptr(dev))
+    _cabi.check(rc, "cet_linear_attention_backward")
+    return dq, dk, dv, ds
+
+
+@linear_attention_backward.register_fake
+def _(q, k, v, log_decay, scale, initial_state, lengths, d_o, d_state, want_initial):
+    B, T, H, K = q.shape
+    shape = (B, H, K, v.shape[3]) if want_initial else (0,)
+    return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), q.new_empty(shape, dtype=torch.float32))
+
+
+def _linattn_setup(ctx, inputs, output):
+    q, k, v, log_decay, scale, initial_state, lengths = inputs
+    if ctx.needs_input_grad[3]:
+        raise RuntimeError("log_decay is a constant of linear_attention: it has no gradient (detach it)")
+    ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+    ctx.scale = scale
+    ctx.set_materialize_grads(False)
+
+
+def _linattn_backward(ctx, d_o, d_state):
+    q, k, v, log_decay, s0, lengths = ctx.saved_tensors
+    if d_o is None:
+        if d_state is None:
+            return (None,) * 7
+        d_o = q.new_zeros((*q.shape[:3], v.shape[3]))
+    want = s0 is not None and ctx.needs_input_grad[5]
+    dq, dk, dv, ds = torch.ops.cet.linear_attention_backward(q, k, v, log_decay, ctx.scale, s0, lengths, d_o, d_state, want)
+    return dq, dk, dv, None, None, ds if want else None, None
+
+
+linear_attention.register_autograd(_linattn_backward, setup_context=_linattn_setup)
+
+
+def _step(q, k, v, log_decay, state, out_state, scale, slots):
+    dev = _dev_check(*(t for t in (q, k, v, log_decay, state, slots) if t is not None))
+    code = _seq_type(q)
+    q = _seq_check("q", q, q.dtype, None, None, None)
+    B, H, K = q.shape
+    k = _seq_check("k", k, q.dtype, B, H, K)
+    v = _seq_check("v", v, q.dtype, B, H, None)
+    V = v.shape[2]
+    if not (1 <= K <= 256 and 1 <= V <= 256):
+        raise RuntimeError(f"head sizes from 1 to 256 are served, got K = {K}, V = {V}")
+    log_decay = _f32("log_decay", log_decay, H)
+    o = torch.empty((B, H, V), dtype=q.dtype, device=dev)
+    wide = 0
+    if slots is not None:
+        slots, wide = _index("slots", slots, B)
+    strides = [(ctypes.c_int64 * 2)(*t.stride()[:2]) for t in (q, k, v)]
+    with torch.cuda.device(dev):
+        rc = _cabi.lib().cet_linear_attention_step(
+            code, B, H, K, V, *strides, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), scale, _ptr(state), _ptr(out_state),
+            state.shape[0], _ptr(slots), wide, _ptr(o), _cabi.current_stream_ptr(dev))
+    _cabi.check(rc, "cet_linear_attention_step")
+    return o
+
+
+@torch.library.custom_op("cet::linear_attention_step", mutates_args=())
+def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                          state: torch.Tensor, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """q, k [B,H,K], v [B,H,V], state float32 [B,H,K,V] -> o [B,H,V], the next state."""
+    if q.dim() != 3 or v.dim() != 3:
+        raise RuntimeError(f"q, k, v must be [B, H, features], got {list(q.shape)}, {list(v.shape)}")
+    state = _f32("state", state, q.shape[0], q.shape[1], q.shape[2], v.shape[2])
+    out = torch.empty_like(state)
+    return _step(q, k, v, log_decay, state, out, scale, None), out
+
+
+@linear_attention_step.register_fake
+def _(q, k, v, log_decay, state, scale):
+    return v.new_empty(v.shape), state.new_empty(state.shape)
+
+
+@torch.library.custom_op("cet::linear_attention_step_", mutates_args=("state",))
+def linear_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+                           state: torch.Tensor, scale: float, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The same with the state (with `slots`: a pool of them) updated in place."""
+    if q.dim() != 3 or v.dim() != 3:
+        raise RuntimeError(f"q, k, v must be [B, H, features], got {list(q.shape)}, {list(v.shape)}")
+    want = (None if slots is not None else q.shape[0], q.shape[1], q.shape[2], v.shape[2])
+    if state.dtype != torch.float32 or not state.is_contiguous() or state.dim() != 4 or any(
+            w is not None and s != w for s, w in zip(state.shape, want)):
+        raise RuntimeError(f"state must be contiguous float32 {list(want)}, got {state.dtype} {list(state.shape)}")
+    return _step(q, k, v, log_decay, state, state, scale, slots)
+
+
+@linear_attention_step_.register_fake
+def _(q, k, v, log_decay, state, scale, slots=None):
+    return v.new_empty(v.shape)

@@ -297,6 +297,63 @@ int cet_nmse_sums(const float* pred, const float* truth, double* sums, long B, i
  * All three arrays 8-byte aligned (CET_ERR_INVALID_ARG otherwise). */
 int cet_qpsk_bit_errors(const float* x_hat, const float* x_true, double* out, long N, void* stream);
 
+/* ---- sequence operators -------------------------------------------------------------------
+ * Building blocks of predictors over histories of any length (the Transformer above holds 48 slots):
+ * beside its fused attention and the recurrent rollouts, linear attention with a decay per head, whose
+ * state of fixed size is carried from slot to slot.
+ * Tensors are float32, bfloat16 or float16 (`dtype`, all of one call the same); sums, states and decays
+ * are float32. Strides are in elements; the innermost axis is always contiguous. Everything else is
+ * as above: caller-owned device buffers, nothing allocated, enqueued on `stream`, no synchronisation. */
+
+enum { CET_F32 = 0, CET_BF16 = 1, CET_F16 = 2 };
+
+/* Sizes and layouts of linear attention over B sequences of at most T slots, H heads, K features of
+ * queries and keys and V of values per head (1 <= K, V <= 256). Strides: {sequence, slot, head}. */
+typedef struct cet_linattn_desc {
+  int32_t dtype, B, T, H, K, V;
+  int32_t lengths64; /* `lengths` holds int64, not int32 */
+  float scale;       /* factor of the queries */
+  int64_t q[3], k[3], v[3];
+  int64_t d_o[3];    /* backward only */
+} cet_linattn_desc;
+
+/* Bytes of workspace that the forward call (backward = 0) or the backward call (1) on these operands
+ * needs (they depend on the pointers' alignment: operands whose rows do not start on 16 bytes are copied
+ * into it); 0 is a valid answer. d_o may be NULL for the forward call. */
+size_t cet_linear_attention_workspace(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
+                                      const void* d_o, int backward);
+
+/* S_t = exp(log_decay[h]) S_{t-1} + k_t^T v_t, o_t = scale q_t S_t for t < lengths[b] (values outside
+ * [0, T] are taken as the nearer end; NULL: T everywhere); o is zero from there on.
+ * log_decay: device [H] float32, <= 0 for a state that fades (minus infinity: no memory).
+ * initial, final: device [B,H,K,V] float32, the state before the first and after the last slot in use;
+ * either may be NULL (zero; not wanted). o: device [B,T,H,V] contiguous, every element is written.
+ * Slots of q, k and v at or behind lengths[b] are not read. The workspace is 16-byte aligned and used by
+ * this call until it has run on the stream. */
+int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
+                         const float* log_decay, const float* initial, const void* lengths, void* o,
+                         float* final_state, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of the call above from d_o (strides d->d_o) and d_final (NULL: zero): dq, dk [B,T,H,K] and
+ * dv [B,T,H,V] contiguous, zero at and behind lengths[b]; d_initial [B,H,K,V] (NULL: not wanted). The
+ * decay is a constant. */
+int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
+                                  const float* log_decay, const float* initial, const void* lengths,
+                                  const void* d_o, const float* d_final, void* dq, void* dk, void* dv,
+                                  float* d_initial, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One slot of B streams: q, k [B,H,K], v [B,H,V] (strides {stream, head} in elements), o [B,H,V]
+ * contiguous. state_in, state_out: device float32 [rows,H,K,V], the same array (updated in place) or
+ * disjoint ones. slots == NULL: stream b owns row b (rows >= B). With slots (device [B] int32, or int64
+ * where slots64) the arrays are the same and stream b owns row slots[b]; a negative slot is an idle
+ * stream (its o is zero), and a slot beyond the array or one that an earlier stream of the call already
+ * has gives an o of NaN and leaves the state alone. */
+int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64_t* q_strides,
+                              const int64_t* k_strides, const int64_t* v_strides, const void* q,
+                              const void* k, const void* v, const float* log_decay, float scale,
+                              const float* state_in, float* state_out, int rows, const void* slots,
+                              int slots64, void* o, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,80 @@
+"""Refusals of the sequence operators and their C entry points; nothing here launches a kernel."""
+import ctypes
+
+import pytest
+import torch
+
+import channelestimationtransformer_amd as cet
+from channelestimationtransformer_amd import _cabi
+
+
+def desc(**kw):
+    d = _cabi.LinattnDesc(0, 2, 8, 2, 16, 16, 0, 0.25)
+    for n in ("q", "k", "v", "d_o"):
+        getattr(d, n)[:] = (256, 32, 16)
+    for n, v in kw.items():
+        setattr(d, n, v)
+    return d
+
+
+P = 4096  # a non-null, aligned address that no refused call may touch
+
+
+def test_linear_attention_refuses_cpu_tensors_and_gradients_of_the_decay():
+    q, g = torch.zeros(2, 4, 2, 8), torch.zeros(2)
+    with pytest.raises(RuntimeError, match="GPU"):
+        cet.linear_attention(q, q, q, g)
+    with pytest.raises(RuntimeError, match="GPU"):
+        cet.linear_attention_step(q[:, 0], q[:, 0], q[:, 0], g, torch.zeros(2, 2, 8, 8))
+    with pytest.raises(RuntimeError, match="constant"):
+        cet.linear_attention(q, q, q, g.requires_grad_())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        cet.linear_attention_step(q[:, 0].requires_grad_(), q[:, 0], q[:, 0], g.detach(), torch.zeros(2, 2, 8, 8))
+
+
+@pytest.mark.parametrize("change, code", [
+    ({"dtype": 3}, 1), ({"dtype": -1}, 1), ({"B": -1}, 1), ({"T": -1}, 1), ({"K": 0}, 1), ({"V": 0}, 1), ({"H": -1}, 1),
+    ({"T": (1 << 30) + 1}, 1), ({"scale": float("nan")}, 1), ({"scale": float("inf")}, 1), ({"K": 257}, 2), ({"V": 300}, 2),
+    ({"B": 1 << 20, "H": 1 << 10}, 2)])
+def test_linear_attention_descriptors(change, code):
+    L = _cabi.lib()
+    d = desc(**change)
+    assert L.cet_linear_attention_workspace(d, P, P, P, P, 1) == 0
+    assert L.cet_linear_attention(d, P, P, P, P, None, None, P, None, P, 1 << 30, None) == code
+    assert L.cet_linear_attention_backward(d, P, P, P, P, None, None, P, None, P, P, P, None, P, 1 << 30, None) == code
+
+
+def test_linear_attention_pointers():
+    L = _cabi.lib()
+    for hole in range(4):  # q, k, v, log_decay
+        p = [P] * 4
+        p[hole] = None
+        assert L.cet_linear_attention(desc(), *p, None, None, P, None, None, 0, None) == 1
+    assert L.cet_linear_attention(desc(), P, P, P, P, None, None, None, None, None, 0, None) == 1  # o
+    assert L.cet_linear_attention(desc(), P, P, P, P, None, None, P, None, P + 8, 1 << 20, None) == 1  # workspace off 16 bytes
+    assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, None, 0, None) == 1  # copy without workspace
+    n = L.cet_linear_attention_workspace(desc(), P + 4, P, P, None, 0)
+    assert n >= 2 * 8 * 2 * 16 * 4
+    assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, P, n - 1, None) == 1
+    assert L.cet_linear_attention(desc(B=0), None, None, None, None, None, None, None, None, None, 0, None) == 0
+    for hole in range(8):
+        p = [P, P, P, P, None, None, P, None, P, P, P]
+        at = [0, 1, 2, 3, 6, 8, 9, 10][hole]
+        p[at] = None
+        assert L.cet_linear_attention_backward(desc(), *p, None, None, 0, None) == 1
+    assert L.cet_linear_attention(None, P, P, P, P, None, None, P, None, None, 0, None) == 1
+
+
+def test_step_arguments():
+    L = _cabi.lib()
+    st = (ctypes.c_int64 * 2)(32, 16)
+
+    def call(dtype=0, B=2, H=2, K=16, V=16, q=P, k=P, v=P, g=P, scale=0.25, a=P, z=P, rows=2, slots=None, o=P):
+        return L.cet_linear_attention_step(dtype, B, H, K, V, st, st, st, q, k, v, g, scale, a, z, rows, slots, 0, o, None)
+
+    for bad in ({"dtype": 4}, {"B": -1}, {"K": 0}, {"V": 0}, {"q": None}, {"k": None}, {"v": None}, {"g": None}, {"a": None}, {"z": None},
+                {"o": None}, {"rows": 1}, {"rows": -1}, {"scale": float("nan")}, {"slots": P, "z": P + (1 << 20)}, {"z": P + 64},
+                {"a": P + 64}):
+        assert call(**bad) == 1, bad
+    assert call(K=300) == 2 and call(V=257) == 2
+    assert call(B=0, q=None) == 0
