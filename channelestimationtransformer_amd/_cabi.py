@@ -22,7 +22,7 @@ EXPORTS = (
     "cet_rnn_blob_size", "cet_rnn_create", "cet_rnn_rollout", "cet_rnn_select", "cet_rnn_rollout_static", "cet_lmmse", "cet_lmmse_direct",
     "cet_lmmse_llr", "cet_lmmse_block", "cet_lmmse_block_llr", "cet_lmmse_grid", "cet_ls_nn", "cet_nmse_sums", "cet_qpsk_bit_errors",
     "cet_linear_attention_workspace", "cet_linear_attention", "cet_linear_attention_backward",
-    "cet_linear_attention_step",
+    "cet_linear_attention_step", "cet_rotary",
 )
 
 
@@ -41,6 +41,12 @@ class LinattnDesc(ctypes.Structure):
     """Mirror of `cet_linattn_desc`."""
     _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "T", "H", "K", "V", "lengths64")] + [
         ("scale", ctypes.c_float)] + [(n, ctypes.c_int64 * 3) for n in ("q", "k", "v", "d_o")]
+
+
+class RotaryDesc(ctypes.Structure):
+    """Mirror of `cet_rotary_desc`."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "T", "Hq", "Hk", "D", "pairs", "interleaved", "positions64")] + [
+        ("gain", ctypes.c_float), ("q", ctypes.c_int64 * 3), ("k", ctypes.c_int64 * 3), ("pos", ctypes.c_int64 * 2)]
 
 
 _lib = None
@@ -100,6 +106,7 @@ def lib():
     L.cet_linear_attention.argtypes = [desc] + [vp] * 9 + [ctypes.c_size_t, vp]
     L.cet_linear_attention_backward.argtypes = [desc] + [vp] * 13 + [ctypes.c_size_t, vp]
     L.cet_linear_attention_step.argtypes = [ip] * 5 + [vp] * 7 + [ctypes.c_float, vp, vp, ip, vp, ip, vp, vp]
+    L.cet_rotary.argtypes = [ctypes.POINTER(RotaryDesc)] + [vp] * 4 + [ip] + [vp] * 3
     for name in EXPORTS:
         getattr(L, name)  # AttributeError here means header and library disagree
     _lib = L

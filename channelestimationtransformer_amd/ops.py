@@ -478,3 +478,69 @@ def linear_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
 @linear_attention_step_.register_fake
 def _(q, k, v, log_decay, state, scale, slots=None):
     return v.new_empty(v.shape)
+
+
+@torch.library.custom_op("cet::rotary", mutates_args=())
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool,
+           gain: float, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """q [B,T,Hq,D], k [B,T,Hk,D] or None, positions int32 / int64 [T] or [B,T], inv_freq float64 [pairs]
+    -> the turned q and k (empty without k)."""
+    dev = _dev_check(*(t for t in (q, k, positions, inv_freq) if t is not None))
+    code = _seq_type(q)
+    q = _seq_check("q", q, q.dtype, None, None, None, None)
+    B, T, Hq, D = q.shape
+    if k is not None:
+        k = _seq_check("k", k, q.dtype, B, T, None, D)
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 1 <= inv_freq.shape[0] <= D // 2:
+        raise RuntimeError(f"inv_freq must be float64 [pairs] with 1 <= pairs <= D / 2, got {inv_freq.dtype} "
+                           f"{list(inv_freq.shape)} for D = {D}")
+    inv_freq = inv_freq.contiguous()
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((T,), (B, T)):
+        raise RuntimeError(f"positions must be int32 or int64 [{T}] or [{B}, {T}], got {positions.dtype} {list(positions.shape)}")
+    if not math.isfinite(gain):
+        raise RuntimeError(f"gain must be finite, got {gain}")
+    Hk = 0 if k is None else k.shape[2]
+    if D > 1024:
+        raise RuntimeError(f"heads of up to 1024 features are served, got D = {D}")
+    d = _cabi.RotaryDesc(code, B, T, Hq, Hk, D, inv_freq.shape[0], int(interleaved), int(positions.dtype == torch.int64), gain)
+    d.q[:] = q.stride()[:3]
+    if k is not None:
+        d.k[:] = k.stride()[:3]
+    d.pos[:] = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
+    ko = torch.empty((B, T, Hk, D) if k is not None else (0,), dtype=q.dtype, device=dev)
+    with torch.cuda.device(dev):
+        rc = _cabi.lib().cet_rotary(d, _ptr(q), _ptr(k), _ptr(positions), _ptr(inv_freq), int(inverse), _ptr(qo), _ptr(ko),
+                                    _cabi.current_stream_ptr(dev))
+    _cabi.check(rc, "cet_rotary")
+    return qo, ko
+
+
+@rotary.register_fake
+def _(q, k, positions, inv_freq, interleaved, gain, inverse):
+    return q.new_empty(q.shape), q.new_empty(k.shape if k is not None else (0,))
+
+
+def _rotary_setup(ctx, inputs, output):
+    q, k, positions, inv_freq, ctx.interleaved, ctx.gain, ctx.inverse = inputs
+    ctx.save_for_backward(positions, inv_freq)
+    ctx.set_materialize_grads(False)
+
+
+def _rotary_backward(ctx, dq, dk):
+    positions, inv_freq = ctx.saved_tensors
+    if not ctx.needs_input_grad[1]:
+        dk = None
+    if not ctx.needs_input_grad[0]:
+        dq = None
+    turn = lambda a, b: torch.ops.cet.rotary(a, b, positions, inv_freq, ctx.interleaved, ctx.gain, not ctx.inverse)  # noqa: E731
+    if dq is None:
+        dk = turn(dk, None)[0] if dk is not None else None
+    elif dk is None:
+        dq = turn(dq, None)[0]
+    else:
+        dq, dk = turn(dq, dk)
+    return dq, dk, None, None, None, None, None
+
+
+rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)

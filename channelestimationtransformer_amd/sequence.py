@@ -1,12 +1,13 @@
 """Sequence operators for predictors over histories of any length.
 
 The Transformer predictors hold at most 48 slots in one tile and the recurrent ones roll a dense state
-forward; these are the blocks between the two. `linear_attention` reads a history in chunks and leaves
-a state of fixed size per head, `linear_attention_step` carries that state on slot by slot.
+forward; these are the blocks between the two. `rotary` gives queries and keys their slots' positions
+(the Transformer adds a fixed table of sinusoids), `linear_attention` reads a history in chunks and
+leaves a state of fixed size per head, `linear_attention_step` carries that state on slot by slot.
 
 All take CUDA (ROCm) tensors of one type (float32, bfloat16 or float16), run on the current stream
-and raise on anything the kernels do not serve. `linear_attention` has gradients (not twice
-differentiable).
+and raise on anything the kernels do not serve. `rotary` and `linear_attention` have gradients
+(`rotary`'s can be differentiated again).
 """
 import math
 
@@ -50,3 +51,52 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None, slots=None, inp
     if slots is not None or inplace:
         return torch.ops.cet.linear_attention_step_(q, k, v, log_decay, state, float(scale), slots), state
     return torch.ops.cet.linear_attention_step(q, k, v, log_decay, state, float(scale))
+
+
+def rotary_frequencies(dim, base=10000.0, scaling="none", factor=1.0, original_length=None, turns=(32.0, 1.0), device="cuda"):
+    """Radians per slot of the dim / 2 pairs of `rotary`, base ** (-2 j / dim), and the gain to call it
+    with: (float64 [dim / 2] on `device`, float). `scaling` stretches positions that were trained on
+    `original_length` slots over `factor` times as many:
+
+    * "linear": every rate divided by `factor`;
+    * "ntk": the base times factor ** (dim / (dim - 2)), so that the slowest pair is stretched by
+      `factor` and the fastest keeps its rate;
+    * "yarn": pairs that turn more than turns[0] times within `original_length` keep their rate, those
+      below turns[1] are divided by `factor`, a linear ramp over the pairs between; gain
+      0.1 ln(factor) + 1."""
+    dim = int(dim)
+    if dim < 2 or dim % 2:
+        raise RuntimeError(f"dim must be even and positive, got {dim}")
+    if not (base > 1.0 and math.isfinite(base) and factor > 0.0 and math.isfinite(factor)):
+        raise RuntimeError(f"base must exceed 1 and factor 0, got {base}, {factor}")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        raise RuntimeError(f'scaling must be "none", "linear", "ntk" or "yarn", got {scaling!r}')
+    if scaling == "ntk":
+        base = base * factor ** (dim / max(dim - 2, 1))
+    j = torch.arange(dim // 2, dtype=torch.float64)
+    freq, gain = base ** (-2.0 * j / dim), 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "yarn":
+        if not original_length or original_length <= 0 or not turns[0] > turns[1] > 0:
+            raise RuntimeError("yarn needs original_length > 0 and turns[0] > turns[1] > 0")
+        pair = [dim * math.log(original_length / (n * 2 * math.pi)) / (2 * math.log(base)) for n in turns]
+        low, high = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), dim // 2 - 1)
+        ramp = ((j - low) / max(high - low, 0.001)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        gain = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return freq.to(device), gain
+
+
+def rotary(q, k, positions, inv_freq, layout="half", gain=1.0):
+    """Turns the pairs of q [B, T, Hq, D] and k [B, T, Hk, D] (or None) by positions * inv_freq:
+    (a, b) -> gain (a cos - b sin, a sin + b cos); returns the two turned tensors (contiguous; the
+    second None without k). `positions`: int32 or int64 [T] or [B, T], any values; `inv_freq`: float64
+    [pairs] with 2 pairs <= D (see `rotary_frequencies`); `layout`: pairs are (j, j + pairs) ("half") or
+    (2j, 2j + 1) ("interleaved"). Features behind the pairs pass through. Angles are formed in float64."""
+    if layout not in ("half", "interleaved"):
+        raise RuntimeError(f'layout must be "half" or "interleaved", got {layout!r}')
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("inv_freq is a constant of rotary: it has no gradient (detach it)")
+    a, b = torch.ops.cet.rotary(q, k, positions, inv_freq, layout == "interleaved", float(gain), False)
+    return a, (b if k is not None else None)

@@ -354,6 +354,24 @@ int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64
                               const float* state_in, float* state_out, int rows, const void* slots,
                               int slots64, void* o, void* stream);
 
+/* Rotary positions of queries [B,T,Hq,D] and keys [B,T,Hk,D] (either head count may be 0 with NULL
+ * pointers): pair j < pairs of a head is turned by position * inv_freq[j] radians and multiplied by
+ * `gain`; the features behind 2 * pairs pass through. Pairs are (j, j + pairs), or (2j, 2j + 1) where
+ * `interleaved`. Strides: {sequence, slot, head}; of the positions {sequence, slot} (0 for a shared row).
+ * Angles are formed in fp64 from the whole positions, negative ones included. */
+typedef struct cet_rotary_desc {
+  int32_t dtype, B, T, Hq, Hk, D, pairs;
+  int32_t interleaved;
+  int32_t positions64; /* positions are int64, not int32 */
+  float gain;
+  int64_t q[3], k[3], pos[2];
+} cet_rotary_desc;
+
+/* q_out, k_out: contiguous, may not overlap the inputs. inv_freq: device [pairs] float64. inverse = 1 turns the other way
+ * (the gradient of the call with inverse = 0). */
+int cet_rotary(const cet_rotary_desc* d, const void* q, const void* k, const void* positions,
+               const double* inv_freq, int inverse, void* q_out, void* k_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

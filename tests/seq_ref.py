@@ -47,3 +47,16 @@ def geometric(H):
 
 def sqrt_scale(K):
     return 1.0 / math.sqrt(K)
+
+
+def rotary(x, positions, freq, layout, gain):
+    """x [B, T, H, D] float64."""
+    P = freq.shape[0]
+    angle = (positions.double()[..., None] * freq).expand(x.shape[0], x.shape[1], P)[:, :, None]
+    c, s = gain * angle.cos(), gain * angle.sin()
+    y = x.clone()
+    ia = torch.arange(P) if layout == "half" else 2 * torch.arange(P)
+    ib = ia + (P if layout == "half" else 1)
+    y[..., ia] = x[..., ia] * c - x[..., ib] * s
+    y[..., ib] = x[..., ia] * s + x[..., ib] * c
+    return y

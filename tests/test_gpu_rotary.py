@@ -1,0 +1,175 @@
+"""Rotary positions against the float64 statement.
+
+Bound of an element of pair (a, b): cos and sin carry the fp32 rounding of the reduced angle and of the
+function (2 units of 2^-24 of 1 each, doubled for the function's own error: 4), of the gain (1) and the two
+products and the sum one each: 8 * 2^-24 of gain (|a| + |b|); then one rounding to the tensors' type.
+The angle itself is a float64 product: the oracle rounds position * rate once, the kernel that, 2 / pi and
+the product with it, 2^-53 of the angle each, and an angle off by e moves a turned value by at most
+e gain (|a| + |b|): 4 * 2^-53 |angle| more (of weight from positions of some 10^9 on)."""
+import pytest
+import torch
+
+import channelestimationtransformer_amd as cet
+import seq_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def limit(x, want, positions, freq, layout, gain, dtype):
+    P = freq.shape[0]
+    size = torch.zeros_like(x)
+    ia = torch.arange(P) if layout == "half" else 2 * torch.arange(P)
+    ib = ia + (P if layout == "half" else 1)
+    size[..., ia] = size[..., ib] = abs(gain) * (x[..., ia].abs() + x[..., ib].abs())
+    angle = torch.zeros_like(x)
+    angle[..., ia] = angle[..., ib] = (positions.double()[..., None] * freq).abs()[..., None, :].expand_as(x[..., ia])
+    return 1.01 * (ref.half_step(dtype) * want.abs() + (8 * 2.0 ** -24 + 4 * 2.0 ** -53 * angle) * size) + (1e-7 if dtype == torch.float16 else 0.0)
+
+
+def check(q, k, positions, freq, layout, gain, dtype, views=lambda t: t):
+    """q, k float64 values of the type; compares both outputs and gradients."""
+    g = torch.Generator().manual_seed(3)
+    leaves = [views(t.to(dtype).cuda()).detach().requires_grad_() for t in (q, k)]
+    outs = cet.rotary(leaves[0], leaves[1], positions.cuda(), freq.cuda(), layout=layout, gain=gain)
+    grads = [torch.randn(t.shape, generator=g).to(dtype) for t in (q, k)]
+    got = torch.autograd.grad(outs, leaves, [views(d.cuda()) for d in grads])
+    for x, o, d, b in zip((q, k), outs, grads, got):
+        for inp, res, sign in ((x, o, 1.0), (d.double(), b, -1.0)):
+            want = ref.rotary(inp, positions * int(sign), freq, layout, gain)
+            assert res.dtype == dtype and res.shape == inp.shape
+            err = (res.detach().double().cpu() - want).abs()
+            lim = limit(inp, want, positions, freq, layout, gain, dtype)
+            assert (err <= lim).all(), (float((err / lim).nan_to_num(9e9).max()), sign)
+            P = 2 * freq.shape[0]
+            assert torch.equal(res.detach().cpu()[..., P:], inp.to(dtype)[..., P:])  # what passes through
+    return outs, got
+
+
+def values(B, T, Hq, Hk, D, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(B, T, h, D, generator=g).to(dtype).double() for h in (Hq, Hk)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 2, 2), (2, 1, 8, 8, 64, 64), (3, 5, 4, 1, 7, 6), (2, 33, 2, 2, 128, 64), (1, 70, 3, 1, 80, 20),
+                                   (2, 9, 6, 2, 48, 48), (1, 4, 1, 1, 1024, 1024), (5, 257, 2, 1, 16, 8), (1, 3, 2, 1, 100, 50), (700, 3, 2, 2, 8, 8)])
+def test_against_the_definition(shape, layout, dtype):
+    B, T, Hq, Hk, D, rot = shape
+    q, k = values(B, T, Hq, Hk, D, dtype, seed=D + T)
+    freq, _ = cet.rotary_frequencies(rot, device="cpu")
+    check(q, k, torch.arange(T), freq, layout, 1.0, dtype)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_far_and_negative_positions_of_each_sequence(kind):
+    B, T = 4, 12
+    q, k = values(B, T, 2, 2, 32, torch.float32, seed=1)
+    freq, _ = cet.rotary_frequencies(32, device="cpu")
+    start = torch.tensor([0, -40, 1_000_000, 2 ** 31 - 1 - T])
+    positions = (start[:, None] + torch.arange(T)[None]).to(kind)
+    for layout in ("half", "interleaved"):
+        check(q, k, positions, freq, layout, 0.7, torch.float32)
+    if kind == torch.int64:
+        check(q, k, positions * 2 ** 20, freq, "half", 1.0, torch.float32)
+        wide = torch.zeros(B, 3 * T, dtype=kind)
+        wide[:, ::3] = positions
+        check(q, k, wide[:, ::3], freq, "half", 1.0, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(dtype):
+    q, k = values(2, 19, 3, 3, 32, dtype, seed=2)
+    freq, _ = cet.rotary_frequencies(32, device="cpu")
+    want = check(q, k, torch.arange(19), freq, "half", 1.0, dtype)
+
+    def heads_first(t):
+        return t.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def off_by_one(t):
+        room = torch.full((*t.shape[:3], t.shape[3] + 5), float("nan"), dtype=t.dtype, device="cuda")
+        room[..., 1:-4] = t
+        return room[..., 1:-4]
+
+    def spread(t):  # every second feature of a wider tensor: copied
+        return t.repeat_interleave(2, -1)[..., ::2]
+
+    for view in (heads_first, off_by_one, spread):
+        got = check(q, k, torch.arange(19), freq, "half", 1.0, dtype, views=view)
+        assert all(torch.equal(a, b) for x, y in zip(want, got) for a, b in zip(x, y))
+
+
+def test_queries_alone_no_slots_and_one_gradient():
+    q, k = values(2, 6, 3, 2, 16, torch.float32, seed=4)
+    freq, _ = cet.rotary_frequencies(16)
+    pos = torch.arange(6, device="cuda")
+    q, k = q.float().cuda(), k.float().cuda()
+    both = cet.rotary(q, k, pos, freq)
+    alone, none = cet.rotary(q, None, pos, freq)
+    assert none is None and torch.equal(alone, both[0])
+    a, b = cet.rotary(q[:, :0], k[:, :0], pos[:0], freq)
+    assert a.shape == (2, 0, 3, 16) and b.shape == (2, 0, 2, 16)
+    for leaf, keep in ((0, 0), (1, 1)):
+        x = [q.clone(), k.clone()]
+        x[leaf].requires_grad_()
+        out = cet.rotary(x[0], x[1], pos, freq)
+        d = torch.randn_like(out[keep])
+        want = cet.rotary(d, None, -pos, freq)[0]
+        got, = torch.autograd.grad(out[keep], x[leaf], d)
+        assert torch.equal(got, want)
+    # twice differentiable: the gradient of the gradient turns forward again
+    x = q.clone().requires_grad_()
+    d = torch.randn_like(q, requires_grad=True)
+    g1, = torch.autograd.grad(cet.rotary(x, None, pos, freq)[0], x, d, create_graph=True)
+    w = torch.randn_like(q)
+    g2, = torch.autograd.grad(g1, d, w)
+    assert torch.equal(g2, cet.rotary(w, None, pos, freq)[0])
+
+
+def test_gradient_against_differences():
+    """The turn is linear: a difference along a direction is the derivative, up to the fp32 bound above."""
+    q, _ = values(2, 11, 2, 1, 32, torch.float32, seed=5)
+    freq, gain = cet.rotary_frequencies(24, scaling="yarn", factor=4.0, original_length=64)
+    pos = torch.arange(11, device="cuda") * 7
+    g = torch.Generator().manual_seed(6)
+    q, d, step = q.float().cuda(), torch.randn(q.shape, generator=g).cuda(), torch.randn(q.shape, generator=g).cuda()
+    x = q.clone().requires_grad_()
+    got, = torch.autograd.grad(cet.rotary(x, None, pos, freq, gain=gain)[0], x, d)
+    up, down = (cet.rotary(q + s * step, None, pos, freq, gain=gain)[0].double() for s in (1, -1))
+    want = float(((up - down) * d.double()).sum() / 2)
+    size = float(((q.abs() + step.abs()) * d.abs()).double().sum()) * 2 * gain
+    assert abs(float((got.double() * step.double()).sum()) - want) <= 16 * 2.0 ** -24 * size
+
+
+def test_frequencies():
+    f, gain = cet.rotary_frequencies(8, device="cpu")
+    assert gain == 1.0 and torch.allclose(f, 10000.0 ** (-torch.arange(4).double() / 4), rtol=1e-15)
+    lin, _ = cet.rotary_frequencies(8, scaling="linear", factor=4.0, device="cpu")
+    assert torch.equal(lin, f / 4)
+    ntk, _ = cet.rotary_frequencies(8, scaling="ntk", factor=4.0, device="cpu")
+    assert ntk[0] == f[0] and torch.allclose(ntk[-1], f[-1] / 4, rtol=1e-12) and (ntk <= f).all()
+    f, _ = cet.rotary_frequencies(64, device="cpu")
+    yarn, gain = cet.rotary_frequencies(64, scaling="yarn", factor=8.0, original_length=4096, device="cpu")
+    turns = 4096 * f / (2 * torch.pi)
+    assert torch.equal(yarn[turns > 40], f[turns > 40]) and torch.allclose(yarn[turns < 0.8], f[turns < 0.8] / 8, rtol=1e-12)
+    assert ((yarn <= f) & (yarn >= f / 8 * (1 - 1e-12))).all() and abs(gain - 1.2079441541679836) < 1e-12
+
+
+def test_graph_replays():
+    q, k = values(2, 40, 4, 2, 64, torch.bfloat16, seed=7)
+    freq, _ = cet.rotary_frequencies(64)
+    q, k = q.bfloat16().cuda(), k.bfloat16().cuda()
+    pos = torch.arange(40, device="cuda")
+    sq, sk, sp = q.clone(), k.clone(), pos.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = cet.rotary(sq, sk, sp, freq)
+    for turn in range(4):
+        sq.copy_(q + turn)
+        sp.copy_(pos + 1000 * turn)
+        g.replay()
+        want = cet.rotary(q + turn, k, pos + 1000 * turn, freq)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])

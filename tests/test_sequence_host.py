@@ -78,3 +78,38 @@ def test_step_arguments():
         assert call(**bad) == 1, bad
     assert call(K=300) == 2 and call(V=257) == 2
     assert call(B=0, q=None) == 0
+
+
+def rot_desc(**kw):
+    d = _cabi.RotaryDesc(0, 2, 4, 2, 1, 16, 8, 0, 1, 1.0)
+    d.q[:], d.k[:], d.pos[:] = (128, 32, 16), (64, 16, 16), (0, 1)
+    for n, v in kw.items():
+        setattr(d, n, v)
+    return d
+
+
+@pytest.mark.parametrize("change, code", [
+    ({"dtype": 3}, 1), ({"B": -1}, 1), ({"T": -2}, 1), ({"Hq": -1}, 1), ({"D": 0}, 1), ({"pairs": 0}, 1), ({"pairs": 9}, 1), ({"gain": float("nan")}, 1),
+    ({"interleaved": 2}, 1), ({"D": 2048}, 2), ({"B": 1 << 20, "T": 1 << 20}, 2), ({"Hq": 1 << 20}, 2)])
+def test_rotary_descriptors(change, code):
+    assert _cabi.lib().cet_rotary(rot_desc(**change), P, P, P, P, 0, P, P, None) == code
+
+
+def test_rotary_refusals():
+    L = _cabi.lib()
+    for hole in range(6):
+        p = [P, P, P, P, P, P]
+        p[hole] = None
+        assert L.cet_rotary(rot_desc(), *p[:4], 0, *p[4:], None) == 1
+    assert L.cet_rotary(rot_desc(B=0), None, None, None, None, 0, None, None, None) == 0
+    q, f = torch.zeros(2, 4, 2, 8), torch.ones(4, dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="GPU"):
+        cet.rotary(q, q, torch.arange(4), f)
+    with pytest.raises(RuntimeError, match="layout"):
+        cet.rotary(q, q, torch.arange(4), f, layout="pairs")
+    with pytest.raises(RuntimeError, match="constant"):
+        cet.rotary(q, q, torch.arange(4), f.clone().requires_grad_())
+    for bad in ({"dim": 7}, {"dim": 0}, {"dim": 8, "base": 1.0}, {"dim": 8, "scaling": "cubic"}, {"dim": 8, "scaling": "yarn"},
+                {"dim": 8, "factor": 0.0}, {"dim": 8, "scaling": "yarn", "original_length": 64, "turns": (1.0, 2.0)}):
+        with pytest.raises(RuntimeError):
+            cet.rotary_frequencies(device="cpu", **bad)
