@@ -6,10 +6,11 @@ from .hostpipe import HostPipeline
 from .lmmse import (LMMSEEqualizer, LSChannelEstimator, ResourceGrid, StreamManagement, lmmse,
                     lmmse_llr)
 from .model import GRU, LSTM, RNN, Informer, InformerStack, InformerStack_e2e
-from .sequence import linear_attention, linear_attention_step, rotary, rotary_frequencies
+from .sequence import (gated_linear, linear_attention, linear_attention_step, rotary,
+                       rotary_frequencies)
 from .utils import LoadBatch, decoder_input, load_batch_device, real2complex
 
 __all__ = ["Informer", "InformerStack", "InformerStack_e2e", "GRU", "LSTM", "RNN", "LoadBatch",
            "real2complex", "load_batch_device", "decoder_input", "lmmse", "lmmse_llr", "LMMSEEqualizer", "LSChannelEstimator",
            "ResourceGrid", "StreamManagement", "HostPipeline",
-           "linear_attention", "linear_attention_step", "rotary", "rotary_frequencies"]
+           "gated_linear", "linear_attention", "linear_attention_step", "rotary", "rotary_frequencies"]

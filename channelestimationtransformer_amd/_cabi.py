@@ -23,6 +23,7 @@ EXPORTS = (
     "cet_lmmse_llr", "cet_lmmse_block", "cet_lmmse_block_llr", "cet_lmmse_grid", "cet_ls_nn", "cet_nmse_sums", "cet_qpsk_bit_errors",
     "cet_linear_attention_workspace", "cet_linear_attention", "cet_linear_attention_backward",
     "cet_linear_attention_step", "cet_rotary",
+    "cet_gated_linear_workspace", "cet_gated_linear", "cet_gated_linear_backward",
 )
 
 
@@ -47,6 +48,12 @@ class RotaryDesc(ctypes.Structure):
     """Mirror of `cet_rotary_desc`."""
     _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "T", "Hq", "Hk", "D", "pairs", "interleaved", "positions64")] + [
         ("gain", ctypes.c_float), ("q", ctypes.c_int64 * 3), ("k", ctypes.c_int64 * 3), ("pos", ctypes.c_int64 * 2)]
+
+
+class GatedDesc(ctypes.Structure):
+    """Mirror of `cet_gated_desc`."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "activation", "N", "D", "F")] + [
+        (n, ctypes.c_int64) for n in ("ld_x", "ld_gate", "ld_up", "ld_dy")]
 
 
 _lib = None
@@ -107,6 +114,11 @@ def lib():
     L.cet_linear_attention_backward.argtypes = [desc] + [vp] * 13 + [ctypes.c_size_t, vp]
     L.cet_linear_attention_step.argtypes = [ip] * 5 + [vp] * 7 + [ctypes.c_float, vp, vp, ip, vp, ip, vp, vp]
     L.cet_rotary.argtypes = [ctypes.POINTER(RotaryDesc)] + [vp] * 4 + [ip] + [vp] * 3
+    gated = ctypes.POINTER(GatedDesc)
+    L.cet_gated_linear_workspace.restype = ctypes.c_size_t
+    L.cet_gated_linear_workspace.argtypes = [gated, vp, vp, vp, ip]
+    L.cet_gated_linear.argtypes = [gated] + [vp] * 7 + [ctypes.c_size_t, vp]
+    L.cet_gated_linear_backward.argtypes = [gated] + [vp] * 12 + [ctypes.c_size_t, vp]
     for name in EXPORTS:
         getattr(L, name)  # AttributeError here means header and library disagree
     _lib = L

@@ -1,0 +1,407 @@
+// The gated projection of a feed-forward block and its gradients: the tiled matrix product that all of its
+// parts run on. Instantiated for float32, bfloat16 and float16 in a translation unit each.
+//
+//     g = x Wg^T + bg,   u = x Wu^T + bu,   y = act(g) * u                              (forward, one kernel)
+//     dg = dy u act'(g), du = dy act(g)       with g and u formed again                 (backward 1, one kernel)
+//     dx = [dg du] [Wg; Wu]                                                             (backward 2)
+//     [dWg; dWu] = [dg du]^T x,   [dbg; dbu] = column sums of [dg du]                   (backward 3)
+//
+// One product form: out[q][p] = sum_k P[p][k] Q[q][k], 16 x 16 tiles with p along the four registers of a
+// lane, so that a lane stores four neighbours of a row. Either operand may lie in memory with k contiguous
+// (rows) or with its own index contiguous (columns: dx reads the weights as they are, backward 3 both dh and x).
+#pragma once
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+#include <cstdint>
+
+#include "cet_internal.h"
+
+namespace cet {
+namespace gated {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+// An operand in memory. Rows (k contiguous): element (i, k) at p[i * ld + k]. Columns: at p[k * ld + i].
+// Where `split` is below the length of the divided index (the rows; with columns, k), what lies from there on
+// comes from p1, and of each part only `part` entries exist.
+struct Operand {
+  const void *p, *p1;
+  long ld, ld1;
+  int split, part;
+};
+
+struct Args {
+  Operand P, Q;
+  int np, nq, nk;     // lengths of p, q and k
+  int tiles_p, tiles_q, splits, k_per_split;
+  int F, Fp;          // features of the hidden layer, and the same rounded up to whole 16-byte pieces
+  int activation;
+  const void *bias_g, *bias_u;
+  const void* dy;
+  long ld_dy;
+  int dy_step;        // elements that a row of dy can be read at once: 4, 2 or 1
+  void *out, *out1;   // out[q][p], rows from `out_split` on to out1
+  long ld_out;
+  int out_split, out_step;
+  float* part;        // column sums per block of rows, or the splits' partial products
+};
+
+enum { FORWARD, BACKWARD, PLAIN, PARTIAL };
+
+template <typename T>
+struct Type;
+template <>
+struct Type<float> {
+  static constexpr int E = 4;
+};
+template <>
+struct Type<__bf16> {
+  static constexpr int E = 2;
+};
+template <>
+struct Type<_Float16> {
+  static constexpr int E = 2;
+};
+
+// 16 bytes of an operand: 8 or 4 values of k
+typedef uint32_t Frag __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ inline f4 mma(const Frag& a, const Frag& b, f4 c) {
+  if constexpr (__is_same(T, float)) {
+    const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], c, 0, 0, 0);
+    return c;
+  } else if constexpr (__is_same(T, __bf16)) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  } else {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+  }
+}
+
+__device__ inline unsigned lds_address(const void* p) {
+  return (unsigned)(unsigned long)(const __attribute__((address_space(3))) char*)p;
+}
+// 16 bytes per lane straight into LDS at lds + 16 * lane. In assembly so that the compiler does not hold back
+// every later LDS read until it has landed; the wait before the barrier orders it.
+__device__ inline void dma16(const void* src, unsigned lds_wave) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(src), "s"(lds_wave)
+      : "memory");
+}
+
+static __device__ const uint4 zeros = {0, 0, 0, 0};
+
+// A tile of ROWS indices by 128 bytes of k in LDS, in 16-byte pieces whose places are permuted so that the
+// reads of a wave touch every bank equally often (LDS takes the pieces in the order of the lanes, so the
+// permutation is made on the memory side).
+//   rows:    piece kc of row r (8 to a row of 128 bytes) at kc ^ (r >> 1 & 7): 16 rows of one kc are 256
+//            different bytes of the banks' 256.
+//   columns: a row of the tile is one k; piece mc at mc ^ turn(k). 16-bit values are read transposed, 8 bytes
+//            of rows 8g..8g+3 (then +4) by each group of 16 lanes; fp32 ones singly, rows 4g + r.
+template <typename T, int ROWS, int NT, bool COLS>
+struct Tile {
+  static constexpr int E = Type<T>::E, VEC = 16 / E, BK = 128 / E;
+  static constexpr int PER_ROW = COLS ? ROWS / VEC : 8, TOTAL = ROWS * 8, N = TOTAL / NT, BYTES = ROWS * 128;
+  static_assert(TOTAL % NT == 0, "whole pieces per thread");
+
+  __device__ static int turn(int k) { return E == 2 ? 2 * ((k & 3) | (k >> 3 & 1) << 2) : 4 * (k >> 2 & 3); }
+
+  // piece of memory that goes to place `at`: index i0.. of the operand, k0.. of the summed axis
+  __device__ static const char* source(const Operand& o, int at, int i0, int len, int k0, int k_end) {
+    if constexpr (!COLS) {
+      const int r = at / 8, kc = (at & 7) ^ (r >> 1 & 7), k = k0 + kc * VEC;
+      // BACKWARD and FORWARD take rows of both weights in one tile: the second half from p1
+      const bool second = o.split < ROWS && r >= o.split;
+      const int i = min(i0 + (second ? r - o.split : r), len - 1);
+      const T* p = static_cast<const T*>(second ? o.p1 : o.p) + (long)i * (second ? o.ld1 : o.ld) + k;
+      return k < k_end ? reinterpret_cast<const char*>(p) : reinterpret_cast<const char*>(&zeros);
+    } else {
+      const int kr = at / PER_ROW, mc = at % PER_ROW ^ turn(kr);
+      int k = k0 + kr;
+      const bool second = k >= o.split;
+      bool live = k < k_end;
+      if (second) k -= o.split;
+      live = live && k < o.part;
+      const int i = min(i0 + mc * VEC, (len - 1) / VEC * VEC);
+      const T* p = static_cast<const T*>(second ? o.p1 : o.p) + (long)k * (second ? o.ld1 : o.ld) + i;
+      return live ? reinterpret_cast<const char*>(p) : reinterpret_cast<const char*>(&zeros);
+    }
+  }
+  __device__ static void fetch(const Operand& o, unsigned lds, int i0, int len, int k0, int k_end) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int u = 0; u < N; ++u) dma16(source(o, u * NT + (int)threadIdx.x, i0, len, k0, k_end), lds + (u * NT + wave * 64) * 16);
+  }
+  // indices r0..r0+15 of step kk (64 bytes of k) as an operand of the matrix instructions
+  __device__ static Frag read(const char* t, int r0, int kk, int i, int g) {
+    if constexpr (!COLS) {
+      const int r = r0 + i, kc = kk * 4 + g;
+      return *reinterpret_cast<const Frag*>(t + r * 128 + ((kc ^ (r >> 1 & 7)) << 4));
+    } else if constexpr (E == 2) {
+      typedef __attribute__((address_space(3))) s4* lds_s4;
+      Frag f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = kk * 32 + 8 * g + 4 * half + (i >> 2), mc = r0 / 8 + (i >> 1 & 1);
+        const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + k * (ROWS * E) + ((mc ^ turn(k)) << 4) + (i & 1) * 8));
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+        const u2 w = __builtin_bit_cast(u2, v);
+        f[2 * half] = w[0];
+        f[2 * half + 1] = w[1];
+      }
+      return f;
+    } else {
+      Frag f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = kk * 16 + 4 * g + r, m = r0 + i;
+        f[r] = *reinterpret_cast<const uint32_t*>(t + k * (ROWS * E) + ((m / 4 ^ turn(k)) << 4) + (m & 3) * 4);
+      }
+      return f;
+    }
+  }
+};
+
+__device__ inline float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+
+enum { SILU, GELU, RELU };
+
+__device__ inline float act(int kind, float g) {
+  if (kind == SILU) return g * sigmoid(g);
+  if (kind == GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752440f));
+  return fmaxf(g, 0.f);
+}
+__device__ inline float act_slope(int kind, float g) {
+  if (kind == SILU) {
+    const float s = sigmoid(g);
+    return s * (1.f + g * (1.f - s));
+  }
+  if (kind == GELU)
+    return 0.5f * (1.f + erff(g * 0.70710678118654752440f)) + g * 0.39894228040143267794f * expf(-0.5f * g * g);
+  return g > 0.f ? 1.f : 0.f;
+}
+
+template <typename T>
+__device__ inline void store4(T* p, const f4& v, int n, int step) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  if (n >= 4 && step == 4) {
+    *reinterpret_cast<t4*>(p) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  } else if (n >= 4 && step == 2) {
+    *reinterpret_cast<t2*>(p) = t2{(T)v[0], (T)v[1]};
+    *reinterpret_cast<t2*>(p + 2) = t2{(T)v[2], (T)v[3]};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) p[r] = (T)v[r];
+  }
+}
+template <typename T>
+__device__ inline f4 load4(const T* p, int n, int step) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  f4 v = {0.f, 0.f, 0.f, 0.f};
+  if (n >= 4 && step == 4) {
+    const t4 x = *reinterpret_cast<const t4*>(p);
+    v = f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+  } else if (n >= 4 && step == 2) {
+    const t2 x = *reinterpret_cast<const t2*>(p), y = *reinterpret_cast<const t2*>(p + 2);
+    v = f4{(float)x[0], (float)x[1], (float)y[0], (float)y[1]};
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < n) v[r] = (float)p[r];
+  }
+  return v;
+}
+
+template <typename T, int BP, int BQ, int WP, int WQ, bool PC, bool QC, int KIND>
+__global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const Args a) {
+  constexpr int NT = 64 * WP * WQ, NPT = BP / WP / 16, NQT = BQ / WQ / 16;
+  constexpr bool GATED = KIND == FORWARD || KIND == BACKWARD;
+  typedef Tile<T, BP, NT, PC> TP;
+  typedef Tile<T, BQ, NT, QC> TQ;
+  constexpr int BK = TP::BK;
+  extern __shared__ __align__(1024) char lds[];  // two of [P tile | Q tile]
+  constexpr int BUF = TP::BYTES + TQ::BYTES;
+
+  // Workgroups go to the 8 XCDs in turn: each XCD is given one run of tiles, in blocks of eight rows of
+  // tiles, so that the tiles that its L2 holds are shared by the workgroups that run on it together.
+  const int total = a.tiles_p * a.tiles_q * a.splits;
+  int id = blockIdx.x;
+  {
+    const int per = total / 8, rest = total % 8, xcd = id % 8, at = id / 8;
+    id = xcd * per + min(xcd, rest) + at;
+  }
+  const int split = id / (a.tiles_p * a.tiles_q);
+  id -= split * a.tiles_p * a.tiles_q;
+  const int block = id / (8 * a.tiles_p), in = id - block * 8 * a.tiles_p;
+  const int high = min(8, a.tiles_q - 8 * block);
+  const int tq = 8 * block + in % high, tp = in / high;
+  const int q0 = tq * BQ, p0 = tp * (GATED ? BP / 2 : BP);
+
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wp = wave % WP, wq = wave / WP;
+  const int k_first = split * a.k_per_split, k_end = min(a.nk, k_first + a.k_per_split);
+  const unsigned base = lds_address(lds);
+
+  f4 acc[NPT][NQT];
+#pragma unroll
+  for (int x = 0; x < NPT; ++x)
+#pragma unroll
+    for (int y = 0; y < NQT; ++y) acc[x][y] = f4{0.f, 0.f, 0.f, 0.f};
+
+  auto fetch = [&](int k0, int buf) {
+    TP::fetch(a.P, base + buf * BUF, p0, a.np, k0, k_end);
+    TQ::fetch(a.Q, base + buf * BUF + TP::BYTES, q0, a.nq, k0, k_end);
+  };
+  // first row of the wave's tile x of P: gate rows, then the up rows of the same features
+  auto p_row = [&](int x) {
+    return GATED ? (x < NPT / 2 ? wp * (BP / 2 / WP) + 16 * x : BP / 2 + wp * (BP / 2 / WP) + 16 * (x - NPT / 2)) : wp * (BP / WP) + 16 * x;
+  };
+
+  if (k_first < k_end) fetch(k_first, 0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = k_first; k0 < k_end; k0 += BK, buf ^= 1) {
+    if (k0 + BK < k_end) fetch(k0 + BK, buf ^ 1);
+    const char* pt = lds + buf * BUF;
+    const char* qt = pt + TP::BYTES;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      Frag fq[NQT];
+#pragma unroll
+      for (int y = 0; y < NQT; ++y) fq[y] = TQ::read(qt, wq * (BQ / WQ) + 16 * y, kk, i, g);
+#pragma unroll
+      for (int x = 0; x < NPT; ++x) {
+        const Frag fp = TP::read(pt, p_row(x), kk, i, g);
+#pragma unroll
+        for (int y = 0; y < NQT; ++y) acc[x][y] = mma<T>(fp, fq[y], acc[x][y]);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  if constexpr (GATED) {
+#pragma unroll
+    for (int x = 0; x < NPT / 2; ++x) {
+      const int f = p0 + wp * (BP / 2 / WP) + 16 * x + 4 * g, n = a.F - f;
+      f4 bg = {0.f, 0.f, 0.f, 0.f}, bu = bg, sg = bg, su = bg;
+      if (a.bias_g) bg = load4(static_cast<const T*>(a.bias_g) + f, n, 1);
+      if (a.bias_u) bu = load4(static_cast<const T*>(a.bias_u) + f, n, 1);
+#pragma unroll
+      for (int y = 0; y < NQT; ++y) {
+        const int q = q0 + wq * (BQ / WQ) + 16 * y + i;
+        f4 gv = acc[x][y] + bg, uv = acc[x + NPT / 2][y] + bu;
+        if constexpr (KIND == FORWARD) {
+          f4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = act(a.activation, gv[r]) * uv[r];
+          if (q < a.nq && n > 0) store4(static_cast<T*>(a.out) + (long)q * a.ld_out + f, v, n, a.out_step);
+        } else {
+          f4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
+          if (q < a.nq && n > 0) {
+            const f4 d = load4(static_cast<const T*>(a.dy) + (long)q * a.ld_dy + f, n, a.dy_step);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              if (r < n) {
+                dg[r] = d[r] * uv[r] * act_slope(a.activation, gv[r]);
+                du[r] = d[r] * act(a.activation, gv[r]);
+              }
+            }
+          }
+          sg += dg;
+          su += du;
+          // dh is summed over in the two products behind this one: its columns behind F are zero
+          if (q < a.nq && f < a.Fp) {
+            T* to = static_cast<T*>(a.out) + (long)q * a.ld_out + f;
+            store4(to, dg, 4, 4);
+            store4(to + a.Fp, du, 4, 4);
+          }
+        }
+      }
+      if constexpr (KIND == BACKWARD) {
+        if (a.part) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int off = 1; off < 16; off *= 2) {
+              sg[r] += __shfl_xor(sg[r], off);
+              su[r] += __shfl_xor(su[r], off);
+            }
+          if (i == 0 && f < a.Fp) {
+            float* to = a.part + (long)(tq * WQ + wq) * 2 * a.Fp + f;
+            *reinterpret_cast<f4*>(to) = sg;
+            *reinterpret_cast<f4*>(to + a.Fp) = su;
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < NPT; ++x) {
+      const int p = p0 + p_row(x) + 4 * g, n = a.np - p;
+#pragma unroll
+      for (int y = 0; y < NQT; ++y) {
+        const int q = q0 + wq * (BQ / WQ) + 16 * y + i;
+        if (q >= a.nq || n <= 0) continue;
+        if constexpr (KIND == PARTIAL) {
+          store4(a.part + ((long)split * a.nq + q) * a.ld_out + p, acc[x][y], n, a.ld_out % 4 == 0 ? 4 : 1);
+        } else {
+          const bool second = q >= a.out_split;
+          const int row = second ? q - a.out_split : q;
+          if (a.F && row >= a.F) continue;  // weights' gradients: rows behind F do not exist
+          store4(static_cast<T*>(second ? a.out1 : a.out) + (long)row * a.ld_out + p, acc[x][y], n, a.out_step);
+        }
+      }
+    }
+  }
+}
+
+int run_f32(const Args& a, int kind, bool large, hipStream_t s);
+int run_bf16(const Args& a, int kind, bool large, hipStream_t s);
+int run_f16(const Args& a, int kind, bool large, hipStream_t s);
+
+// Which product: KIND and the operands' layouts go together.
+enum { STEP_FORWARD, STEP_DH, STEP_DX, STEP_DW, STEP_DW_PARTIAL, STEP_DX_PARTIAL };
+
+template <typename T, int BP, int BQ, int WP, int WQ, bool PC, bool QC, int KIND>
+inline int run1(const Args& a, hipStream_t s) {
+  constexpr int LDS = 2 * (BP + BQ) * 128;
+  auto* f = &product<T, BP, BQ, WP, WQ, PC, QC, KIND>;
+  if (LDS > 65536) CET_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
+  f<<<(unsigned)(a.tiles_p * a.tiles_q * a.splits), 64 * WP * WQ, LDS, s>>>(a);
+  CET_HIP(hipGetLastError());
+  return CET_OK;
+}
+template <typename T, int BP, int BQ, int WP, int WQ>
+inline int run2(const Args& a, int step, hipStream_t s) {
+  switch (step) {
+    case STEP_FORWARD: return run1<T, BP, BQ, WP, WQ, false, false, FORWARD>(a, s);
+    case STEP_DH: return run1<T, BP, BQ, WP, WQ, false, false, BACKWARD>(a, s);
+    case STEP_DX: return run1<T, BP, BQ, WP, WQ, true, false, PLAIN>(a, s);
+    case STEP_DX_PARTIAL: return run1<T, BP, BQ, WP, WQ, true, false, PARTIAL>(a, s);
+    case STEP_DW: return run1<T, BP, BQ, WP, WQ, true, true, PLAIN>(a, s);
+    default: return run1<T, BP, BQ, WP, WQ, true, true, PARTIAL>(a, s);
+  }
+}
+template <typename T>
+inline int run(const Args& a, int step, bool large, hipStream_t s) {
+  return large ? run2<T, 256, 256, 2, 4>(a, step, s) : run2<T, 128, 128, 2, 2>(a, step, s);
+}
+
+}  // namespace gated
+}  // namespace cet

@@ -1,0 +1,10 @@
+// The gated projection: the matrix products for float tensors.
+#include "gated.h"
+
+namespace cet {
+namespace gated {
+
+int run_f32(const Args& a, int step, bool large, hipStream_t s) { return run<float>(a, step, large, s); }
+
+}  // namespace gated
+}  // namespace cet

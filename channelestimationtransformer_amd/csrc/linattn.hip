@@ -230,9 +230,8 @@ bool bad_desc(const cet_linattn_desc* d) {
   return !d || d->dtype < CET_F32 || d->dtype > CET_F16 || d->B < 0 || d->T < 0 || d->H < 0 || d->K < 1 || d->V < 1 ||
          d->T > (1 << 30) || !std::isfinite(d->scale);
 }
-bool too_large(const cet_linattn_desc& d) {
-  return d.K > 256 || d.V > 256 || (double)d.B * d.H * std::max(d.K, d.V) > 2e9 * 4 || (double)d.B * d.H * 16 > 2e9;
-}
+// (a launch holds fewer than 2^32 threads: 256 for each head of each sequence and slice)
+bool too_large(const cet_linattn_desc& d) { return d.K > 256 || d.V > 256 || (double)d.B * d.H > (1 << 22); }
 Strides contiguous(const cet_linattn_desc& d, int D) { return Strides{(long)d.T * d.H * D, (long)d.H * D, D}; }
 
 template <typename IO, int W>
@@ -365,7 +364,7 @@ int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64
                               const void* slots, int slots64, void* o, void* stream) {
   if (dtype < CET_F32 || dtype > CET_F16 || B < 0 || H < 0 || K < 1 || V < 1 || rows < 0 || !std::isfinite(scale))
     return CET_ERR_INVALID_ARG;
-  if (K > 256 || V > 256 || (double)B * H * V > 2e9) return CET_ERR_UNSUPPORTED;
+  if (K > 256 || V > 256 || (double)B * H > (1 << 21)) return CET_ERR_UNSUPPORTED;
   if ((long)B * H == 0) return CET_OK;
   if (!q_strides || !k_strides || !v_strides || !q || !k || !v || !log_decay || !o) return CET_ERR_INVALID_ARG;
   if (rows > 0 && (!state_in || !state_out)) return CET_ERR_INVALID_ARG;

@@ -147,17 +147,18 @@ int launch(RotArgs a, int interleaved, bool wide, hipStream_t s) {
   a.head_groups = (heads + a.heads_per_wg - 1) / a.heads_per_wg;
   a.units = Div((unsigned)units);
   a.heads = Div((unsigned)a.heads_per_wg);
-  const unsigned blocks = (unsigned)((n + tile - 1) / tile * a.head_groups);
+  const long blocks = (n + tile - 1) / tile * a.head_groups;
+  if (blocks >= 1 << 24) return CET_ERR_UNSUPPORTED;  // a launch holds fewer than 2^32 threads
   const size_t lds = (size_t)tile * a.pairs * sizeof(float2);
   if (wide) {
     if (interleaved)
-      rotary_kernel<E, VEC, false><<<blocks, 256, lds, s>>>(a);
+      rotary_kernel<E, VEC, false><<<(unsigned)blocks, 256, lds, s>>>(a);
     else
-      rotary_kernel<E, VEC, true><<<blocks, 256, lds, s>>>(a);
+      rotary_kernel<E, VEC, true><<<(unsigned)blocks, 256, lds, s>>>(a);
   } else if (interleaved) {
-    rotary_kernel<E, 1, false><<<blocks, 256, lds, s>>>(a);
+    rotary_kernel<E, 1, false><<<(unsigned)blocks, 256, lds, s>>>(a);
   } else {
-    rotary_kernel<E, 1, true><<<blocks, 256, lds, s>>>(a);
+    rotary_kernel<E, 1, true><<<(unsigned)blocks, 256, lds, s>>>(a);
   }
   CET_HIP(hipGetLastError());
   return CET_OK;

@@ -544,3 +544,90 @@ def _rotary_backward(ctx, dq, dk):
 
 
 rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+GATED_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+def _gated(x, w_gate, w_up, b_gate, b_up, activation, dy=None):
+    """Checked operands of the gated projection and their descriptor; x and dy as matrices."""
+    dev = _dev_check(*(t for t in (x, w_gate, w_up, b_gate, b_up, dy) if t is not None))
+    code = _seq_type(x)
+    if activation not in GATED_ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {sorted(GATED_ACTIVATIONS)}, got {activation!r}")
+    x = _seq_check("x", x, x.dtype, None, None)
+    N, D = x.shape
+    w_gate = _seq_check("w_gate", w_gate, x.dtype, None, D)
+    F = w_gate.shape[0]
+    w_up = _seq_check("w_up", w_up, x.dtype, F, D)
+    if D < 1 or F < 1 or D > 1 << 20 or F > 1 << 20 or N > 1 << 28:
+        raise RuntimeError(f"x [N, D] and weights [F, D] with N up to 2^28, D and F from 1 to 2^20 are served, got {N}, {D}, {F}")
+    b_gate, b_up = (None if b is None else _seq_check(n, b, x.dtype, F) for n, b in (("b_gate", b_gate), ("b_up", b_up)))
+    if dy is not None:
+        dy = _seq_check("dy", dy, x.dtype, N, F)
+    d = _cabi.GatedDesc(code, GATED_ACTIVATIONS[activation], N, D, F, x.stride(0), w_gate.stride(0), w_up.stride(0),
+                        0 if dy is None else dy.stride(0))
+    return dev, d, x, w_gate, w_up, b_gate, b_up, dy
+
+
+@torch.library.custom_op("cet::gated_linear", mutates_args=())
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor],
+                 b_up: Optional[torch.Tensor], activation: str) -> torch.Tensor:
+    """x [N,D], w_gate, w_up [F,D], b_gate, b_up [F] or None -> act(x w_gate^T + b_gate) * (x w_up^T + b_up) [N,F]."""
+    dev, d, x, w_gate, w_up, b_gate, b_up, _ = _gated(x, w_gate, w_up, b_gate, b_up, activation)
+    out = torch.empty((d.N, d.F), dtype=x.dtype, device=dev)
+    L = _cabi.lib()
+    with torch.cuda.device(dev):
+        n = L.cet_gated_linear_workspace(d, _ptr(x), _ptr(w_gate), _ptr(w_up), 0)
+        ws = _workspace(n, dev)
+        rc = L.cet_gated_linear(d, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(b_gate), _ptr(b_up), _ptr(out), _ptr(ws), n,
+                                _cabi.current_stream_ptr(dev))
+    _cabi.check(rc, "cet_gated_linear")
+    return out
+
+
+@gated_linear.register_fake
+def _(x, w_gate, w_up, b_gate, b_up, activation):
+    return x.new_empty((x.shape[0], w_gate.shape[0]))
+
+
+@torch.library.custom_op("cet::gated_linear_backward", mutates_args=())
+def gated_linear_backward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor],
+                          b_up: Optional[torch.Tensor], activation: str, dy: torch.Tensor, want_x: bool, want_w: bool,
+                          want_b: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> dx, dw_gate, dw_up, db_gate, db_up; empty where not wanted."""
+    dev, d, x, w_gate, w_up, b_gate, b_up, dy = _gated(x, w_gate, w_up, b_gate, b_up, activation, dy)
+    new = lambda want, *shape: torch.empty(shape if want else (0,), dtype=x.dtype, device=dev)  # noqa: E731
+    dx, dw_gate, dw_up = new(want_x, d.N, d.D), new(want_w, d.F, d.D), new(want_w, d.F, d.D)
+    db_gate, db_up = new(want_b, d.F), new(want_b, d.F)
+    L = _cabi.lib()
+    with torch.cuda.device(dev):
+        n = L.cet_gated_linear_workspace(d, _ptr(x), _ptr(w_gate), _ptr(w_up), 1)
+        ws = _workspace(n, dev)
+        rc = L.cet_gated_linear_backward(d, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(b_gate), _ptr(b_up), _ptr(dy), _ptr(dx),
+                                         _ptr(dw_gate), _ptr(dw_up), _ptr(db_gate), _ptr(db_up), _ptr(ws), n,
+                                         _cabi.current_stream_ptr(dev))
+    _cabi.check(rc, "cet_gated_linear_backward")
+    return dx, dw_gate, dw_up, db_gate, db_up
+
+
+@gated_linear_backward.register_fake
+def _(x, w_gate, w_up, b_gate, b_up, activation, dy, want_x, want_w, want_b):
+    shapes = ((want_x, x.shape), (want_w, w_gate.shape), (want_w, w_up.shape), (want_b, w_gate.shape[:1]), (want_b, w_up.shape[:1]))
+    return tuple(x.new_empty(s if want else (0,)) for want, s in shapes)
+
+
+def _gated_setup(ctx, inputs, output):
+    x, w_gate, w_up, b_gate, b_up, ctx.activation = inputs
+    ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up)
+
+
+def _gated_backward(ctx, dy):
+    x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dwg, dwu, dbg, dbu = torch.ops.cet.gated_linear_backward(
+        x, w_gate, w_up, b_gate, b_up, ctx.activation, dy, need[0], need[1] or need[2], need[3] or need[4])
+    return tuple(t if n else None for t, n in zip((dx, dwg, dwu, dbg, dbu), need)) + (None,)
+
+
+gated_linear.register_autograd(_gated_backward, setup_context=_gated_setup)

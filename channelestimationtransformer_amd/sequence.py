@@ -3,11 +3,12 @@
 The Transformer predictors hold at most 48 slots in one tile and the recurrent ones roll a dense state
 forward; these are the blocks between the two. `rotary` gives queries and keys their slots' positions
 (the Transformer adds a fixed table of sinusoids), `linear_attention` reads a history in chunks and
-leaves a state of fixed size per head, `linear_attention_step` carries that state on slot by slot.
+leaves a state of fixed size per head, `linear_attention_step` carries that state on slot by slot, and
+`gated_linear` is the first half of a gated feed-forward (the Transformer's is a plain one).
 
 All take CUDA (ROCm) tensors of one type (float32, bfloat16 or float16), run on the current stream
-and raise on anything the kernels do not serve. `rotary` and `linear_attention` have gradients
-(`rotary`'s can be differentiated again).
+and raise on anything the kernels do not serve. `rotary`, `linear_attention` and
+`gated_linear` have gradients (`rotary`'s can be differentiated again).
 """
 import math
 
@@ -100,3 +101,15 @@ def rotary(q, k, positions, inv_freq, layout="half", gain=1.0):
         raise RuntimeError("inv_freq is a constant of rotary: it has no gradient (detach it)")
     a, b = torch.ops.cet.rotary(q, k, positions, inv_freq, layout == "interleaved", float(gain), False)
     return a, (b if k is not None else None)
+
+
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up) in one kernel: x [..., D], w_gate and w_up [F, D] (the
+    layout of `torch.nn.Linear`, or two halves of one [2F, D]), biases [F] or None, one type for all;
+    returns [..., F]. `activation`: "silu", "gelu" (erf form) or "relu". Projections and activation are
+    formed in float32 and the result is rounded once; the projections are not kept for the gradient but
+    formed again, their gradients are rounded to the tensors' type before the last products."""
+    if x.dim() < 1:
+        raise RuntimeError("x must be [..., D]")
+    out = torch.ops.cet.gated_linear(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, w_gate, w_up, b_gate, b_up, activation)
+    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], w_gate.shape[0])

@@ -372,6 +372,32 @@ typedef struct cet_rotary_desc {
 int cet_rotary(const cet_rotary_desc* d, const void* q, const void* k, const void* positions,
                const double* inv_freq, int inverse, void* q_out, void* k_out, void* stream);
 
+/* The gated projection of a feed-forward block: out = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel, for
+ * x [N,D], Wg and Wu [F,D] (rows at the given strides, in elements), bg and bu [F] (either may be NULL: zero),
+ * out [N,F] contiguous. Products and the activation are formed in fp32, out is rounded once. */
+typedef struct cet_gated_desc {
+  int32_t dtype;
+  int32_t activation; /* 0 silu, 1 gelu (exact erf form), 2 relu */
+  int32_t N, D, F;
+  int64_t ld_x, ld_gate, ld_up;
+  int64_t ld_dy; /* backward only */
+} cet_gated_desc;
+
+/* Bytes of workspace (16-byte aligned, in use until the call has run on the stream). */
+size_t cet_gated_linear_workspace(const cet_gated_desc* d, const void* x, const void* w_gate, const void* w_up,
+                                  int backward);
+int cet_gated_linear(const cet_gated_desc* d, const void* x, const void* w_gate, const void* w_up,
+                     const void* b_gate, const void* b_up, void* out, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Gradients from dy [N,F] (rows at ld_dy); the projections are formed again. dx [N,D], dw_* [F,D], db_* [F],
+ * contiguous; dx, both dw or both db may be NULL (not wanted). The gradients of the projections are rounded to
+ * the tensors' type once before the products that dx and dw are; db is summed from them in fp32. */
+int cet_gated_linear_backward(const cet_gated_desc* d, const void* x, const void* w_gate, const void* w_up,
+                              const void* b_gate, const void* b_up, const void* dy, void* dx, void* dw_gate,
+                              void* dw_up, void* db_gate, void* db_up, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

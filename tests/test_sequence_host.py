@@ -113,3 +113,44 @@ def test_rotary_refusals():
                 {"dim": 8, "factor": 0.0}, {"dim": 8, "scaling": "yarn", "original_length": 64, "turns": (1.0, 2.0)}):
         with pytest.raises(RuntimeError):
             cet.rotary_frequencies(device="cpu", **bad)
+
+
+def gated_desc(**kw):
+    d = _cabi.GatedDesc(0, 0, 100, 64, 48, 64, 64, 64, 48)
+    for n, v in kw.items():
+        setattr(d, n, v)
+    return d
+
+
+@pytest.mark.parametrize("change, code", [
+    ({"dtype": 3}, 1), ({"activation": 3}, 1), ({"activation": -1}, 1), ({"N": -1}, 1), ({"D": 0}, 1), ({"F": 0}, 1), ({"D": 1 << 21}, 2),
+    ({"F": 1 << 21}, 2), ({"N": 1 << 29}, 2), ({"N": 1 << 28, "F": 1 << 20}, 2)])
+def test_gated_descriptors(change, code):
+    L = _cabi.lib()
+    d = gated_desc(**change)
+    assert L.cet_gated_linear_workspace(d, P, P, P, 1) == 0
+    assert L.cet_gated_linear(d, P, P, P, None, None, P, P, 1 << 40, None) == code
+    assert L.cet_gated_linear_backward(d, P, P, P, None, None, P, P, P, P, None, None, P, 1 << 40, None) == code
+
+
+def test_gated_refusals():
+    L = _cabi.lib()
+    d = gated_desc()
+    for hole in range(4):
+        p = [P, P, P, P]
+        p[hole] = None
+        assert L.cet_gated_linear(d, *p[:3], None, None, p[3], None, 0, None) == 1
+        assert L.cet_gated_linear_backward(d, *p[:3], None, None, p[3], P, P, P, None, None, P, 1 << 40, None) == 1
+    n = L.cet_gated_linear_workspace(d, P, P, P, 1)
+    assert n > 0
+    assert L.cet_gated_linear_backward(d, P, P, P, None, None, P, P, P, P, None, None, P, n - 1, None) == 1
+    assert L.cet_gated_linear_backward(d, P, P, P, None, None, P, P, P, P, None, None, P + 8, n + 99, None) == 1
+    assert L.cet_gated_linear_backward(d, P, P, P, None, None, P, P, P, None, None, None, P, n, None) == 1
+    assert L.cet_gated_linear_backward(d, P, P, P, None, None, P, P, P, P, P, None, P, n, None) == 1
+    assert L.cet_gated_linear(d, P + 4, P, P, None, None, P, None, 0, None) == 1  # copy without workspace
+    assert L.cet_gated_linear(gated_desc(N=0), None, None, None, None, None, None, None, 0, None) == 0
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        cet.gated_linear(x, w, w)
+    with pytest.raises(RuntimeError):
+        cet.gated_linear(torch.zeros(()), w, w)
