@@ -4,6 +4,7 @@ Each op checks device / dtype / contiguity, allocates the outputs with torch (th
 never allocates results) and enqueues the HIP kernel on torch's current stream through the
 ctypes binding. Handles are created and owned by the host-side model objects.
 """
+import contextlib
 import ctypes
 import math
 from typing import Optional
@@ -344,8 +345,24 @@ def _workspace(n, dev):
     return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
 
 
-@torch.library.custom_op("cet::linear_attention", mutates_args=())
-def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
+def _at(t):
+    """Address of a tensor's first element (None without one), as the C entry points take it."""
+    return t.data_ptr() or None if t is not None else None
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """`dev` as the current device; nothing to do, and no time spent, where it is already."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def run_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
                      initial_state: Optional[torch.Tensor] = None,
                      lengths: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """q, k [B,T,H,K], v [B,T,H,V] -> o [B,T,H,V], state float32 [B,H,K,V]."""
@@ -353,13 +370,16 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     o = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
     state = torch.empty((d.B, d.H, d.K, d.V), dtype=torch.float32, device=dev)
     L = _cabi.lib()
-    with torch.cuda.device(dev):
-        n = L.cet_linear_attention_workspace(d, _ptr(q), _ptr(k), _ptr(v), None, 0)
+    with _on(dev):
+        n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), None, 0)
         ws = _workspace(n, dev)
-        rc = L.cet_linear_attention(d, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(s0), _ptr(lengths), _ptr(o),
-                                    _ptr(state), _ptr(ws), n, _cabi.current_stream_ptr(dev))
+        rc = L.cet_linear_attention(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths), _at(o),
+                                    _at(state), _at(ws), n, _stream(dev))
     _cabi.check(rc, "cet_linear_attention")
     return o, state
+
+
+linear_attention = torch.library.custom_op("cet::linear_attention", mutates_args=())(run_linear_attention)
 
 
 @linear_attention.register_fake
@@ -368,8 +388,7 @@ def _(q, k, v, log_decay, scale, initial_state=None, lengths=None):
     return q.new_empty((B, T, H, v.shape[3])), q.new_empty((B, H, K, v.shape[3]), dtype=torch.float32)
 
 
-@torch.library.custom_op("cet::linear_attention_backward", mutates_args=())
-def linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
+def run_linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
                               initial_state: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
                               d_o: torch.Tensor, d_state: Optional[torch.Tensor], want_initial: bool
                               ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -382,14 +401,17 @@ def linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     dv = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
     ds = torch.empty((d.B, d.H, d.K, d.V) if want_initial else (0,), dtype=torch.float32, device=dev)
     L = _cabi.lib()
-    with torch.cuda.device(dev):
-        n = L.cet_linear_attention_workspace(d, _ptr(q), _ptr(k), _ptr(v), _ptr(d_o), 1)
+    with _on(dev):
+        n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), _at(d_o), 1)
         ws = _workspace(n, dev)
-        rc = L.cet_linear_attention_backward(d, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(s0), _ptr(lengths),
-                                             _ptr(d_o), _ptr(d_state), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ds), _ptr(ws),
-                                             n, _cabi.current_stream_ptr(dev))
+        rc = L.cet_linear_attention_backward(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths),
+                                             _at(d_o), _at(d_state), _at(dq), _at(dk), _at(dv), _at(ds), _at(ws),
+                                             n, _stream(dev))
     _cabi.check(rc, "cet_linear_attention_backward")
     return dq, dk, dv, ds
+
+
+linear_attention_backward = torch.library.custom_op("cet::linear_attention_backward", mutates_args=())(run_linear_attention_backward)
 
 
 @linear_attention_backward.register_fake
@@ -408,18 +430,29 @@ def _linattn_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _linattn_backward(ctx, d_o, d_state):
+def _linattn_backward(ctx, d_o, d_state, run=linear_attention_backward):
     q, k, v, log_decay, s0, lengths = ctx.saved_tensors
     if d_o is None:
         if d_state is None:
             return (None,) * 7
         d_o = q.new_zeros((*q.shape[:3], v.shape[3]))
     want = s0 is not None and ctx.needs_input_grad[5]
-    dq, dk, dv, ds = torch.ops.cet.linear_attention_backward(q, k, v, log_decay, ctx.scale, s0, lengths, d_o, d_state, want)
+    dq, dk, dv, ds = run(q, k, v, log_decay, ctx.scale, s0, lengths, d_o, d_state, want)
     return dq, dk, dv, None, None, ds if want else None, None
 
 
 linear_attention.register_autograd(_linattn_backward, setup_context=_linattn_setup)
+
+
+class LinearAttention(torch.autograd.Function):
+    """The same operator without the dispatcher (eager calls on plain tensors: a fifth of the host time)."""
+    forward = staticmethod(run_linear_attention)
+    setup_context = staticmethod(_linattn_setup)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_state):
+        return _linattn_backward(ctx, d_o, d_state, run_linear_attention_backward)
 
 
 def _step(q, k, v, log_decay, state, out_state, scale, slots):
@@ -438,16 +471,15 @@ def _step(q, k, v, log_decay, state, out_state, scale, slots):
     if slots is not None:
         slots, wide = _index("slots", slots, B)
     strides = [(ctypes.c_int64 * 2)(*t.stride()[:2]) for t in (q, k, v)]
-    with torch.cuda.device(dev):
+    with _on(dev):
         rc = _cabi.lib().cet_linear_attention_step(
-            code, B, H, K, V, *strides, _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), scale, _ptr(state), _ptr(out_state),
-            state.shape[0], _ptr(slots), wide, _ptr(o), _cabi.current_stream_ptr(dev))
+            code, B, H, K, V, *strides, _at(q), _at(k), _at(v), _at(log_decay), scale, _at(state), _at(out_state),
+            state.shape[0], _at(slots), wide, _at(o), _stream(dev))
     _cabi.check(rc, "cet_linear_attention_step")
     return o
 
 
-@torch.library.custom_op("cet::linear_attention_step", mutates_args=())
-def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+def run_linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
                           state: torch.Tensor, scale: float) -> tuple[torch.Tensor, torch.Tensor]:
     """q, k [B,H,K], v [B,H,V], state float32 [B,H,K,V] -> o [B,H,V], the next state."""
     if q.dim() != 3 or v.dim() != 3:
@@ -457,13 +489,15 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     return _step(q, k, v, log_decay, state, out, scale, None), out
 
 
+linear_attention_step = torch.library.custom_op("cet::linear_attention_step", mutates_args=())(run_linear_attention_step)
+
+
 @linear_attention_step.register_fake
 def _(q, k, v, log_decay, state, scale):
     return v.new_empty(v.shape), state.new_empty(state.shape)
 
 
-@torch.library.custom_op("cet::linear_attention_step_", mutates_args=("state",))
-def linear_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
+def run_linear_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor,
                            state: torch.Tensor, scale: float, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same with the state (with `slots`: a pool of them) updated in place."""
     if q.dim() != 3 or v.dim() != 3:
@@ -475,13 +509,15 @@ def linear_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     return _step(q, k, v, log_decay, state, state, scale, slots)
 
 
+linear_attention_step_ = torch.library.custom_op("cet::linear_attention_step_", mutates_args=("state",))(run_linear_attention_step_)
+
+
 @linear_attention_step_.register_fake
 def _(q, k, v, log_decay, state, scale, slots=None):
     return v.new_empty(v.shape)
 
 
-@torch.library.custom_op("cet::rotary", mutates_args=())
-def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool,
+def run_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, interleaved: bool,
            gain: float, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """q [B,T,Hq,D], k [B,T,Hk,D] or None, positions int32 / int64 [T] or [B,T], inv_freq float64 [pairs]
     -> the turned q and k (empty without k)."""
@@ -509,11 +545,14 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     d.pos[:] = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
     qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
     ko = torch.empty((B, T, Hk, D) if k is not None else (0,), dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
-        rc = _cabi.lib().cet_rotary(d, _ptr(q), _ptr(k), _ptr(positions), _ptr(inv_freq), int(inverse), _ptr(qo), _ptr(ko),
-                                    _cabi.current_stream_ptr(dev))
+    with _on(dev):
+        rc = _cabi.lib().cet_rotary(d, _at(q), _at(k), _at(positions), _at(inv_freq), int(inverse), _at(qo), _at(ko),
+                                    _stream(dev))
     _cabi.check(rc, "cet_rotary")
     return qo, ko
+
+
+rotary = torch.library.custom_op("cet::rotary", mutates_args=())(run_rotary)
 
 
 @rotary.register_fake
@@ -527,13 +566,13 @@ def _rotary_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _rotary_backward(ctx, dq, dk):
+def _rotary_backward(ctx, dq, dk, run=rotary):
     positions, inv_freq = ctx.saved_tensors
     if not ctx.needs_input_grad[1]:
         dk = None
     if not ctx.needs_input_grad[0]:
         dq = None
-    turn = lambda a, b: torch.ops.cet.rotary(a, b, positions, inv_freq, ctx.interleaved, ctx.gain, not ctx.inverse)  # noqa: E731
+    turn = lambda a, b: run(a, b, positions, inv_freq, ctx.interleaved, ctx.gain, not ctx.inverse)  # noqa: E731
     if dq is None:
         dk = turn(dk, None)[0] if dk is not None else None
     elif dk is None:
@@ -544,6 +583,20 @@ def _rotary_backward(ctx, dq, dk):
 
 
 rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
+
+
+class Rotary(torch.autograd.Function):
+    forward = staticmethod(run_rotary)
+    setup_context = staticmethod(_rotary_setup)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        return _rotary_backward(ctx, dq, dk, direct_rotary)
+
+
+def direct_rotary(q, k, *rest):
+    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    return (Rotary.apply if grad else run_rotary)(q, k, *rest)
 
 
 GATED_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
@@ -570,20 +623,22 @@ def _gated(x, w_gate, w_up, b_gate, b_up, activation, dy=None):
     return dev, d, x, w_gate, w_up, b_gate, b_up, dy
 
 
-@torch.library.custom_op("cet::gated_linear", mutates_args=())
-def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor],
+def run_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor],
                  b_up: Optional[torch.Tensor], activation: str) -> torch.Tensor:
     """x [N,D], w_gate, w_up [F,D], b_gate, b_up [F] or None -> act(x w_gate^T + b_gate) * (x w_up^T + b_up) [N,F]."""
     dev, d, x, w_gate, w_up, b_gate, b_up, _ = _gated(x, w_gate, w_up, b_gate, b_up, activation)
     out = torch.empty((d.N, d.F), dtype=x.dtype, device=dev)
     L = _cabi.lib()
-    with torch.cuda.device(dev):
-        n = L.cet_gated_linear_workspace(d, _ptr(x), _ptr(w_gate), _ptr(w_up), 0)
+    with _on(dev):
+        n = L.cet_gated_linear_workspace(d, _at(x), _at(w_gate), _at(w_up), 0)
         ws = _workspace(n, dev)
-        rc = L.cet_gated_linear(d, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(b_gate), _ptr(b_up), _ptr(out), _ptr(ws), n,
-                                _cabi.current_stream_ptr(dev))
+        rc = L.cet_gated_linear(d, _at(x), _at(w_gate), _at(w_up), _at(b_gate), _at(b_up), _at(out), _at(ws), n,
+                                _stream(dev))
     _cabi.check(rc, "cet_gated_linear")
     return out
+
+
+gated_linear = torch.library.custom_op("cet::gated_linear", mutates_args=())(run_gated_linear)
 
 
 @gated_linear.register_fake
@@ -591,8 +646,7 @@ def _(x, w_gate, w_up, b_gate, b_up, activation):
     return x.new_empty((x.shape[0], w_gate.shape[0]))
 
 
-@torch.library.custom_op("cet::gated_linear_backward", mutates_args=())
-def gated_linear_backward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor],
+def run_gated_linear_backward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor],
                           b_up: Optional[torch.Tensor], activation: str, dy: torch.Tensor, want_x: bool, want_w: bool,
                           want_b: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """-> dx, dw_gate, dw_up, db_gate, db_up; empty where not wanted."""
@@ -601,14 +655,17 @@ def gated_linear_backward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Ten
     dx, dw_gate, dw_up = new(want_x, d.N, d.D), new(want_w, d.F, d.D), new(want_w, d.F, d.D)
     db_gate, db_up = new(want_b, d.F), new(want_b, d.F)
     L = _cabi.lib()
-    with torch.cuda.device(dev):
-        n = L.cet_gated_linear_workspace(d, _ptr(x), _ptr(w_gate), _ptr(w_up), 1)
+    with _on(dev):
+        n = L.cet_gated_linear_workspace(d, _at(x), _at(w_gate), _at(w_up), 1)
         ws = _workspace(n, dev)
-        rc = L.cet_gated_linear_backward(d, _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(b_gate), _ptr(b_up), _ptr(dy), _ptr(dx),
-                                         _ptr(dw_gate), _ptr(dw_up), _ptr(db_gate), _ptr(db_up), _ptr(ws), n,
-                                         _cabi.current_stream_ptr(dev))
+        rc = L.cet_gated_linear_backward(d, _at(x), _at(w_gate), _at(w_up), _at(b_gate), _at(b_up), _at(dy), _at(dx),
+                                         _at(dw_gate), _at(dw_up), _at(db_gate), _at(db_up), _at(ws), n,
+                                         _stream(dev))
     _cabi.check(rc, "cet_gated_linear_backward")
     return dx, dw_gate, dw_up, db_gate, db_up
+
+
+gated_linear_backward = torch.library.custom_op("cet::gated_linear_backward", mutates_args=())(run_gated_linear_backward)
 
 
 @gated_linear_backward.register_fake
@@ -622,12 +679,41 @@ def _gated_setup(ctx, inputs, output):
     ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up)
 
 
-def _gated_backward(ctx, dy):
+def _gated_backward(ctx, dy, run=gated_linear_backward):
     x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
     need = ctx.needs_input_grad
-    dx, dwg, dwu, dbg, dbu = torch.ops.cet.gated_linear_backward(
+    dx, dwg, dwu, dbg, dbu = run(
         x, w_gate, w_up, b_gate, b_up, ctx.activation, dy, need[0], need[1] or need[2], need[3] or need[4])
     return tuple(t if n else None for t, n in zip((dx, dwg, dwu, dbg, dbu), need)) + (None,)
 
 
 gated_linear.register_autograd(_gated_backward, setup_context=_gated_setup)
+
+
+class GatedLinear(torch.autograd.Function):
+    forward = staticmethod(run_gated_linear)
+    setup_context = staticmethod(_gated_setup)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return _gated_backward(ctx, dy, run_gated_linear_backward)
+
+
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
+
+
+def step_in_place(q, k, v, log_decay, state, scale, slots):
+    """run_linear_attention_step_, and autograd told of the write as the dispatcher would."""
+    o = run_linear_attention_step_(q, k, v, log_decay, state, scale, slots)
+    torch.autograd.graph.increment_version(state)
+    return o
+
+
+def direct(*tensors):
+    """Whether a call may pass the dispatcher by: eager, and on plain tensors only (none of a tracer's)."""
+    return not torch.compiler.is_compiling() and all(type(t) in _PLAIN for t in tensors)
+
+
+def wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

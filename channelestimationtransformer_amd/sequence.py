@@ -33,7 +33,10 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("log_decay is a constant of linear_attention: it has no gradient (detach it)")
-    return torch.ops.cet.linear_attention(q, k, v, log_decay, float(scale), initial_state, lengths)
+    args = q, k, v, log_decay, float(scale), initial_state, lengths
+    if not ops.direct(q, k, v, log_decay, initial_state, lengths):
+        return torch.ops.cet.linear_attention(*args)
+    return ops.LinearAttention.apply(*args) if ops.wants_grad(q, k, v, initial_state) else ops.run_linear_attention(*args)
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None, slots=None, inplace=False):
@@ -49,9 +52,10 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None, slots=None, inp
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
         raise RuntimeError("linear_attention_step has no gradient: call it under torch.no_grad(), or "
                            "linear_attention with T = 1")
+    direct, args = ops.direct(q, k, v, log_decay, state, slots), (q, k, v, log_decay, state, float(scale))
     if slots is not None or inplace:
-        return torch.ops.cet.linear_attention_step_(q, k, v, log_decay, state, float(scale), slots), state
-    return torch.ops.cet.linear_attention_step(q, k, v, log_decay, state, float(scale))
+        return (ops.step_in_place if direct else torch.ops.cet.linear_attention_step_)(*args, slots), state
+    return (ops.run_linear_attention_step if direct else torch.ops.cet.linear_attention_step)(*args)
 
 
 def rotary_frequencies(dim, base=10000.0, scaling="none", factor=1.0, original_length=None, turns=(32.0, 1.0), device="cuda"):
@@ -99,7 +103,8 @@ def rotary(q, k, positions, inv_freq, layout="half", gain=1.0):
         raise RuntimeError(f'layout must be "half" or "interleaved", got {layout!r}')
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("inv_freq is a constant of rotary: it has no gradient (detach it)")
-    a, b = torch.ops.cet.rotary(q, k, positions, inv_freq, layout == "interleaved", float(gain), False)
+    run = ops.direct_rotary if ops.direct(q, k, positions, inv_freq) else torch.ops.cet.rotary
+    a, b = run(q, k, positions, inv_freq, layout == "interleaved", float(gain), False)
     return a, (b if k is not None else None)
 
 
@@ -111,5 +116,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     formed again, their gradients are rounded to the tensors' type before the last products."""
     if x.dim() < 1:
         raise RuntimeError("x must be [..., D]")
-    out = torch.ops.cet.gated_linear(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, w_gate, w_up, b_gate, b_up, activation)
+    args = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, w_gate, w_up, b_gate, b_up, activation
+    if not ops.direct(x, w_gate, w_up, b_gate, b_up):
+        out = torch.ops.cet.gated_linear(*args)
+    else:
+        out = ops.GatedLinear.apply(*args) if ops.wants_grad(x, w_gate, w_up, b_gate, b_up) else ops.run_gated_linear(*args)
     return out if x.dim() == 2 else out.reshape(*x.shape[:-1], w_gate.shape[0])
