@@ -112,7 +112,7 @@ struct Type<__bf16> {
   typedef __bf16 Lds;
   typedef bf4 Quad;
   static constexpr bool BF = true;
-  static constexpr int VEC = 8, C = 64, LDPAD = 8;
+  static constexpr int VEC = 8, C = 32, LDPAD = 8;
   __device__ static void to_lds(__bf16* p, const uint4& raw) { *reinterpret_cast<uint4*>(p) = raw; }
   __device__ static float load(const __bf16* p) { return (float)*p; }
   __device__ static void store(__bf16* p, float v) { *p = (__bf16)v; }
@@ -156,35 +156,51 @@ __device__ inline bf4 quad_cols(const __bf16* t, int ld, int r0, int c0, int i, 
   return __builtin_bit_cast(bf4, r);
 }
 
-// Rows of a chunk on their way from memory to LDS: C rows of COLS columns over NT threads.
+// Rows of consecutive chunks on their way from memory to LDS: C rows of COLS columns over NT threads. A
+// thread keeps the address of each of its pieces and moves it on by a chunk with every fetch.
 template <typename IO, int C, int COLS, int NT>
 struct Rows {
   typedef Type<IO> Ty;
   static constexpr int VEC = Ty::VEC, PER_ROW = COLS / VEC, TOTAL = C * PER_ROW, N = (TOTAL + NT - 1) / NT;
   uint4 raw[N];
+  const char* at[N];
+  long step;  // bytes from chunk to chunk
 
-  // place i0 + r of the sequence is slot i0 + r, or rows - 1 - (i0 + r) backward in time; rows from n
-  // on and columns from `cols` on are zero
-  __device__ void fetch(const IO* base, long st, int i0, int n, int rows, int reverse, int c0, int cols) {
+  __device__ static int row_of(int u) { return (u * NT + (int)threadIdx.x) / PER_ROW; }
+  __device__ static int col_of(int u) { return (u * NT + (int)threadIdx.x) % PER_ROW * VEC; }
+
+  // place i of the sequence is slot i, or rows - 1 - i backward in time; the first fetch takes places i0..
+  __device__ void init(const IO* p, long st, int i0, int rows, int reverse, int c0) {
+    step = (reverse ? -C : C) * st * (long)sizeof(IO);
 #pragma unroll
     for (int u = 0; u < N; ++u) {
-      const int at = u * NT + (int)threadIdx.x;
-      const int r = at / PER_ROW, c = c0 + at % PER_ROW * VEC;
+      const long place = i0 + row_of(u);
+      at[u] = reinterpret_cast<const char*>(p + (reverse ? rows - 1 - place : place) * st + c0 + col_of(u));
+    }
+  }
+  // rows from n on and columns from `cols` (counted from c0) on are zero
+  __device__ void fetch(int n, int cols) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
       raw[u] = uint4{0, 0, 0, 0};
-      if ((TOTAL % NT == 0 || at < TOTAL) && r < n && c < cols) {
-        const IO* p = base + (long)(reverse ? rows - 1 - (i0 + r) : i0 + r) * st + c;
-        raw[u] = *reinterpret_cast<const uint4*>(p);
-      }
+      if (row_of(u) < n && col_of(u) < cols) raw[u] = *reinterpret_cast<const uint4*>(at[u]);
+      at[u] += step;
     }
   }
   __device__ void put(typename Ty::Lds* lds, int ld) const {
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const int at = u * NT + (int)threadIdx.x;
-      if (TOTAL % NT == 0 || at < TOTAL) Ty::to_lds(lds + at / PER_ROW * ld + at % PER_ROW * VEC, raw[u]);
-    }
+    for (int u = 0; u < N; ++u)
+      if (TOTAL % NT == 0 || row_of(u) < C) Ty::to_lds(lds + row_of(u) * ld + col_of(u), raw[u]);
   }
 };
+
+template <int NK, int NV>
+__device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
+#pragma unroll
+  for (int x = 0; x < NK; ++x)
+#pragma unroll
+    for (int y = 0; y < NV; ++y) S[x][y] *= f;
+}
 
 // OUT: with outputs; without, only the state that a segment of slots adds is formed (into ws).
 template <typename IO, int NK, int NV, int NW, bool OUT>
@@ -242,32 +258,43 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
     }
   }
 
-  const float ld = a.log_decay[h], g2 = ld * 1.44269504088896340736f;
+  const float g2 = a.log_decay[h] * 1.44269504088896340736f;
   const int e = a.reverse ? 0 : 1;
   // scores: same block (masked), next block; further blocks by d^16 each
-  float wd[4], wo[4], wb[4];
+  float wd[4], wo[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int s = 4 * g + r;
     wd[r] = i >= s ? pw(g2, i - s) * a.s_intra : 0.f;
     wo[r] = pw(g2, 16 + i - s) * a.s_intra;
-    wb[r] = pw(g2, 16 - e - s) * a.s_kv;  // what a slot of the last block keeps at the end of a full chunk
   }
   float d16[NB];
 #pragma unroll
   for (int x = 0; x < NB; ++x) d16[x] = pw(g2, 16 * x);
   const float rf = pw(g2, i + e) * a.s_inter;
-  // d^C in two parts: a rounding of it would be raised to the number of chunks in the weight of a slot far back
-  const double dc = exp((double)C * (double)ld);
-  const float dc_hi = (float)dc, dc_lo = (float)(dc - (double)dc_hi);
+  // A state that fades slowly is kept as S / d^m, m slots since it was last multiplied out: a chunk then adds
+  // its keys and values by the weights d^-(m + 1 + j) and touches no element of S otherwise (multiplying S by
+  // d^C per chunk took 512 of some 3,300 cycles of a chunk's issue, and rounded the weight of a far slot once
+  // per chunk). It is multiplied out when d^m would leave 2^+-20. Where 2^-16 is passed within one chunk S is
+  // multiplied by d^n for each, and the weights are d^(n-1-j).
+  const bool slow = fabsf(g2) * C < 16.f;
+  int m = 0;
+  float wk[NB][4];
+#pragma unroll
+  for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) wk[sb][r] = slow ? pw(g2, -(16 * sb + 4 * g + r + e)) * a.s_kv : 0.f;
 
   Rows<IO, C, DK, NT> rq, rk;
   Rows<IO, C, SL, NT> rv;
+  if (OUT) rq.init(q, a.sq.t, first, rows, a.reverse, 0);
+  rk.init(k, a.sk.t, first, rows, a.reverse, 0);
+  rv.init(v, a.sv.t, first, rows, a.reverse, c0);
   auto fetch = [&](int at) {
     const int n = min(C, end - at);
-    if (OUT) rq.fetch(q, a.sq.t, at, n, rows, a.reverse, 0, a.K);
-    rk.fetch(k, a.sk.t, at, n, rows, a.reverse, 0, a.K);
-    rv.fetch(v, a.sv.t, at, n, rows, a.reverse, c0, a.V);
+    if (OUT) rq.fetch(n, a.K);
+    rk.fetch(n, a.K);
+    rv.fetch(n, a.V - c0);
   };
   if (first < end) fetch(first);
   for (int at = first; at < end; at += C) {
@@ -286,6 +313,16 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
       for (int y = 0; y < NV; ++y) vf[sb][y] = quad_cols(vs, LV, 16 * sb, wave * 16 * NV + 16 * y, i, g);
 
     if (OUT) {
+      const float dm = pw(g2, m);
+      Quad sf[Ty::BF ? NK : 1][Ty::BF ? NV : 1];
+      if constexpr (Ty::BF) {
+        // the state enters this product rounded to bf16, the only place where it is: an error of at most
+        // half a step of the output's own type on its share of the sum
+#pragma unroll
+        for (int x = 0; x < NK; ++x)
+#pragma unroll
+          for (int y = 0; y < NV; ++y) sf[x][y] = to_bf(S[x][y]);
+      }
 #pragma unroll
       for (int tb = 0; tb < NB; ++tb) {
         if (16 * tb >= n) break;
@@ -297,19 +334,17 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
         for (int y = 0; y < NV; ++y) acc[y] = f4{0.f, 0.f, 0.f, 0.f};
         if (have) {
           if constexpr (Ty::BF) {
-            // the state enters this product rounded to bf16, the only place where it is: an error of at most
-            // half a step of the output's own type on its share of the sum
 #pragma unroll
             for (int x = 0; x < NK; x += 2)
 #pragma unroll
-              for (int y = 0; y < NV; ++y) acc[y] = mma32(to_bf(S[x][y]), to_bf(S[x + 1][y]), qf[x], qf[x + 1], acc[y]);
+              for (int y = 0; y < NV; ++y) acc[y] = mma32(sf[x][y], sf[x + 1][y], qf[x], qf[x + 1], acc[y]);
           } else {
 #pragma unroll
             for (int x = 0; x < NK; ++x)
 #pragma unroll
               for (int y = 0; y < NV; ++y) acc[y] = mma16(S[x][y], qf[x], acc[y]);
           }
-          const float f = rf * d16[tb];
+          const float f = rf * d16[tb] * dm;
 #pragma unroll
           for (int y = 0; y < NV; ++y) acc[y] *= f;
         }
@@ -370,27 +405,26 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
     }
 
     if (OUT && at + C >= end && !a.fin) break;  // nobody reads the state behind the last slot
-    if (have) {
-      float hi = dc_hi, lo = dc_lo;
-      if (n < C) {
-        const double dn = exp((double)n * (double)ld);
-        hi = (float)dn;
-        lo = (float)(dn - (double)hi);
+    float w[NB][4];
+    if (slow) {
+      if (fabsf(g2) * (float)(m + C) > 20.f) {
+        multiply_out(S, pw(g2, m));
+        m = 0;
       }
+      const float f = pw(g2, -m);
 #pragma unroll
-      for (int x = 0; x < NK; ++x)
+      for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
-        for (int y = 0; y < NV; ++y)
+        for (int r = 0; r < 4; ++r) w[sb][r] = wk[sb][r] * f;
+      m += n;
+    } else {
+      multiply_out(S, pw(g2, n));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) S[x][y][r] = fmaf(S[x][y][r], hi, S[x][y][r] * lo);
+      for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[sb][r] = pw(g2, max(0, n - e - (16 * sb + 4 * g + r))) * a.s_kv;
     }
     have = true;
-    float w[NB][4];
-#pragma unroll
-    for (int sb = 0; sb < NB; ++sb)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        w[sb][r] = n == C ? wb[r] * d16[NB - 1 - sb] : pw(g2, max(0, n - e - (16 * sb + 4 * g + r))) * a.s_kv;
     if constexpr (Ty::BF) {
       // the decayed v in three bf16 terms (24 bits): the state is as exact as products of the tensors in fp32
 #pragma unroll
@@ -445,6 +479,7 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
     for (long at = (long)from * wide + threadIdx.x; at < (long)to * wide; at += NT)
       Ty::store(o + at / wide * a.so.t + c0 + at % wide, 0.f);
   }
+  if (m) multiply_out(S, pw(g2, m));
   float* to = nullptr;
   int tk = a.V, tv = 1;
   if (OUT) {
@@ -467,8 +502,8 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
 }
 
 // Columns of V that a workgroup takes: 16 (one wave, as long as that wave can stage the rows of K in
-// few loads), 64 or 128.
-inline int slice_columns(int K, int V) { return V <= 16 && K <= 64 ? 16 : V <= 64 ? 64 : 128; }
+// few loads), 64, or 128 as long as its share of the state leaves a wave registers to work with.
+inline int slice_columns(int K, int V) { return V <= 16 && K <= 64 ? 16 : V <= 64 || K > 128 ? 64 : 128; }
 inline int chunk_slots(int dtype) { return dtype == CET_BF16 ? Type<__bf16>::C : Type<float>::C; }
 
 template <typename IO, int NK, bool OUT>
@@ -479,7 +514,7 @@ inline void launch_k(const Args& a, unsigned blocks, hipStream_t s) {
   } else if (cols == 64) {
     chunks<IO, NK, 1, 4, OUT><<<blocks, 256, 0, s>>>(a);
   } else {
-    chunks<IO, NK, 2, 4, OUT><<<blocks, 256, 0, s>>>(a);
+    if constexpr (NK <= 8) chunks<IO, NK, 2, 4, OUT><<<blocks, 256, 0, s>>>(a);
   }
 }
 

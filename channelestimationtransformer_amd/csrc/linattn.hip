@@ -13,18 +13,23 @@ constexpr size_t align_up(size_t n) { return (n + 255) & ~(size_t)255; }
 constexpr int elem_bytes(int dtype) { return dtype == CET_F32 ? 4 : 2; }
 
 // ws[bh][s] holds what segment s adds to the state; afterwards the state behind segment s (the one that
-// segment s + 1 starts from). One thread per state element, segments in order.
+// segment s + 1 starts from). One thread per state element, segments in order; blockIdx.y is the head.
 __global__ __launch_bounds__(256) void join_segments(const Args a) {
-  const long states = (long)a.K * a.V, at = (long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= states * a.B * a.H) return;
-  const long bh = at / states, e = at % states;
-  const double dn = exp((double)a.seg_len * (double)a.log_decay[bh % a.H]);
-  const float hi = (float)dn, lo = (float)(dn - (double)hi);
-  float cur = a.init ? a.init[bh * states + e / a.V * a.init_k + e % a.V * a.init_v] : 0.f;
+  const int states = a.K * a.V, e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= states) return;
+  const long bh = blockIdx.y;
+  const float d = pw(a.log_decay[bh % a.H] * 1.44269504088896340736f, a.seg_len);
+  float cur = a.init ? a.init[bh * states + (long)(e / a.V) * a.init_k + (long)(e % a.V) * a.init_v] : 0.f;
   float* p = a.ws + bh * (a.nseg - 1) * states + e;
-  for (int s = 0; s < a.nseg - 1; ++s, p += states) {
-    cur = fmaf(cur, hi, cur * lo) + *p;
-    *p = cur;
+  for (int s0 = 0; s0 < a.nseg - 1; s0 += 8) {
+    float add[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) add[j] = s0 + j < a.nseg - 1 ? p[(long)(s0 + j) * states] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      cur = fmaf(cur, d, add[j]);
+      if (s0 + j < a.nseg - 1) p[(long)(s0 + j) * states] = cur;
+    }
   }
 }
 
@@ -220,7 +225,7 @@ int pass(Args a, const Cut& c, int dtype, hipStream_t s) {
   const long bh = (long)a.B * a.H;
   if (c.nseg > 1) {
     if (const int rc = launch(a, false, (unsigned)(bh * (c.nseg - 1) * c.nslice), dtype, s)) return rc;
-    join_segments<<<(unsigned)((bh * a.K * a.V + 255) / 256), 256, 0, s>>>(a);
+    join_segments<<<dim3((unsigned)((a.K * a.V + 255) / 256), (unsigned)bh), 256, 0, s>>>(a);
     CET_HIP(hipGetLastError());
   }
   return launch(a, true, (unsigned)(bh * c.nseg * c.nslice), dtype, s);
