@@ -13,14 +13,12 @@
 // last state enters the last slot undecayed and the carry at the end is that of the first state.
 //
 // One wave owns 16 NV columns of V and all of K: S stays in its accumulators from the first chunk to
-// the last, and the waves of a workgroup share nothing but the staged rows of q, k and v, so a chunk
-// costs two barriers. All products are laid out so that an accumulator is the next product's operand
+// the last, and the waves of a workgroup share nothing but the staged rows of q, k and v and the scores, so a chunk
+// costs one or two barriers. All products are laid out so that an accumulator is the next product's operand
 // without a move: a 16 x 16 tile holds, in lane (i = l % 16, g = l / 16), rows 4g..4g+3 of column i,
 // and an operand of the matrix instructions holds k = 4g..4g+3 of row i, the same values:
 //     P^T = K Q^T (columns: slots of q)     -> O^T += V^T P^T takes P^T as it is,
 //     S  += K^T V (rows K, columns V)       -> O^T += S^T Q^T takes S as it is.
-// The columns of V that each wave recomputes P for cost 16 x 16 x K operations per block; handing P
-// over through LDS instead would cost a third barrier per chunk.
 #pragma once
 
 #include <hip/hip_bf16.h>
@@ -41,13 +39,13 @@ struct Args {
   const void *q, *k, *v;
   void* o;
   const float* init;       // state before the first slot (nullptr: zero), element (k, v) at k * init_k + v * init_v
-  float* fin;              // state after the last slot (nullptr: not wanted), same addressing
+  float* fin;              // state after the last slot [B * H][K][V] (nullptr: not wanted)
   const float* log_decay;  // [H]
   const void* lengths;     // [B] int32 or int64 (nullptr: all T)
-  float* ws;               // [B * H][nseg - 1][K * V]
+  float* ws;               // states between segments: [B * H][nseg - 1] states, element (k, v) at k * ws_k + v * ws_v
   Strides sq, sk, sv, so;
   int B, T, H, K, V;
-  int init_k, init_v, fin_k, fin_v;
+  int init_k, init_v, ws_k, ws_v;
   int lengths64, reverse;
   int seg_len, nseg, nslice;
   int vec_o;  // rows of o start on the boundaries that stores of four need (those of q, k and v always do)
@@ -61,8 +59,19 @@ typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
+template <bool B, typename X, typename Y>
+struct Pick {
+  typedef X T;
+};
+template <typename X, typename Y>
+struct Pick<false, X, Y> {
+  typedef Y T;
+};
+
 // d^n with d^0 = 1 also for d = 0 (a log decay of minus infinity)
 __device__ inline float pw(float g2, int n) { return n == 0 ? 1.f : exp2f((float)n * g2); }
+// the same without denormal results (below 2^-126 they are zero), in one instruction
+__device__ inline float pw_fast(float g2, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f((float)n * g2); }
 
 __device__ inline int row_count(const Args& a, int b) {
   if (!a.lengths) return a.T;
@@ -72,53 +81,23 @@ __device__ inline int row_count(const Args& a, int b) {
 
 // The arithmetic of a tensor type. float32 and float16 tensors are multiplied in fp32 (a float16
 // state or score would leave that type's range on long histories), bfloat16 ones in bf16.
+
+// Slots of a chunk: 32 with outputs, 64 where only states are formed (fewer barriers; no scores to hold).
+constexpr int OUT_SLOTS = 32, STATE_SLOTS = 64;
+
 template <typename IO>
-struct Type;
-
-template <>
-struct Type<float> {
-  typedef float Lds;
-  typedef f4 Quad;  // four values of an operand: k = 4g..4g+3
-  static constexpr bool BF = false;
-  static constexpr int VEC = 4, C = 32, LDPAD = 4;
-  __device__ static void to_lds(float* p, const uint4& raw) { *reinterpret_cast<uint4*>(p) = raw; }
-  __device__ static float load(const float* p) { return *p; }
-  __device__ static void store(float* p, float v) { *p = v; }
-  __device__ static void store4(float* p, const f4& v) { *reinterpret_cast<f4*>(p) = v; }
-};
-
-template <>
-struct Type<_Float16> {
-  typedef float Lds;
-  typedef f4 Quad;
-  static constexpr bool BF = false;
-  static constexpr int VEC = 8, C = 32, LDPAD = 4;
-  __device__ static void to_lds(float* p, const uint4& raw) {
-    const h8 v = *reinterpret_cast<const h8*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<f4*>(p + 4 * i) = f4{(float)v[4 * i], (float)v[4 * i + 1], (float)v[4 * i + 2], (float)v[4 * i + 3]};
+struct Type {
+  typedef IO V4 __attribute__((ext_vector_type(4)));
+  static constexpr bool BF = __is_same(IO, __bf16);
+  typedef typename Pick<BF, bf4, f4>::T Quad;  // four values of an operand: k = 4g..4g+3
+  __device__ static Quad quad(const V4& v) {
+    if constexpr (BF || __is_same(IO, float))
+      return v;
+    else
+      return f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
   }
-  __device__ static float load(const _Float16* p) { return (float)*p; }
-  __device__ static void store(_Float16* p, float v) { *p = (_Float16)v; }
-  __device__ static void store4(_Float16* p, const f4& v) {
-    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<h4*>(p) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-  }
-};
-
-template <>
-struct Type<__bf16> {
-  typedef __bf16 Lds;
-  typedef bf4 Quad;
-  static constexpr bool BF = true;
-  static constexpr int VEC = 8, C = 32, LDPAD = 8;
-  __device__ static void to_lds(__bf16* p, const uint4& raw) { *reinterpret_cast<uint4*>(p) = raw; }
-  __device__ static float load(const __bf16* p) { return (float)*p; }
-  __device__ static void store(__bf16* p, float v) { *p = (__bf16)v; }
-  __device__ static void store4(__bf16* p, const f4& v) {
-    *reinterpret_cast<bf4*>(p) = bf4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-  }
+  __device__ static void store(IO* p, float v) { *p = (IO)v; }
+  __device__ static void store4(IO* p, const f4& v) { *reinterpret_cast<V4*>(p) = V4{(IO)v[0], (IO)v[1], (IO)v[2], (IO)v[3]}; }
 };
 
 // acc += A B over 16 values of k in one tile (fp32: four instructions of k = 4)
@@ -136,63 +115,80 @@ __device__ inline f4 mma32(const bf4& a0, const bf4& a1, const bf4& b0, const bf
 __device__ inline bf4 to_bf(const f4& v) { return bf4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}; }
 __device__ inline f4 to_f(const bf4& v) { return f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
 
-// rows r0..r0+15, k columns c0..c0+15 of a row-major tile as an operand (k = columns)
-__device__ inline f4 quad_rows(const float* t, int ld, int r0, int c0, int i, int g) {
-  return *reinterpret_cast<const f4*>(t + (r0 + i) * ld + c0 + 4 * g);
+__device__ inline unsigned lds_address(const void* p) {
+  return (unsigned)(unsigned long)(const __attribute__((address_space(3))) char*)p;
 }
-__device__ inline bf4 quad_rows(const __bf16* t, int ld, int r0, int c0, int i, int g) {
-  return *reinterpret_cast<const bf4*>(t + (r0 + i) * ld + c0 + 4 * g);
+// 16 bytes per lane straight into LDS at lds + 16 * lane, in assembly: loads into registers are waited for by the
+// compiler wherever it merges or copies them, which left a chunk's rows no time to travel. The waits below order them.
+__device__ inline void dma16(const void* src, unsigned lds_wave) {
+  unsigned keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(src), "s"(lds_wave)
+      : "memory");
 }
-// the same tile as an operand with k = rows: bf16 through the transposing LDS read, which hands lane
-// i of each 16 the column i of the four rows that the 16 lanes read 8 bytes of each
-__device__ inline f4 quad_cols(const float* t, int ld, int r0, int c0, int i, int g) {
-  const float* p = t + (r0 + 4 * g) * ld + c0 + i;
-  return f4{p[0], p[ld], p[2 * ld], p[3 * ld]};
-}
-__device__ inline bf4 quad_cols(const __bf16* t, int ld, int r0, int c0, int i, int g) {
-  typedef __attribute__((address_space(3))) s4* lds_s4;
-  const __bf16* p = t + (r0 + 4 * g + (i >> 2)) * ld + c0 + 4 * (i & 3);
-  const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p);
-  return __builtin_bit_cast(bf4, r);
-}
+static __device__ const uint4 zeros = {0, 0, 0, 0};
 
-// Rows of consecutive chunks on their way from memory to LDS: C rows of COLS columns over NT threads. A
-// thread keeps the address of each of its pieces and moves it on by a chunk with every fetch.
-template <typename IO, int C, int COLS, int NT>
-struct Rows {
-  typedef Type<IO> Ty;
-  static constexpr int VEC = Ty::VEC, PER_ROW = COLS / VEC, TOTAL = C * PER_ROW, N = (TOTAL + NT - 1) / NT;
-  uint4 raw[N];
-  const char* at[N];
-  long step;  // bytes from chunk to chunk
+// The SLOTS rows of a chunk in LDS, COLS columns in 16-byte pieces. Piece p of row r lies at p ^ turn(r), so that the
+// reads of a wave touch all banks equally often; LDS takes the pieces in the order of the lanes, so the
+// permutation is made on the memory side. Rows as an operand: 16 rows of one piece (fp32) or of one half piece.
+// Columns as an operand: fp32 rows 4g + r of four pieces each, 2-byte types rows of two pieces each through the
+// transposing read, which hands lane i of each 16 the column i of the four rows that they read 8 bytes of each.
+template <typename IO, int COLS, int SLOTS>
+struct Tile {
+  static constexpr int E = sizeof(IO), VEC = 16 / E, P = COLS / VEC, PB = P < 16 ? P : 16, SHARE256 = 16 / PB;
+  static constexpr int BYTES = SLOTS * COLS * E, PARTS = BYTES / 1024;  // a part: what one instruction of a wave brings
+  typedef typename Type<IO>::V4 V4;
+  typedef typename Type<IO>::Quad Quad;
 
-  __device__ static int row_of(int u) { return (u * NT + (int)threadIdx.x) / PER_ROW; }
-  __device__ static int col_of(int u) { return (u * NT + (int)threadIdx.x) % PER_ROW * VEC; }
-
-  // place i of the sequence is slot i, or rows - 1 - i backward in time; the first fetch takes places i0..
-  __device__ void init(const IO* p, long st, int i0, int rows, int reverse, int c0) {
-    step = (reverse ? -C : C) * st * (long)sizeof(IO);
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      const long place = i0 + row_of(u);
-      at[u] = reinterpret_cast<const char*>(p + (reverse ? rows - 1 - place : place) * st + c0 + col_of(u));
-    }
+  __device__ static int turn(int r) {
+    const int u = r / SHARE256;  // rows of this many share the banks' 256 bytes
+    return E == 2 ? ((u & (PB / 2 - 1)) << 1 | (r >> 3 & 1)) & (PB - 1) : u & (PB - 1);
   }
-  // rows from n on and columns from `cols` (counted from c0) on are zero
-  __device__ void fetch(int n, int cols) {
-#pragma unroll
-    for (int u = 0; u < N; ++u) {
-      raw[u] = uint4{0, 0, 0, 0};
-      if (row_of(u) < n && col_of(u) < cols) raw[u] = *reinterpret_cast<const uint4*>(at[u]);
-      at[u] += step;
-    }
+  __device__ static Quad rows(const char* t, int r0, int c0, int i, int g) {
+    const int r = r0 + i;
+    const char* p = E == 2 ? t + r * (COLS * E) + ((c0 / VEC + (g >> 1) ^ turn(r)) << 4) + (g & 1) * 8
+                           : t + r * (COLS * E) + ((c0 / VEC + g ^ turn(r)) << 4);
+    return Type<IO>::quad(*reinterpret_cast<const V4*>(p));
   }
-  __device__ void put(typename Ty::Lds* lds, int ld) const {
+  __device__ static Quad cols(const char* t, int r0, int c0, int i, int g) {
+    if constexpr (E == 2) {
+      typedef __attribute__((address_space(3))) s4* lds_s4;
+      const int r = r0 + 4 * g + (i >> 2);
+      const char* p = t + r * (COLS * E) + ((c0 / VEC + (i >> 1 & 1) ^ turn(r)) << 4) + (i & 1) * 8;
+      return Type<IO>::quad(__builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p)));
+    } else {
+      f4 v;
 #pragma unroll
-    for (int u = 0; u < N; ++u)
-      if (TOTAL % NT == 0 || row_of(u) < C) Ty::to_lds(lds + row_of(u) * ld + col_of(u), raw[u]);
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + 4 * g + j, c = c0 + i;
+        v[j] = *reinterpret_cast<const float*>(t + r * (COLS * E) + ((c / VEC ^ turn(r)) << 4) + (c & 3) * 4);
+      }
+      return v;
+    }
   }
 };
+
+// One operand in memory: place i of the sequence is slot i, or rows - 1 - i backward in time. Places from `end`
+// on and columns from `cols` on do not exist and are zero.
+struct Source {
+  const char* base;  // first place, first column
+  long st;           // bytes from place to place
+  int end, cols;
+
+  template <typename Ti>
+  __device__ void fetch(int part, int i0, unsigned lds, int lane) const {
+    const int at = part * 64 + lane, r = at / Ti::P, c = (at % Ti::P ^ Ti::turn(r)) * Ti::VEC;
+    const char* p = base + (i0 + r) * st + c * Ti::E;
+    dma16(i0 + r < end && c < cols ? p : reinterpret_cast<const char*>(&zeros), lds + part * 1024);
+  }
+};
+template <typename IO>
+__device__ inline Source source(const IO* p, long st, int rows, int end, int reverse, int c0, int cols) {
+  return Source{reinterpret_cast<const char*>(p + c0 + (reverse ? (rows - 1) * st : 0)), (reverse ? -st : st) * (long)sizeof(IO), end, cols - c0};
+}
 
 template <int NK, int NV>
 __device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
@@ -202,21 +198,43 @@ __device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
     for (int y = 0; y < NV; ++y) S[x][y] *= f;
 }
 
-// OUT: with outputs; without, only the state that a segment of slots adds is formed (into ws).
-template <typename IO, int NK, int NV, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(const Args a) {
+// A workgroup is WC x KH waves: WC side by side along V, 16 NV columns each, and KH (1 or 2) that share the K of
+// those columns. OUT: with outputs; without, only the state that a segment of slots adds is formed (into ws).
+//
+// Per chunk and wave: its blocks of the scores into LDS; its part of q S; what the chunk adds to its part of S; the
+// one barrier; the rows of a later chunk asked for; scores times v, and the outputs. With two waves to the K of a
+// column each finishes the outputs of one block of 16 slots, with the other's half of q S for it, which comes
+// through LDS behind the same barrier.
+template <typename IO, int NK, int NV, int WC, int KH, bool OUT>
+__global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(const Args a) {
   typedef Type<IO> Ty;
-  typedef typename Ty::Lds Lds;
   typedef typename Ty::Quad Quad;
-  constexpr int C = Ty::C, NB = C / 16, NT = 64 * NW, DK = 16 * NK, SL = 16 * NV * NW;
-  constexpr int LK = DK + Ty::LDPAD, LV = SL + Ty::LDPAD;
-  __shared__ __align__(16) Lds qs[OUT ? C * LK : 1];
-  __shared__ __align__(16) Lds ks[C * LK];
-  __shared__ __align__(16) Lds vs[C * LV];
+  constexpr int C = OUT ? OUT_SLOTS : STATE_SLOTS, NB = C / 16;
+  constexpr int NW = WC * KH, DK = 16 * NK, NKW = NK / KH, SL = 16 * NV * WC;
+  constexpr bool SHARE = NW > 1;  // one wave keeps its scores
+  constexpr int BLOCKS = NB * (NB + 1) / 2, MINE = KH == 2 ? 1 : NB;
+  static_assert((!OUT || NB == 2) && KH <= 2 && NK % KH == 0, "two blocks of slots in a chunk with outputs");
+  typedef Tile<IO, DK, C> TK;
+  typedef Tile<IO, SL, C> TV;
+  // Buffers in a ring: rows of chunk c + BUFS are asked for when everybody has left chunk c.
+  constexpr int BUF = (OUT ? 2 : 1) * TK::BYTES + TV::BYTES;
+  // Three where that leaves room for two workgroups on a CU, or where two would not either.
+  constexpr int REST = (OUT && SHARE ? 2 * BLOCKS * 64 * (int)sizeof(Quad) : 0) + (OUT && KH == 2 ? 2 * NW * NV * 1024 : 0) + 2048;
+  constexpr int BUFS = SHARE && (3 * BUF + REST <= 81920 || (2 * BUF + REST > 81920 && 3 * BUF + REST <= 163840)) ? 3 : 2;
+  constexpr int PARTS = BUF / 1024, PER = PARTS / NW, EXTRA = PARTS % NW;  // of a chunk; of each wave; of the first waves
+  __shared__ __align__(1024) char tiles[BUFS][BUF];
+  __shared__ Quad ps[2][OUT && SHARE ? BLOCKS : 1][64];
+  __shared__ f4 xs[2][OUT && KH == 2 ? NW : 1][NV][64];
 
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, kh = wave / WC;
+  // Workgroups go to the 8 XCDs in turn: an XCD is given one run of them, so that the slices of a head, which
+  // read the same q and k, share its L2.
   unsigned id = blockIdx.x;
+  {
+    const unsigned per = gridDim.x / 8, rest = gridDim.x % 8, xcd = id % 8;
+    id = xcd * per + min(xcd, rest) + id / 8;
+  }
   const int slice = id % a.nslice;
   id /= a.nslice;
   const int nseg_here = OUT ? a.nseg : a.nseg - 1;  // without outputs the last segment has nothing to add
@@ -226,16 +244,37 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
   const int rows = row_count(a, b);
   const int first = seg * a.seg_len;
   const int end = min(rows, first + a.seg_len);
-  const int c0 = slice * SL, col = c0 + wave * 16 * NV;  // first column of V: of the workgroup, of the wave
+  const int c0 = slice * SL, col = c0 + wc * 16 * NV;  // first column of V: of the workgroup, of the wave
+  const int k0 = kh * NKW * 16;                        // first row of the wave's part of S
 
   const IO* q = static_cast<const IO*>(a.q) + b * a.sq.b + h * a.sq.h;
   const IO* k = static_cast<const IO*>(a.k) + b * a.sk.b + h * a.sk.h;
   const IO* v = static_cast<const IO*>(a.v) + b * a.sv.b + h * a.sv.h;
   IO* o = OUT ? static_cast<IO*>(a.o) + b * a.so.b + h * a.so.h : nullptr;
 
-  f4 S[NK][NV];
+  const Source from_q = source(q, a.sq.t, rows, end, a.reverse, 0, a.K), from_k = source(k, a.sk.t, rows, end, a.reverse, 0, a.K);
+  const Source from_v = source(v, a.sv.t, rows, end, a.reverse, c0, a.V);
+  const unsigned lds = lds_address(tiles);
+  auto fetch = [&](int at, int buf) {  // this wave's parts of a chunk's rows: k, v, q one behind the other
+    const unsigned to = lds + buf * BUF;
 #pragma unroll
-  for (int x = 0; x < NK; ++x)
+    for (int u = 0; u < PER + (EXTRA ? 1 : 0); ++u) {
+      const int part = u * NW + wave;
+      if (part < TK::PARTS)
+        from_k.fetch<TK>(part, at, to, lane);
+      else if (part < TK::PARTS + TV::PARTS)
+        from_v.fetch<TV>(part - TK::PARTS, at, to + TK::BYTES, lane);
+      else if (OUT && part < PARTS)
+        from_q.fetch<TK>(part - TK::PARTS - TV::PARTS, at, to + TK::BYTES + TV::BYTES, lane);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < BUFS; ++u)
+    if (first + u * C < end) fetch(first + u * C, u);
+
+  f4 S[NKW][NV];
+#pragma unroll
+  for (int x = 0; x < NKW; ++x)
 #pragma unroll
     for (int y = 0; y < NV; ++y) S[x][y] = f4{0.f, 0.f, 0.f, 0.f};
 
@@ -243,16 +282,24 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
   bool have = false;  // S is not all zero
   if (OUT) {
     const float* from = seg ? a.ws + (bh * (a.nseg - 1) + seg - 1) * states : a.init ? a.init + bh * states : nullptr;
-    const int fk = seg ? a.V : a.init_k, fv = seg ? 1 : a.init_v;
+    const int fk = seg ? a.ws_k : a.init_k, fv = seg ? a.ws_v : a.init_v;
     have = from != nullptr && (first < end || seg == 0);
-    if (have) {
+    if (have && fk == 1 && a.K % 4 == 0) {  // a transposed state: four neighbours at once (states start on 16 bytes)
 #pragma unroll
-      for (int x = 0; x < NK; ++x)
+      for (int x = 0; x < NKW; ++x)
+#pragma unroll
+        for (int y = 0; y < NV; ++y) {
+          const int kk = k0 + 16 * x + 4 * g, vv = col + 16 * y + i;
+          if (kk < a.K && vv < a.V) S[x][y] = *reinterpret_cast<const f4*>(from + kk + (long)vv * fv);
+        }
+    } else if (have) {
+#pragma unroll
+      for (int x = 0; x < NKW; ++x)
 #pragma unroll
         for (int y = 0; y < NV; ++y)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int kk = 16 * x + 4 * g + r, vv = col + 16 * y + i;
+            const int kk = k0 + 16 * x + 4 * g + r, vv = col + 16 * y + i;
             if (kk < a.K && vv < a.V) S[x][y][r] = from[(long)kk * fk + (long)vv * fv];
           }
     }
@@ -260,23 +307,18 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
 
   const float g2 = a.log_decay[h] * 1.44269504088896340736f;
   const int e = a.reverse ? 0 : 1;
-  // scores: same block (masked), next block; further blocks by d^16 each
-  float wd[4], wo[4];
+  float wd[4], wo[4];  // scores of a block with itself (masked) and with the one before
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int s = 4 * g + r;
     wd[r] = i >= s ? pw(g2, i - s) * a.s_intra : 0.f;
     wo[r] = pw(g2, 16 + i - s) * a.s_intra;
   }
-  float d16[NB];
-#pragma unroll
-  for (int x = 0; x < NB; ++x) d16[x] = pw(g2, 16 * x);
-  const float rf = pw(g2, i + e) * a.s_inter;
+  const float rf[OUT_SLOTS / 16] = {pw(g2, i + e) * a.s_inter, pw(g2, 16 + i + e) * a.s_inter};
   // A state that fades slowly is kept as S / d^m, m slots since it was last multiplied out: a chunk then adds
-  // its keys and values by the weights d^-(m + 1 + j) and touches no element of S otherwise (multiplying S by
-  // d^C per chunk took 512 of some 3,300 cycles of a chunk's issue, and rounded the weight of a far slot once
-  // per chunk). It is multiplied out when d^m would leave 2^+-20. Where 2^-16 is passed within one chunk S is
-  // multiplied by d^n for each, and the weights are d^(n-1-j).
+  // its keys and values by the weights d^-(m + 1 + j) and touches no element of S otherwise, and the weight of
+  // a slot far back is not rounded once per chunk. It is multiplied out when d^m would leave 2^+-20. Where 2^-16
+  // is passed within one chunk S is multiplied by d^n for each, and the weights are d^(n-1-j).
   const bool slow = fabsf(g2) * C < 16.f;
   int m = 0;
   float wk[NB][4];
@@ -285,151 +327,118 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
 #pragma unroll
     for (int r = 0; r < 4; ++r) wk[sb][r] = slow ? pw(g2, -(16 * sb + 4 * g + r + e)) * a.s_kv : 0.f;
 
-  Rows<IO, C, DK, NT> rq, rk;
-  Rows<IO, C, SL, NT> rv;
-  if (OUT) rq.init(q, a.sq.t, first, rows, a.reverse, 0);
-  rk.init(k, a.sk.t, first, rows, a.reverse, 0);
-  rv.init(v, a.sv.t, first, rows, a.reverse, c0);
-  auto fetch = [&](int at) {
-    const int n = min(C, end - at);
-    if (OUT) rq.fetch(n, a.K);
-    rk.fetch(n, a.K);
-    rv.fetch(n, a.V - c0);
+  // block (tb, sb) of the scores, decayed, as an operand
+  auto scores = [&](const char* qt, const char* kt, int tb, int sb) {
+    f4 p = f4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (Ty::BF) {
+#pragma unroll
+      for (int x = 0; x < NK; x += 2)
+        p = mma32(TK::rows(kt, 16 * sb, 16 * x, i, g), TK::rows(kt, 16 * sb, 16 * x + 16, i, g),
+                  TK::rows(qt, 16 * tb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x + 16, i, g), p);
+    } else {
+#pragma unroll
+      for (int x = 0; x < NK; ++x) p = mma16(TK::rows(kt, 16 * sb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x, i, g), p);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = sb == tb ? (i >= 4 * g + r ? p[r] * wd[r] : 0.f) : p[r] * wo[r];
+    if constexpr (Ty::BF)
+      return to_bf(p);  // rounded to the tensors' type for the second product, as its sum will be
+    else
+      return p;
   };
-  if (first < end) fetch(first);
+
+  IO* po[MINE];  // where this lane's slots of the chunk go
+  const long po_step = (a.reverse ? -C : C) * a.so.t;
+#pragma unroll
+  for (int t = 0; t < MINE; ++t) {
+    const long place = first + 16 * (KH == 2 ? kh : t) + i;
+    po[t] = o + (a.reverse ? rows - 1 - place : place) * a.so.t + col + 4 * g;
+  }
+
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int buf = 0;
   for (int at = first; at < end; at += C) {
     const int n = min(C, end - at);
-    if (at != first) __syncthreads();  // the products of the chunk before have read their rows
-    if (OUT) rq.put(qs, LK);
-    rk.put(ks, LK);
-    rv.put(vs, LV);
-    __syncthreads();
-    if (at + C < end) fetch(at + C);  // on their way while this chunk is computed
+    const char *kt = tiles[buf], *vt = kt + TK::BYTES, *qt = vt + TV::BYTES;
 
     Quad vf[NB][NV];
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
-      for (int y = 0; y < NV; ++y) vf[sb][y] = quad_cols(vs, LV, 16 * sb, wave * 16 * NV + 16 * y, i, g);
+      for (int y = 0; y < NV; ++y) vf[sb][y] = TV::cols(vt, 16 * sb, wc * 16 * NV + 16 * y, i, g);
 
+    f4 acc[OUT ? NB : 1][NV];
+    Quad pf[OUT ? BLOCKS : 1];
+    const int flip = (at / C) & 1;
     if (OUT) {
-      const float dm = pw(g2, m);
-      Quad sf[Ty::BF ? NK : 1][Ty::BF ? NV : 1];
-      if constexpr (Ty::BF) {
-        // the state enters this product rounded to bf16, the only place where it is: an error of at most
-        // half a step of the output's own type on its share of the sum
+      constexpr int TB[3] = {0, 1, 1}, SB[3] = {0, 0, 1};  // the blocks on and below the diagonal
 #pragma unroll
-        for (int x = 0; x < NK; ++x)
-#pragma unroll
-          for (int y = 0; y < NV; ++y) sf[x][y] = to_bf(S[x][y]);
+      for (int x = 0; x < BLOCKS; ++x) {
+        if constexpr (SHARE) {
+          if (x % NW == wave) ps[flip][x][lane] = scores(qt, kt, TB[x], SB[x]);
+        } else {
+          pf[x] = scores(qt, kt, TB[x], SB[x]);
+        }
       }
 #pragma unroll
-      for (int tb = 0; tb < NB; ++tb) {
-        if (16 * tb >= n) break;
-        Quad qf[NK];
+      for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
-        for (int x = 0; x < NK; ++x) qf[x] = quad_rows(qs, LK, 16 * tb, 16 * x, i, g);
-        f4 acc[NV];
+        for (int y = 0; y < NV; ++y) acc[tb][y] = f4{0.f, 0.f, 0.f, 0.f};
+      if (have) {
+        // the state enters this product rounded to bf16 (where the tensors are), the only place where it is: an
+        // error of at most half a step of the output's own type on its share of the sum
+        const float dm = pw_fast(g2, m);
 #pragma unroll
-        for (int y = 0; y < NV; ++y) acc[y] = f4{0.f, 0.f, 0.f, 0.f};
-        if (have) {
-          if constexpr (Ty::BF) {
+        for (int x = 0; x < NKW; x += Ty::BF ? 2 : 1)
 #pragma unroll
-            for (int x = 0; x < NK; x += 2)
+          for (int tb = 0; tb < NB; ++tb) {
+            if constexpr (Ty::BF) {
+              const Quad q0 = TK::rows(qt, 16 * tb, k0 + 16 * x, i, g), q1 = TK::rows(qt, 16 * tb, k0 + 16 * x + 16, i, g);
 #pragma unroll
-              for (int y = 0; y < NV; ++y) acc[y] = mma32(sf[x][y], sf[x + 1][y], qf[x], qf[x + 1], acc[y]);
-          } else {
-#pragma unroll
-            for (int x = 0; x < NK; ++x)
-#pragma unroll
-              for (int y = 0; y < NV; ++y) acc[y] = mma16(S[x][y], qf[x], acc[y]);
-          }
-          const float f = rf * d16[tb] * dm;
-#pragma unroll
-          for (int y = 0; y < NV; ++y) acc[y] *= f;
-        }
-        Quad pf[NB];
-#pragma unroll
-        for (int sb = 0; sb < NB; ++sb) {
-          if (sb > tb) continue;
-          f4 p = f4{0.f, 0.f, 0.f, 0.f};
-          if constexpr (Ty::BF) {
-#pragma unroll
-            for (int x = 0; x < NK; x += 2)
-              p = mma32(quad_rows(ks, LK, 16 * sb, 16 * x, i, g), quad_rows(ks, LK, 16 * sb, 16 * x + 16, i, g), qf[x], qf[x + 1], p);
-          } else {
-#pragma unroll
-            for (int x = 0; x < NK; ++x) p = mma16(quad_rows(ks, LK, 16 * sb, 16 * x, i, g), qf[x], p);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) p[r] = sb == tb ? (i >= 4 * g + r ? p[r] * wd[r] : 0.f) : p[r] * (wo[r] * d16[tb - sb - 1]);
-          if constexpr (Ty::BF) {
-            pf[sb] = to_bf(p);  // scores rounded to the tensors' type for the second product, as their sum will be
-          } else {
-            pf[sb] = p;
-          }
-        }
-        if constexpr (Ty::BF) {
-          const bf4 none = bf4{(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
-#pragma unroll
-          for (int sb = 0; sb < NB; sb += 2) {
-            if (sb > tb) continue;
-#pragma unroll
-            for (int y = 0; y < NV; ++y)
-              acc[y] = mma32(vf[sb][y], sb + 1 <= tb ? vf[sb + 1][y] : none, pf[sb], sb + 1 <= tb ? pf[sb + 1] : none, acc[y]);
-          }
-        } else {
-#pragma unroll
-          for (int sb = 0; sb < NB; ++sb) {
-            if (sb > tb) continue;
-#pragma unroll
-            for (int y = 0; y < NV; ++y) acc[y] = mma16(vf[sb][y], pf[sb], acc[y]);
-          }
-        }
-        const int place = 16 * tb + i;
-        if (place < n) {
-          IO* po = o + (long)(a.reverse ? rows - 1 - (at + place) : at + place) * a.so.t;
-#pragma unroll
-          for (int y = 0; y < NV; ++y) {
-            const int vv = col + 16 * y + 4 * g;
-            if (a.vec_o && vv + 4 <= a.V) {
-              Ty::store4(po + vv, acc[y]);
+              for (int y = 0; y < NV; ++y) acc[tb][y] = mma32(to_bf(S[x][y]), to_bf(S[x + 1][y]), q0, q1, acc[tb][y]);
             } else {
+              const Quad q0 = TK::rows(qt, 16 * tb, k0 + 16 * x, i, g);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (vv + r < a.V) Ty::store(po + vv + r, acc[y][r]);
+              for (int y = 0; y < NV; ++y) acc[tb][y] = mma16(S[x][y], q0, acc[tb][y]);
             }
           }
-        }
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+          for (int y = 0; y < NV; ++y) acc[tb][y] *= rf[tb] * dm;
+      }
+      if constexpr (KH == 2) {
+#pragma unroll
+        for (int y = 0; y < NV; ++y) xs[flip][wave][y][lane] = kh ? acc[0][y] : acc[1][y];
       }
     }
 
-    if (OUT && at + C >= end && !a.fin) break;  // nobody reads the state behind the last slot
-    float w[NB][4];
-    if (slow) {
-      if (fabsf(g2) * (float)(m + C) > 20.f) {
-        multiply_out(S, pw(g2, m));
-        m = 0;
+    if (!OUT || at + C < end || a.fin) {  // nobody reads the state behind the last slot otherwise
+      float w[NB][4];
+      if (slow) {
+        if (fabsf(g2) * (float)(m + C) > 20.f) {
+          multiply_out(S, pw(g2, m));
+          m = 0;
+        }
+        const float f = pw_fast(g2, -m);
+#pragma unroll
+        for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[sb][r] = wk[sb][r] * f;
+        m += n;
+      } else {
+        multiply_out(S, pw(g2, n));
+#pragma unroll
+        for (int sb = 0; sb < NB; ++sb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[sb][r] = pw_fast(g2, max(0, n - e - (16 * sb + 4 * g + r))) * a.s_kv;
       }
-      const float f = pw(g2, -m);
+      if constexpr (Ty::BF) {
 #pragma unroll
-      for (int sb = 0; sb < NB; ++sb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w[sb][r] = wk[sb][r] * f;
-      m += n;
-    } else {
-      multiply_out(S, pw(g2, n));
-#pragma unroll
-      for (int sb = 0; sb < NB; ++sb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) w[sb][r] = pw(g2, max(0, n - e - (16 * sb + 4 * g + r))) * a.s_kv;
-    }
-    have = true;
-    if constexpr (Ty::BF) {
-      // the decayed v in three bf16 terms (24 bits): the state is as exact as products of the tensors in fp32
-#pragma unroll
-      for (int sb = 0; sb < NB; sb += 2) {
+       for (int sb = 0; sb < NB; sb += 2) {
         if (16 * sb >= n) break;
+        // the decayed v in three bf16 terms (24 bits): the state is as exact as products of the tensors in fp32
         bf4 t0[2][NV], t1[2][NV], t2[2][NV];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -444,30 +453,86 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
             t2[u][y] = to_bf(x1 - to_f(t1[u][y]));
           }
 #pragma unroll
-        for (int x = 0; x < NK; ++x) {
-          const bf4 k0 = quad_cols(ks, LK, 16 * sb, 16 * x, i, g), k1 = quad_cols(ks, LK, 16 * sb + 16, 16 * x, i, g);
+        for (int x = 0; x < NKW; ++x) {
+          const bf4 kq0 = TK::cols(kt, 16 * sb, k0 + 16 * x, i, g), kq1 = TK::cols(kt, 16 * sb + 16, k0 + 16 * x, i, g);
 #pragma unroll
           for (int y = 0; y < NV; ++y) {
-            S[x][y] = mma32(k0, k1, t2[0][y], t2[1][y], S[x][y]);
-            S[x][y] = mma32(k0, k1, t1[0][y], t1[1][y], S[x][y]);
-            S[x][y] = mma32(k0, k1, t0[0][y], t0[1][y], S[x][y]);
+            S[x][y] = mma32(kq0, kq1, t2[0][y], t2[1][y], S[x][y]);
+            S[x][y] = mma32(kq0, kq1, t1[0][y], t1[1][y], S[x][y]);
+            S[x][y] = mma32(kq0, kq1, t0[0][y], t0[1][y], S[x][y]);
+          }
+        }
+       }
+      } else {
+#pragma unroll
+        for (int sb = 0; sb < NB; ++sb) {
+          if (16 * sb >= n) break;
+          f4 vw[NV];
+#pragma unroll
+          for (int y = 0; y < NV; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vw[y][r] = vf[sb][y][r] * w[sb][r];
+#pragma unroll
+          for (int x = 0; x < NKW; ++x) {
+            const f4 kq = TK::cols(kt, 16 * sb, k0 + 16 * x, i, g);
+#pragma unroll
+            for (int y = 0; y < NV; ++y) S[x][y] = mma16(kq, vw[y], S[x][y]);
           }
         }
       }
+      have = true;
+    }
+
+    // The next chunk's rows have landed. In a ring of three the rows of the chunk behind it may still travel: as
+    // many instructions of this wave as it has parts (stores between them only make the wait longer).
+    if (BUFS == 3 && at + 2 * C < end) {
+      if (wave < EXTRA)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER + 1) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
     } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __syncthreads();
+    if (at + BUFS * C < end) fetch(at + BUFS * C, buf);
+    buf = buf == BUFS - 1 ? 0 : buf + 1;
+
+    if (OUT) {
+      if constexpr (SHARE) {
 #pragma unroll
-      for (int sb = 0; sb < NB; ++sb) {
-        if (16 * sb >= n) break;
+        for (int x = 0; x < BLOCKS; ++x) pf[x] = ps[flip][x][lane];
+      }
 #pragma unroll
-        for (int y = 0; y < NV; ++y)
+      for (int t = 0; t < MINE; ++t) {
+        const int tb = KH == 2 ? kh : t;
+        if (16 * tb >= n) break;
+        f4 out[NV];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) vf[sb][y][r] *= w[sb][r];
-#pragma unroll
-        for (int x = 0; x < NK; ++x) {
-          const f4 kq = quad_cols(ks, LK, 16 * sb, 16 * x, i, g);
-#pragma unroll
-          for (int y = 0; y < NV; ++y) S[x][y] = mma16(kq, vf[sb][y], S[x][y]);
+        for (int y = 0; y < NV; ++y) {
+          out[y] = KH == 2 ? (kh ? acc[1][y] : acc[0][y]) : acc[t][y];
+          if constexpr (KH == 2) out[y] += xs[flip][kh ? wave - WC : wave + WC][y][lane];
+          if constexpr (Ty::BF) {
+            const bf4 none = bf4{(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
+            out[y] = mma32(vf[0][y], tb ? vf[1][y] : none, tb ? pf[1] : pf[0], tb ? pf[2] : none, out[y]);
+          } else {
+            out[y] = mma16(vf[0][y], tb ? pf[1] : pf[0], out[y]);
+            if (tb) out[y] = mma16(vf[1][y], pf[2], out[y]);
+          }
         }
+        if (16 * tb + i < n) {
+#pragma unroll
+          for (int y = 0; y < NV; ++y) {
+            const int vv = col + 16 * y + 4 * g;
+            if (a.vec_o && vv + 4 <= a.V) {
+              Ty::store4(po[t] + 16 * y, out[y]);
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (vv + r < a.V) Ty::store(po[t] + 16 * y + r, out[y][r]);
+            }
+          }
+        }
+        po[t] += po_step;
       }
     }
   }
@@ -476,52 +541,62 @@ __global__ __launch_bounds__(64 * NW, NK >= 16 || NW == 1 ? 1 : 2) void chunks(c
     // slots behind the sequence's end
     const int from = max(rows, first), to = min(a.T, first + a.seg_len);
     const int wide = min(a.V, c0 + SL) - c0;
-    for (long at = (long)from * wide + threadIdx.x; at < (long)to * wide; at += NT)
+    for (long at = (long)from * wide + threadIdx.x; at < (long)to * wide; at += 64 * NW)
       Ty::store(o + at / wide * a.so.t + c0 + at % wide, 0.f);
   }
   if (m) multiply_out(S, pw(g2, m));
   float* to = nullptr;
-  int tk = a.V, tv = 1;
+  int tk = a.ws_k, tv = a.ws_v;
   if (OUT) {
     const int owner = rows > 0 ? (rows - 1) / a.seg_len : 0;
-    if (a.fin && seg == owner) to = a.fin + bh * states, tk = a.fin_k, tv = a.fin_v;
+    if (a.fin && seg == owner) to = a.fin + bh * states, tk = a.V, tv = 1;
   } else {
     to = a.ws + (bh * (a.nseg - 1) + seg) * states;
   }
   if (to) {
 #pragma unroll
-    for (int x = 0; x < NK; ++x)
+    for (int x = 0; x < NKW; ++x)
 #pragma unroll
       for (int y = 0; y < NV; ++y)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int kk = 16 * x + 4 * g + r, vv = col + 16 * y + i;
+          const int kk = k0 + 16 * x + 4 * g + r, vv = col + 16 * y + i;
           if (kk < a.K && vv < a.V) to[(long)kk * tk + (long)vv * tv] = S[x][y][r];
         }
   }
 }
 
-// Columns of V that a workgroup takes: 16 (one wave, as long as that wave can stage the rows of K in
-// few loads), 64, or 128 as long as its share of the state leaves a wave registers to work with.
-inline int slice_columns(int K, int V) { return V <= 16 && K <= 64 ? 16 : V <= 64 || K > 128 ? 64 : 128; }
-inline int chunk_slots(int dtype) { return dtype == CET_BF16 ? Type<__bf16>::C : Type<float>::C; }
+// Columns of V that a workgroup takes: 16 (one wave, as long as that wave can bring in the rows of K in few
+// instructions); 128 in bf16 up to K = 128, where four waves hold their state in 64 registers each; else 64, and 32
+// where rows of 256 fp32 fill LDS. (bf16, 128 x 128, 8 x 16 heads x 2048 slots: 82 us a pass; 64 columns by eight
+// waves, two to the K of a column, 101 us, and 119 us with one workgroup per CU and no segments.)
+inline int slice_columns(int dtype, int K, int V) {
+  if (V <= 16 && K <= 64) return 16;
+  if (K > 128 && dtype != CET_BF16) return 32;
+  return V > 64 && K <= 128 && dtype == CET_BF16 ? 128 : 64;
+}
 
 template <typename IO, int NK, bool OUT>
 inline void launch_k(const Args& a, unsigned blocks, hipStream_t s) {
-  const int cols = slice_columns(a.K, a.V);
-  if (cols == 16) {
-    if constexpr (NK <= 4) chunks<IO, NK, 1, 1, OUT><<<blocks, 64, 0, s>>>(a);
-  } else if (cols == 64) {
-    chunks<IO, NK, 1, 4, OUT><<<blocks, 256, 0, s>>>(a);
-  } else {
-    if constexpr (NK <= 8) chunks<IO, NK, 2, 4, OUT><<<blocks, 256, 0, s>>>(a);
-  }
+  constexpr bool BF = Type<IO>::BF;
+  const int cols = slice_columns(BF ? CET_BF16 : CET_F32, a.K, a.V);
+  if constexpr (NK <= 4)
+    if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(a);
+  if constexpr (NK <= 8 && BF)
+    if (cols == 128) return chunks<IO, NK, 2, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
+  if constexpr (NK <= 4)
+    chunks<IO, NK, 1, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
+  else if constexpr (NK == 16 && !BF)
+    chunks<IO, NK, 1, 2, 2, OUT><<<blocks, 256, 0, s>>>(a);
+  else
+    chunks<IO, NK, 1, 4, 2, OUT><<<blocks, 512, 0, s>>>(a);
 }
 
 template <typename IO, bool OUT>
 inline void launch(const Args& a, unsigned blocks, hipStream_t s) {
-  if (!Type<IO>::BF && a.K <= 16)
-    launch_k<IO, Type<IO>::BF ? 2 : 1, OUT>(a, blocks, s);
+  // 2-byte rows of 16 would be smaller than the 1024 bytes that an instruction brings: 32 at least
+  if (sizeof(IO) == 4 && a.K <= 16)
+    launch_k<IO, sizeof(IO) == 4 ? 1 : 2, OUT>(a, blocks, s);
   else if (a.K <= 32)
     launch_k<IO, 2, OUT>(a, blocks, s);
   else if (a.K <= 64)

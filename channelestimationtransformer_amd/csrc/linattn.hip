@@ -13,22 +13,25 @@ constexpr size_t align_up(size_t n) { return (n + 255) & ~(size_t)255; }
 constexpr int elem_bytes(int dtype) { return dtype == CET_F32 ? 4 : 2; }
 
 // ws[bh][s] holds what segment s adds to the state; afterwards the state behind segment s (the one that
-// segment s + 1 starts from). One thread per state element, segments in order; blockIdx.y is the head.
+// segment s + 1 starts from). A thread takes W state elements, segments in order; blockIdx.y is the head.
+template <int W>
 __global__ __launch_bounds__(256) void join_segments(const Args a) {
-  const int states = a.K * a.V, e = blockIdx.x * 256 + threadIdx.x;
+  typedef float vec __attribute__((ext_vector_type(W)));
+  const int states = a.K * a.V, e = (blockIdx.x * 256 + threadIdx.x) * W;
   if (e >= states) return;
   const long bh = blockIdx.y;
   const float d = pw(a.log_decay[bh % a.H] * 1.44269504088896340736f, a.seg_len);
-  float cur = a.init ? a.init[bh * states + (long)(e / a.V) * a.init_k + (long)(e % a.V) * a.init_v] : 0.f;
+  vec cur = {};
+  if (a.init) cur = *reinterpret_cast<const vec*>(a.init + bh * states + e);
   float* p = a.ws + bh * (a.nseg - 1) * states + e;
   for (int s0 = 0; s0 < a.nseg - 1; s0 += 8) {
-    float add[8];
+    vec add[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) add[j] = s0 + j < a.nseg - 1 ? p[(long)(s0 + j) * states] : 0.f;
+    for (int j = 0; j < 8; ++j) add[j] = *reinterpret_cast<const vec*>(p + (long)min(s0 + j, a.nseg - 2) * states);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      cur = fmaf(cur, d, add[j]);
-      if (s0 + j < a.nseg - 1) p[(long)(s0 + j) * states] = cur;
+      cur = cur * d + add[j];
+      if (s0 + j < a.nseg - 1) *reinterpret_cast<vec*>(p + (long)(s0 + j) * states) = cur;
     }
   }
 }
@@ -184,24 +187,23 @@ struct Operand {
   }
 };
 
-// How a pass over the slots is cut: slices of V, and segments of the time axis where heads, sequences and
-// slices alone are fewer than two workgroups per CU.
+// How the time axis is cut: into segments where heads, sequences and slices alone are fewer than two workgroups
+// per CU, none shorter than 256 slots. Forward and backward cut it alike, and share the segments' states.
 struct Cut {
-  int nslice, nseg, seg_len;
-  size_t ws;  // bytes for the segments' states
+  int nseg, seg_len;
+  size_t states;  // bytes of the states between segments, K x V per head
 };
 
-Cut cut(const cet_linattn_desc& d, int K, int V, int cus) {
-  Cut c;
-  const int cols = slice_columns(K, V), C = chunk_slots(d.dtype);
-  c.nslice = (V + cols - 1) / cols;
-  const long tasks = (long)d.B * d.H * c.nslice, chunks = (d.T + C - 1) / C;
-  long nseg = tasks ? std::min<long>(2L * cus / tasks, chunks / 4) : 1;
+Cut cut(const cet_linattn_desc& d) {
+  const int cols = slice_columns(d.dtype, d.K, d.V);
+  const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
+  long nseg = tasks ? std::min<long>(2L * cu_count() / tasks, chunks / 4) : 1;
   nseg = std::max<long>(nseg, 1);
   const long per = (std::max<long>(chunks, 1) + nseg - 1) / nseg;
-  c.seg_len = (int)(per * C);
+  Cut c;
+  c.seg_len = (int)(per * STATE_SLOTS);
   c.nseg = (int)std::max<long>((chunks + per - 1) / per, 1);
-  c.ws = c.nseg > 1 ? align_up((size_t)d.B * d.H * (c.nseg - 1) * K * V * sizeof(float)) : 0;
+  c.states = c.nseg > 1 ? align_up((size_t)d.B * d.H * (c.nseg - 1) * d.K * d.V * sizeof(float)) : 0;
   return c;
 }
 
@@ -216,19 +218,37 @@ int launch(const Args& a, bool out, unsigned blocks, int dtype, hipStream_t s) {
   return CET_OK;
 }
 
-// One pass of the recurrence over packed operands.
-int pass(Args a, const Cut& c, int dtype, hipStream_t s) {
-  a.nslice = c.nslice;
-  a.nseg = c.nseg;
-  a.seg_len = c.seg_len;
+unsigned blocks(const Args& a, int dtype, int nseg) {
+  const int cols = slice_columns(dtype, a.K, a.V);
+  return (unsigned)((long)a.B * a.H * nseg * ((a.V + cols - 1) / cols));
+}
+
+// The states between segments from (k, v) into ws, as K x V.
+int segment_states(Args a, const Cut& c, int dtype, hipStream_t s) {
+  if (c.nseg == 1) return CET_OK;
+  a.nseg = c.nseg, a.seg_len = c.seg_len;
+  a.ws_k = a.V, a.ws_v = 1;
+  const int cols = slice_columns(dtype, a.K, a.V);
+  a.nslice = (a.V + cols - 1) / cols;
+  if (const int rc = launch(a, false, blocks(a, dtype, c.nseg - 1), dtype, s)) return rc;
+  const unsigned heads = (unsigned)((long)a.B * a.H), states = (unsigned)(a.K * a.V);
+  if (states % 4 == 0 && (reinterpret_cast<uintptr_t>(a.init) & 15) == 0)
+    join_segments<4><<<dim3((states / 4 + 255) / 256, heads), 256, 0, s>>>(a);
+  else
+    join_segments<1><<<dim3((states + 255) / 256, heads), 256, 0, s>>>(a);
+  CET_HIP(hipGetLastError());
+  return CET_OK;
+}
+
+// One pass of the recurrence, segments from their states in ws (transposed: of the operands' roles exchanged).
+int pass(Args a, const Cut& c, bool transposed, int dtype, hipStream_t s) {
+  a.nseg = c.nseg, a.seg_len = c.seg_len;
+  a.ws_k = a.init_k = transposed ? 1 : a.V;
+  a.ws_v = a.init_v = transposed ? a.K : 1;
+  const int cols = slice_columns(dtype, a.K, a.V);
+  a.nslice = (a.V + cols - 1) / cols;
   a.vec_o = a.V % 4 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
-  const long bh = (long)a.B * a.H;
-  if (c.nseg > 1) {
-    if (const int rc = launch(a, false, (unsigned)(bh * (c.nseg - 1) * c.nslice), dtype, s)) return rc;
-    join_segments<<<dim3((unsigned)((a.K * a.V + 255) / 256), (unsigned)bh), 256, 0, s>>>(a);
-    CET_HIP(hipGetLastError());
-  }
-  return launch(a, true, (unsigned)(bh * c.nseg * c.nslice), dtype, s);
+  return launch(a, true, blocks(a, dtype, c.nseg), dtype, s);
 }
 
 bool bad_desc(const cet_linattn_desc* d) {
@@ -279,27 +299,27 @@ using namespace cet::la;
 
 extern "C" {
 
+size_t cet_linear_attention_states(const cet_linattn_desc* d) {
+  return bad_desc(d) || too_large(*d) ? 0 : cut(*d).states;
+}
+
 size_t cet_linear_attention_workspace(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
                                       const void* d_o, int backward) {
   if (bad_desc(d) || too_large(*d)) return 0;
-  const int cus = cu_count();
   size_t n = Operand(q, d->q, d->K, *d).copy + Operand(k, d->k, d->K, *d).copy + Operand(v, d->v, d->V, *d).copy;
-  size_t states = cut(*d, d->K, d->V, cus).ws;
-  if (backward) {
-    n += Operand(d_o, d->d_o, d->V, *d).copy;
-    states = std::max(states, cut(*d, d->V, d->K, cus).ws);
-  }
-  return n + states;
+  if (backward) n += Operand(d_o, d->d_o, d->V, *d).copy;
+  return n + cut(*d).states * (backward ? 2 : 1);
 }
 
 int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k, const void* v, const float* log_decay,
-                         const float* initial, const void* lengths, void* o, float* final_state, void* workspace,
-                         size_t workspace_bytes, void* stream) {
+                         const float* initial, const void* lengths, void* o, float* final_state, float* states,
+                         void* workspace, size_t workspace_bytes, void* stream) {
   if (bad_desc(d)) return CET_ERR_INVALID_ARG;
   if (too_large(*d)) return CET_ERR_UNSUPPORTED;
   if ((long)d->B * d->H == 0) return CET_OK;
   if (!log_decay || (d->T > 0 && (!q || !k || !v || !o))) return CET_ERR_INVALID_ARG;
-  if (reinterpret_cast<uintptr_t>(workspace) & 15) return CET_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(initial)) & 15)
+    return CET_ERR_INVALID_ARG;
   const size_t need = cet_linear_attention_workspace(d, q, k, v, nullptr, 0);
   if (need > workspace_bytes || (need && !workspace)) return CET_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -307,27 +327,30 @@ int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k
   Operand oq(q, d->q, d->K, *d), ok(k, d->k, d->K, *d), ov(v, d->v, d->V, *d);
   for (Operand* x : {&oq, &ok, &ov})
     if (const int rc = x->pack(*d, ws, s)) return rc;
+  const Cut c = cut(*d);
   Args a{};
   a.q = oq.p, a.k = ok.p, a.v = ov.p, a.o = o;
   a.sq = oq.s, a.sk = ok.s, a.sv = ov.s, a.so = contiguous(*d, d->V);
   a.init = initial, a.fin = final_state;
-  a.init_k = a.fin_k = d->V, a.init_v = a.fin_v = 1;
   a.log_decay = log_decay, a.lengths = lengths, a.lengths64 = d->lengths64;
-  a.ws = reinterpret_cast<float*>(ws);
+  a.ws = states ? states : reinterpret_cast<float*>(ws);
   a.B = d->B, a.T = d->T, a.H = d->H, a.K = d->K, a.V = d->V;
   a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
-  return pass(a, cut(*d, d->K, d->V, cu_count()), d->dtype, s);
+  if (const int rc = segment_states(a, c, d->dtype, s)) return rc;
+  return pass(a, c, false, d->dtype, s);
 }
 
 int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
-                                  const float* log_decay, const float* initial, const void* lengths, const void* d_o,
-                                  const float* d_final, void* dq, void* dk, void* dv, float* d_initial, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+                                  const float* log_decay, const float* initial, const void* lengths, const float* states,
+                                  const void* d_o, const float* d_final, void* dq, void* dk, void* dv,
+                                  float* d_initial, void* workspace, size_t workspace_bytes, void* stream) {
   if (bad_desc(d)) return CET_ERR_INVALID_ARG;
   if (too_large(*d)) return CET_ERR_UNSUPPORTED;
   if ((long)d->B * d->H == 0) return CET_OK;
   if (!log_decay || (d->T > 0 && (!q || !k || !v || !d_o || !dq || !dk || !dv))) return CET_ERR_INVALID_ARG;
-  if (reinterpret_cast<uintptr_t>(workspace) & 15) return CET_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(initial) |
+       reinterpret_cast<uintptr_t>(d_final)) & 15)
+    return CET_ERR_INVALID_ARG;
   const size_t need = cet_linear_attention_workspace(d, q, k, v, d_o, 1);
   if (need > workspace_bytes || (need && !workspace)) return CET_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -335,32 +358,44 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   Operand oq(q, d->q, d->K, *d), ok(k, d->k, d->K, *d), ov(v, d->v, d->V, *d), og(d_o, d->d_o, d->V, *d);
   for (Operand* x : {&oq, &ok, &ov, &og})
     if (const int rc = x->pack(*d, ws, s)) return rc;
-  const int cus = cu_count();
-  const Cut by_k = cut(*d, d->V, d->K, cus), by_v = cut(*d, d->K, d->V, cus);
+  const Cut c = cut(*d);
+  float* const forward = states ? const_cast<float*>(states) : reinterpret_cast<float*>(ws);  // only read where given
+  float* const back = reinterpret_cast<float*>(ws + c.states);
   Args a{};
   a.log_decay = log_decay, a.lengths = lengths, a.lengths64 = d->lengths64;
-  a.ws = reinterpret_cast<float*>(ws);
   a.B = d->B, a.T = d->T, a.H = d->H;
+  a.so = contiguous(*d, d->K);
+  a.ws = forward;
+  a.init = initial;
+  if (!states) {
+    a.k = ok.p, a.sk = ok.s, a.v = ov.p, a.sv = ov.s;
+    a.K = d->K, a.V = d->V, a.s_kv = 1.f;
+    if (const int rc = segment_states(a, c, d->dtype, s)) return rc;
+  }
   // dq: (do, v, k) forward in time, states transposed
   a.q = og.p, a.sq = og.s, a.k = ov.p, a.sk = ov.s, a.v = ok.p, a.sv = ok.s;
-  a.o = dq, a.so = contiguous(*d, d->K);
+  a.o = dq;
   a.K = d->V, a.V = d->K;
-  a.init = initial, a.init_k = 1, a.init_v = d->V;
   a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
-  if (const int rc = pass(a, by_k, d->dtype, s)) return rc;
+  if (const int rc = pass(a, c, true, d->dtype, s)) return rc;
+  // the gradients of the states, backward in time, which the two other passes share
+  a.ws = back;
+  a.init = d_final;
+  a.reverse = 1, a.s_inter = 1.f, a.s_intra = a.s_kv = d->scale;
+  a.k = oq.p, a.sk = oq.s, a.v = og.p, a.sv = og.s;
+  a.K = d->K, a.V = d->V;
+  if (const int rc = segment_states(a, c, d->dtype, s)) return rc;
   // dk: (v, do, q) backward in time, states transposed
   a.q = ov.p, a.sq = ov.s, a.k = og.p, a.sk = og.s, a.v = oq.p, a.sv = oq.s;
   a.o = dk;
-  a.init = d_final;
-  a.reverse = 1, a.s_inter = 1.f, a.s_intra = a.s_kv = d->scale;
-  if (const int rc = pass(a, by_k, d->dtype, s)) return rc;
+  a.K = d->V, a.V = d->K;
+  if (const int rc = pass(a, c, true, d->dtype, s)) return rc;
   // dv: (k, q, do) backward in time; the carry at the end is the gradient of the first state
   a.q = ok.p, a.sq = ok.s, a.k = oq.p, a.sk = oq.s, a.v = og.p, a.sv = og.s;
   a.o = dv, a.so = contiguous(*d, d->V);
   a.K = d->K, a.V = d->V;
-  a.init_k = a.fin_k = d->V, a.init_v = a.fin_v = 1;
   a.fin = d_initial;
-  return pass(a, by_v, d->dtype, s);
+  return pass(a, c, false, d->dtype, s);
 }
 
 int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64_t* q_strides, const int64_t* k_strides,

@@ -363,36 +363,41 @@ def _stream(dev):
 
 
 def run_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
-                     initial_state: Optional[torch.Tensor] = None,
-                     lengths: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """q, k [B,T,H,K], v [B,T,H,V] -> o [B,T,H,V], state float32 [B,H,K,V]."""
+                         initial_state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                         keep: bool = False) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """q, k [B,T,H,K], v [B,T,H,V] -> o [B,T,H,V], state float32 [B,H,K,V], and with `keep` the states between
+    segments of a long time axis for the backward call (else empty)."""
     dev, d, q, k, v, log_decay, s0, lengths, _ = _linattn(q, k, v, log_decay, scale, initial_state, lengths)
     o = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
     state = torch.empty((d.B, d.H, d.K, d.V), dtype=torch.float32, device=dev)
     L = _cabi.lib()
     with _on(dev):
+        segments = torch.empty((L.cet_linear_attention_states(d) // 4 if keep else 0,), dtype=torch.float32, device=dev)
         n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), None, 0)
         ws = _workspace(n, dev)
-        rc = L.cet_linear_attention(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths), _at(o),
-                                    _at(state), _at(ws), n, _stream(dev))
+        rc = L.cet_linear_attention(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths), _at(o), _at(state),
+                                    _at(segments), _at(ws), n, _stream(dev))
     _cabi.check(rc, "cet_linear_attention")
-    return o, state
+    return o, state, segments
 
 
 linear_attention = torch.library.custom_op("cet::linear_attention", mutates_args=())(run_linear_attention)
 
 
 @linear_attention.register_fake
-def _(q, k, v, log_decay, scale, initial_state=None, lengths=None):
+def _(q, k, v, log_decay, scale, initial_state=None, lengths=None, keep=False):
     B, T, H, K = q.shape
-    return q.new_empty((B, T, H, v.shape[3])), q.new_empty((B, H, K, v.shape[3]), dtype=torch.float32)
+    segments = torch.library.get_ctx().new_dynamic_size() if keep else 0
+    return (q.new_empty((B, T, H, v.shape[3])), q.new_empty((B, H, K, v.shape[3]), dtype=torch.float32),
+            q.new_empty((segments,), dtype=torch.float32))
 
 
 def run_linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
-                              initial_state: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
-                              d_o: torch.Tensor, d_state: Optional[torch.Tensor], want_initial: bool
-                              ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """-> dq, dk, dv, d_initial (empty unless `want_initial`)."""
+                                  initial_state: Optional[torch.Tensor], lengths: Optional[torch.Tensor],
+                                  segments: Optional[torch.Tensor], d_o: torch.Tensor, d_state: Optional[torch.Tensor],
+                                  want_initial: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> dq, dk, dv, d_initial (empty unless `want_initial`). `segments`: what the forward call on the same
+    operands kept (None: formed again)."""
     dev, d, q, k, v, log_decay, s0, lengths, d_o = _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o)
     if d_state is not None:
         _dev_check(q, d_state)
@@ -402,43 +407,47 @@ def run_linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     ds = torch.empty((d.B, d.H, d.K, d.V) if want_initial else (0,), dtype=torch.float32, device=dev)
     L = _cabi.lib()
     with _on(dev):
+        if segments is not None and segments.numel():
+            _dev_check(q, segments)
+            segments = _f32("segments", segments, L.cet_linear_attention_states(d) // 4)
         n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), _at(d_o), 1)
         ws = _workspace(n, dev)
-        rc = L.cet_linear_attention_backward(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths),
-                                             _at(d_o), _at(d_state), _at(dq), _at(dk), _at(dv), _at(ds), _at(ws),
-                                             n, _stream(dev))
+        rc = L.cet_linear_attention_backward(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths), _at(segments),
+                                             _at(d_o), _at(d_state), _at(dq), _at(dk), _at(dv), _at(ds), _at(ws), n,
+                                             _stream(dev))
     _cabi.check(rc, "cet_linear_attention_backward")
     return dq, dk, dv, ds
 
 
-linear_attention_backward = torch.library.custom_op("cet::linear_attention_backward", mutates_args=())(run_linear_attention_backward)
+linear_attention_backward = torch.library.custom_op("cet::linear_attention_backward", mutates_args=())(
+    run_linear_attention_backward)
 
 
 @linear_attention_backward.register_fake
-def _(q, k, v, log_decay, scale, initial_state, lengths, d_o, d_state, want_initial):
+def _(q, k, v, log_decay, scale, initial_state, lengths, segments, d_o, d_state, want_initial):
     B, T, H, K = q.shape
     shape = (B, H, K, v.shape[3]) if want_initial else (0,)
     return (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), q.new_empty(shape, dtype=torch.float32))
 
 
 def _linattn_setup(ctx, inputs, output):
-    q, k, v, log_decay, scale, initial_state, lengths = inputs
+    q, k, v, log_decay, scale, initial_state, lengths, keep = inputs
     if ctx.needs_input_grad[3]:
         raise RuntimeError("log_decay is a constant of linear_attention: it has no gradient (detach it)")
-    ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+    ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths, output[2] if keep else None)
     ctx.scale = scale
     ctx.set_materialize_grads(False)
 
 
-def _linattn_backward(ctx, d_o, d_state, run=linear_attention_backward):
-    q, k, v, log_decay, s0, lengths = ctx.saved_tensors
+def _linattn_backward(ctx, d_o, d_state, _, run=linear_attention_backward):
+    q, k, v, log_decay, s0, lengths, segments = ctx.saved_tensors
     if d_o is None:
         if d_state is None:
-            return (None,) * 7
+            return (None,) * 8
         d_o = q.new_zeros((*q.shape[:3], v.shape[3]))
     want = s0 is not None and ctx.needs_input_grad[5]
-    dq, dk, dv, ds = run(q, k, v, log_decay, ctx.scale, s0, lengths, d_o, d_state, want)
-    return dq, dk, dv, None, None, ds if want else None, None
+    dq, dk, dv, ds = run(q, k, v, log_decay, ctx.scale, s0, lengths, segments, d_o, d_state, want)
+    return dq, dk, dv, None, None, ds if want else None, None, None
 
 
 linear_attention.register_autograd(_linattn_backward, setup_context=_linattn_setup)
@@ -447,12 +456,16 @@ linear_attention.register_autograd(_linattn_backward, setup_context=_linattn_set
 class LinearAttention(torch.autograd.Function):
     """The same operator without the dispatcher (eager calls on plain tensors: a fifth of the host time)."""
     forward = staticmethod(run_linear_attention)
-    setup_context = staticmethod(_linattn_setup)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _linattn_setup(ctx, inputs, output)
+        ctx.mark_non_differentiable(output[2])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, d_o, d_state):
-        return _linattn_backward(ctx, d_o, d_state, run_linear_attention_backward)
+    def backward(ctx, d_o, d_state, _):
+        return _linattn_backward(ctx, d_o, d_state, None, run_linear_attention_backward)
 
 
 def _step(q, k, v, log_decay, state, out_state, scale, slots):

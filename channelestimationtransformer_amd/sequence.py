@@ -33,10 +33,12 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("log_decay is a constant of linear_attention: it has no gradient (detach it)")
-    args = q, k, v, log_decay, float(scale), initial_state, lengths
+    grad = ops.wants_grad(q, k, v, initial_state)
     if not ops.direct(q, k, v, log_decay, initial_state, lengths):
-        return torch.ops.cet.linear_attention(*args)
-    return ops.LinearAttention.apply(*args) if ops.wants_grad(q, k, v, initial_state) else ops.run_linear_attention(*args)
+        run = torch.ops.cet.linear_attention
+    else:
+        run = ops.LinearAttention.apply if grad else ops.run_linear_attention
+    return run(q, k, v, log_decay, float(scale), initial_state, lengths, grad)[:2]
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None, slots=None, inplace=False):

@@ -323,23 +323,29 @@ typedef struct cet_linattn_desc {
 size_t cet_linear_attention_workspace(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
                                       const void* d_o, int backward);
 
+/* Bytes of the states that the forward call forms between segments of a long time axis (0 where it is not cut). */
+size_t cet_linear_attention_states(const cet_linattn_desc* d);
+
 /* S_t = exp(log_decay[h]) S_{t-1} + k_t^T v_t, o_t = scale q_t S_t for t < lengths[b] (values outside
  * [0, T] are taken as the nearer end; NULL: T everywhere); o is zero from there on.
  * log_decay: device [H] float32, <= 0 for a state that fades (minus infinity: no memory).
  * initial, final: device [B,H,K,V] float32, the state before the first and after the last slot in use;
  * either may be NULL (zero; not wanted). o: device [B,T,H,V] contiguous, every element is written.
+ * states: NULL, or cet_linear_attention_states() bytes that keep the states between segments for the backward call.
+ * initial and states start on 16 bytes.
  * Slots of q, k and v at or behind lengths[b] are not read. The workspace is 16-byte aligned and used by
  * this call until it has run on the stream. */
 int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
                          const float* log_decay, const float* initial, const void* lengths, void* o,
-                         float* final_state, void* workspace, size_t workspace_bytes, void* stream);
+                         float* final_state, float* states, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of the call above from d_o (strides d->d_o) and d_final (NULL: zero): dq, dk [B,T,H,K] and
- * dv [B,T,H,V] contiguous, zero at and behind lengths[b]; d_initial [B,H,K,V] (NULL: not wanted). The
+ * dv [B,T,H,V] contiguous, zero at and behind lengths[b]; d_initial [B,H,K,V] (NULL: not wanted). states: as the
+ * forward call on the same operands left them (NULL: formed again). initial, d_final and states start on 16 bytes. The
  * decay is a constant. */
 int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
                                   const float* log_decay, const float* initial, const void* lengths,
-                                  const void* d_o, const float* d_final, void* dq, void* dk, void* dv,
+                                  const float* states, const void* d_o, const float* d_final, void* dq, void* dk, void* dv,
                                   float* d_initial, void* workspace, size_t workspace_bytes, void* stream);
 
 /* One slot of B streams: q, k [B,H,K], v [B,H,V] (strides {stream, head} in elements), o [B,H,V]

@@ -292,6 +292,19 @@ def test_graphs_and_streams():
                 assert all(torch.equal(a, b) for a, b in zip(out, want[(turn + j) % 2]))
 
 
+def test_states_of_segments_kept_or_formed_again():
+    """The gradient from the states that the forward call kept and from formed ones: the same bits."""
+    y = gpu(make(1, 1200, 2, 48, 32, torch.bfloat16, seed=15), torch.bfloat16)
+    args = y["q"], y["k"], y["v"], y["g"], 0.2, y["s0"], None
+    kept = torch.ops.cet.linear_attention(*args, True)[2]
+    assert kept.numel() >= 2 * 48 * 32
+    one = torch.ops.cet.linear_attention_backward(*args, kept, y["d_o"], y["d_state"], True)
+    two = torch.ops.cet.linear_attention_backward(*args, None, y["d_o"], y["d_state"], True)
+    assert all(torch.equal(a, b) for a, b in zip(one, two))
+    with pytest.raises(RuntimeError, match="segments"):
+        torch.ops.cet.linear_attention_backward(*args, kept[:-4], y["d_o"], y["d_state"], True)
+
+
 def test_same_bits_every_time():
     y = gpu(make(1, 2000, 2, 64, 64, torch.bfloat16, seed=13), torch.bfloat16)
     first = cet.linear_attention(y["q"], y["k"], y["v"], y["g"])

@@ -40,8 +40,9 @@ def test_linear_attention_descriptors(change, code):
     L = _cabi.lib()
     d = desc(**change)
     assert L.cet_linear_attention_workspace(d, P, P, P, P, 1) == 0
-    assert L.cet_linear_attention(d, P, P, P, P, None, None, P, None, P, 1 << 30, None) == code
-    assert L.cet_linear_attention_backward(d, P, P, P, P, None, None, P, None, P, P, P, None, P, 1 << 30, None) == code
+    assert L.cet_linear_attention_states(d) == 0
+    assert L.cet_linear_attention(d, P, P, P, P, None, None, P, None, None, P, 1 << 30, None) == code
+    assert L.cet_linear_attention_backward(d, P, P, P, P, None, None, None, P, None, P, P, P, None, P, 1 << 30, None) == code
 
 
 def test_linear_attention_pointers():
@@ -49,20 +50,21 @@ def test_linear_attention_pointers():
     for hole in range(4):  # q, k, v, log_decay
         p = [P] * 4
         p[hole] = None
-        assert L.cet_linear_attention(desc(), *p, None, None, P, None, None, 0, None) == 1
-    assert L.cet_linear_attention(desc(), P, P, P, P, None, None, None, None, None, 0, None) == 1  # o
-    assert L.cet_linear_attention(desc(), P, P, P, P, None, None, P, None, P + 8, 1 << 20, None) == 1  # workspace off 16 bytes
-    assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, None, 0, None) == 1  # copy without workspace
+        assert L.cet_linear_attention(desc(), *p, None, None, P, None, None, None, 0, None) == 1
+    assert L.cet_linear_attention(desc(), P, P, P, P, None, None, None, None, None, None, 0, None) == 1  # o
+    for off in ((None, None, P + 8), (None, P + 8, None), (P + 4, None, None)):  # initial, states, workspace off 16 bytes
+        assert L.cet_linear_attention(desc(), P, P, P, P, off[0], None, P, None, off[1], off[2], 1 << 20, None) == 1
+    assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, None, None, 0, None) == 1  # copy without workspace
     n = L.cet_linear_attention_workspace(desc(), P + 4, P, P, None, 0)
     assert n >= 2 * 8 * 2 * 16 * 4
-    assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, P, n - 1, None) == 1
-    assert L.cet_linear_attention(desc(B=0), None, None, None, None, None, None, None, None, None, 0, None) == 0
+    assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, None, P, n - 1, None) == 1
+    assert L.cet_linear_attention(desc(B=0), None, None, None, None, None, None, None, None, None, None, 0, None) == 0
     for hole in range(8):
-        p = [P, P, P, P, None, None, P, None, P, P, P]
-        at = [0, 1, 2, 3, 6, 8, 9, 10][hole]
+        p = [P, P, P, P, None, None, None, P, None, P, P, P]
+        at = [0, 1, 2, 3, 7, 9, 10, 11][hole]
         p[at] = None
         assert L.cet_linear_attention_backward(desc(), *p, None, None, 0, None) == 1
-    assert L.cet_linear_attention(None, P, P, P, P, None, None, P, None, None, 0, None) == 1
+    assert L.cet_linear_attention(None, P, P, P, P, None, None, P, None, None, None, 0, None) == 1
 
 
 def test_step_arguments():
