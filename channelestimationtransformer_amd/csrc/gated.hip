@@ -8,6 +8,15 @@
 
 namespace cet {
 namespace gated {
+
+// gated_narrow.hip
+bool narrow(const cet_gated_desc& d);
+size_t narrow_workspace(const cet_gated_desc& d, int cus);
+int narrow_forward_run(const cet_gated_desc& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
+                       void* out, int cus, hipStream_t s);
+int narrow_backward_run(const cet_gated_desc& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
+                        const void* dy, void* dx, void* dwg, void* dwu, void* dbg, void* dbu, float* part, int cus, hipStream_t s);
+
 namespace {
 
 constexpr size_t align_up(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -158,7 +167,7 @@ Cut cut(int dtype, long np, long nq, long nk, bool gated, bool may_split, int cu
   for (int large = 0; large < 2; ++large) {
     const long b = large ? 256 : 128, bp = gated ? b / 2 : b;
     const long tiles = ((np + bp - 1) / bp) * ((nq + b - 1) / b), slots = large ? cus : 2L * cus;
-    for (int s = 1; s <= (may_split ? 32 : 1); ++s) {
+    for (int s = 1; s <= (may_split ? 512 : 1); s += s < 32 ? 1 : s / 8) {
       const long per = std::max<long>(((nk + s - 1) / s + bk - 1) / bk * bk, bk);
       const long used = std::max<long>((nk + per - 1) / per, 1);
       if (used != s) continue;
@@ -310,6 +319,7 @@ extern "C" {
 
 size_t cet_gated_linear_workspace(const cet_gated_desc* d, const void* x, const void* w_gate, const void* w_up, int backward) {
   if (bad_desc(d) || too_large(*d)) return 0;
+  if (narrow(*d)) return backward ? narrow_workspace(*d, cu_count()) : 0;
   return Plan(*d, x, w_gate, w_up, backward != 0).bytes();
 }
 
@@ -319,6 +329,7 @@ int cet_gated_linear(const cet_gated_desc* d, const void* x, const void* w_gate,
   if (too_large(*d)) return CET_ERR_UNSUPPORTED;
   if (d->N == 0) return CET_OK;
   if (!x || !w_gate || !w_up || !out || (reinterpret_cast<uintptr_t>(workspace) & 15)) return CET_ERR_INVALID_ARG;
+  if (narrow(*d)) return narrow_forward_run(*d, x, w_gate, w_up, b_gate, b_up, out, cu_count(), static_cast<hipStream_t>(stream));
   Plan p(*d, x, w_gate, w_up, false);
   if (p.bytes() > workspace_bytes || (p.bytes() && !workspace)) return CET_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -346,9 +357,15 @@ int cet_gated_linear_backward(const cet_gated_desc* d, const void* x, const void
                               void* db_gate, void* db_up, void* workspace, size_t workspace_bytes, void* stream) {
   if (bad_desc(d)) return CET_ERR_INVALID_ARG;
   if (too_large(*d)) return CET_ERR_UNSUPPORTED;
-  if (d->N > 0 && (!x || !w_gate || !w_up || !dy)) return CET_ERR_INVALID_ARG;
+  if (!w_gate || !w_up || (d->N > 0 && (!x || !dy))) return CET_ERR_INVALID_ARG;
   if ((dw_gate == nullptr) != (dw_up == nullptr) || (db_gate == nullptr) != (db_up == nullptr)) return CET_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return CET_ERR_INVALID_ARG;
+  if (narrow(*d)) {
+    const int cus = cu_count();
+    if (narrow_workspace(*d, cus) > workspace_bytes || !workspace) return CET_ERR_INVALID_ARG;
+    return narrow_backward_run(*d, x, w_gate, w_up, b_gate, b_up, dy, dx, dw_gate, dw_up, db_gate, db_up,
+                               static_cast<float*>(workspace), cus, static_cast<hipStream_t>(stream));
+  }
   Plan p(*d, x, w_gate, w_up, true);
   if (p.bytes() > workspace_bytes || (p.bytes() && !workspace)) return CET_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -188,7 +188,9 @@ struct Operand {
 };
 
 // How the time axis is cut: into segments where heads, sequences and slices alone are fewer than two workgroups
-// per CU, none shorter than 256 slots. Forward and backward cut it alike, and share the segments' states.
+// per CU, none shorter than 128 slots. Forward and backward cut it alike, and share the segments' states. (16 x 6
+// heads of up to 777 slots, fp32: two segments 66 us a pass, three 56, four 70, five 57; three or four workgroups per
+// CU cost the bf16 training pass 20 to 25 %.)
 struct Cut {
   int nseg, seg_len;
   size_t states;  // bytes of the states between segments, K x V per head
@@ -197,7 +199,8 @@ struct Cut {
 Cut cut(const cet_linattn_desc& d) {
   const int cols = slice_columns(d.dtype, d.K, d.V);
   const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
-  long nseg = tasks ? std::min<long>(2L * cu_count() / tasks, chunks / 4) : 1;
+  long nseg = tasks ? std::min<long>((2L * cu_count() + tasks - 1) / tasks, chunks / 2) : 1;
+  if (tasks >= 2L * cu_count()) nseg = 1;
   nseg = std::max<long>(nseg, 1);
   const long per = (std::max<long>(chunks, 1) + nseg - 1) / nseg;
   Cut c;

@@ -78,7 +78,7 @@ def check(args, kind, dtype, scale_ok=True):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 64), (5, 33, 17), (16, 128, 48), (40, 100, 130), (64, 256, 64), (65, 64, 64), (100, 16, 500), (129, 136, 128),
-          (300, 72, 200), (700, 256, 520), (17, 2050, 31), (2000, 64, 64), (257, 513, 9), (5000, 40, 24)]
+          (300, 72, 200), (70, 32, 32), (333, 20, 60), (90, 64, 7), (1000, 33, 64), (9000, 64, 64), (700, 256, 520), (17, 2050, 31), (2000, 64, 64), (257, 513, 9), (5000, 40, 24)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -118,7 +118,7 @@ def test_rotary_refusals():
 
 
 def gated_desc(**kw):
-    d = _cabi.GatedDesc(0, 0, 100, 64, 48, 64, 64, 64, 48)
+    d = _cabi.GatedDesc(0, 0, 100, 128, 48, 128, 128, 128, 48)
     for n, v in kw.items():
         setattr(d, n, v)
     return d
@@ -151,6 +151,10 @@ def test_gated_refusals():
     assert L.cet_gated_linear_backward(d, P, P, P, None, None, P, P, P, P, P, None, P, n, None) == 1
     assert L.cet_gated_linear(d, P + 4, P, P, None, None, P, None, 0, None) == 1  # copy without workspace
     assert L.cet_gated_linear(gated_desc(N=0), None, None, None, None, None, None, None, 0, None) == 0
+    n = gated_desc(D=64)  # narrow layers: no copies, sums per workgroup
+    assert L.cet_gated_linear_workspace(n, P + 4, P, P, 0) == 0 and L.cet_gated_linear_workspace(n, P + 4, P, P, 1) > 0
+    assert L.cet_gated_linear_backward(n, P, P, P, None, None, P, P, P, P, None, None, None, 0, None) == 1
+    assert L.cet_gated_linear_backward(gated_desc(D=64, N=0), None, None, P, None, None, None, P, P, P, None, None, P, 1 << 30, None) == 1
     x, w = torch.zeros(4, 8), torch.zeros(6, 8)
     with pytest.raises(RuntimeError, match="GPU"):
         cet.gated_linear(x, w, w)
