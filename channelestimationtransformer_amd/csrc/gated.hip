@@ -126,10 +126,9 @@ __global__ __launch_bounds__(512) void few_rows(const Args a) {
     const int f = f0 + 4 * g, n = a.F - f, q = 16 * y + i;
     if (a.bias_g) gv += load4(static_cast<const T*>(a.bias_g) + f, n, 1);
     if (a.bias_u) uv += load4(static_cast<const T*>(a.bias_u) + f, n, 1);
-    f4 v;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = act(a.activation, gv[r]) * uv[r];
-    if (q < a.nq && n > 0) store4(static_cast<T*>(a.out) + (long)q * a.ld_out + f, v, n, a.out_step);
+    f4 v, slope;
+    act4(a.activation, gv, v, slope);
+    if (q < a.nq && n > 0) store4(static_cast<T*>(a.out) + (long)q * a.ld_out + f, v * uv, n, a.out_step);
   }
 }
 

@@ -40,17 +40,32 @@ __device__ inline void load_rows(f4 (&q)[NK], const void* p, long ld, long row, 
   for (int kk = 0; kk < NK; ++kk) q[kk] = load4(at + 16 * kk + 4 * g, live ? cols - 16 * kk - 4 * g : 0, step);
 }
 
+// Both weights as operands (k along the inputs) into LDS, once per workgroup: [gate tiles, up tiles][ND][lane]
+template <typename T, int ND, int NF, int NT>
+__device__ inline void stage_weights(const Narrow& a, f4 (*w)[ND][64]) {
+  for (int at = threadIdx.x; at < 2 * NF * ND * 64; at += NT) {
+    const int l = at & 63, li = l & 15, lg = l >> 4, kk = at / 64 % ND, f = at / 64 / ND;
+    const bool up = f >= NF;
+    const int row = 16 * (up ? f - NF : f) + li, c = 16 * kk + 4 * lg;
+    const T* p = static_cast<const T*>(up ? a.wu : a.wg) + (long)(row < a.F ? row : 0) * (up ? a.ld_u : a.ld_g) + c;
+    w[f][kk][l] = load4(p, row < a.F ? a.D - c : 0, up ? a.u_step : a.g_step);
+  }
+}
+
 template <typename T, int ND, int NF>
-__global__ __launch_bounds__(256, 2) void narrow_forward(const Narrow a) {
+__global__ __launch_bounds__(512, 2) void narrow_forward(const Narrow a) {
+  __shared__ f4 w[2 * NF][ND][64];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const long wave = (long)blockIdx.x * 4 + (threadIdx.x >> 6), waves = (long)gridDim.x * 4, tiles = ((long)a.N + 15) / 16;
+  const long wave = (long)blockIdx.x * 8 + (threadIdx.x >> 6), waves = (long)gridDim.x * 8, tiles = ((long)a.N + 15) / 16;
   f4 x[ND], next[ND];
   if (wave < tiles) load_rows<T, ND>(x, a.x, a.ld_x, wave * 16, a.N, a.D, a.x_step, i, g);
+  stage_weights<T, ND, NF, 512>(a, w);
   f4 wg[NF][ND], wu[NF][ND], bg[NF], bu[NF];
+  __syncthreads();
 #pragma unroll
   for (int f = 0; f < NF; ++f) {
-    load_rows<T, ND>(wg[f], a.wg, a.ld_g, 16 * f, a.F, a.D, a.g_step, i, g);
-    load_rows<T, ND>(wu[f], a.wu, a.ld_u, 16 * f, a.F, a.D, a.u_step, i, g);
+#pragma unroll
+    for (int kk = 0; kk < ND; ++kk) wg[f][kk] = w[f][kk][lane], wu[f][kk] = w[NF + f][kk][lane];
     const int at = 16 * f + 4 * g, n = a.F - at;
     bg[f] = bu[f] = f4{0.f, 0.f, 0.f, 0.f};
     if (a.bg) bg[f] = load4(static_cast<const T*>(a.bg) + at, n, 1);
@@ -59,18 +74,22 @@ __global__ __launch_bounds__(256, 2) void narrow_forward(const Narrow a) {
   for (long t = wave; t < tiles; t += waves) {
     if (t + waves < tiles) load_rows<T, ND>(next, a.x, a.ld_x, (t + waves) * 16, a.N, a.D, a.x_step, i, g);
     const long row = t * 16 + i;
+    f4 gv[NF], uv[NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      f4 gv = bg[f], uv = bu[f], v;
+    for (int f = 0; f < NF; ++f) gv[f] = bg[f], uv[f] = bu[f];
 #pragma unroll
-      for (int kk = 0; kk < ND; ++kk) {
-        gv = mma4(wg[f][kk], x[kk], gv);
-        uv = mma4(wu[f][kk], x[kk], uv);
+    for (int kk = 0; kk < ND; ++kk)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        gv[f] = mma4(wg[f][kk], x[kk], gv[f]);
+        uv[f] = mma4(wu[f][kk], x[kk], uv[f]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = act(a.activation, gv[r]) * uv[r];
+    for (int f = 0; f < NF; ++f) {
+      f4 v, slope;
+      act4(a.activation, gv[f], v, slope);
       const int at = 16 * f + 4 * g;
-      if (row < a.N && at < a.F) store4(static_cast<T*>(a.out) + row * a.F + at, v, a.F - at, a.out_step);
+      if (row < a.N && at < a.F) store4(static_cast<T*>(a.out) + row * a.F + at, v * uv[f], a.F - at, a.out_step);
     }
 #pragma unroll
     for (int kk = 0; kk < ND; ++kk) x[kk] = next[kk];
@@ -85,13 +104,7 @@ __global__ __launch_bounds__(256, 1) void narrow_backward(const Narrow a) {
   __shared__ __align__(16) float xs[4][16 * XLD], hs[4][16 * HLD];
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wv = threadIdx.x >> 6;
   const long wave = (long)blockIdx.x * 4 + wv, waves = (long)gridDim.x * 4, tiles = ((long)a.N + 15) / 16;
-  for (int at = threadIdx.x; at < 2 * NF * ND * 64; at += 256) {
-    const int l = at & 63, li = l & 15, lg = l >> 4, kk = at / 64 % ND, f = at / 64 / ND;
-    const bool up = f >= NF;
-    const int row = 16 * (up ? f - NF : f) + li, c = 16 * kk + 4 * lg;
-    const T* p = static_cast<const T*>(up ? a.wu : a.wg) + (long)(row < a.F ? row : 0) * (up ? a.ld_u : a.ld_g) + c;
-    w[f][kk][l] = load4(p, row < a.F ? a.D - c : 0, up ? a.u_step : a.g_step);
-  }
+  stage_weights<T, ND, NF, 256>(a, w);
   __syncthreads();
   for (int at = threadIdx.x; at < 2 * NF * ND * 64; at += 256) {
     // element (feature 16 f + 4 lg + r, input 16 d + li) of the weights as laid down above
@@ -122,23 +135,31 @@ __global__ __launch_bounds__(256, 1) void narrow_backward(const Narrow a) {
     load_rows<T, NF>(dy, a.dy, a.ld_dy, wave * 16, a.N, a.F, a.dy_step, i, g);
   }
   __syncthreads();
+  f4 wr[2 * NF][ND];
+#pragma unroll
+  for (int f = 0; f < 2 * NF; ++f)
+#pragma unroll
+    for (int kk = 0; kk < ND; ++kk) wr[f][kk] = w[f][kk][lane];
   float* const xt = xs[wv];
   float* const ht = hs[wv];
   for (long t = wave; t < tiles; t += waves) {
     f4 dh[2 * NF];
 #pragma unroll
+    for (int f = 0; f < NF; ++f) dh[f] = bg[f], dh[NF + f] = bu[f];
+#pragma unroll
+    for (int kk = 0; kk < ND; ++kk)
+#pragma unroll
+      for (int f = 0; f < 2 * NF; ++f) dh[f] = mma4(wr[f][kk], x[kk], dh[f]);
+#pragma unroll
     for (int f = 0; f < NF; ++f) {
-      f4 gv = bg[f], uv = bu[f];
+      f4 v, slope;
+      act4(a.activation, dh[f], v, slope);
+      const f4 uv = dh[NF + f];
 #pragma unroll
-      for (int kk = 0; kk < ND; ++kk) {
-        gv = mma4(w[f][kk][lane], x[kk], gv);
-        uv = mma4(w[NF + f][kk][lane], x[kk], uv);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {  // dy is zero behind the last row and feature, and so are these
+      for (int r = 0; r < 4; ++r) {
         const bool live = 16 * f + 4 * g + r < a.F && t * 16 + i < a.N;
-        dh[f][r] = live ? dy[f][r] * uv[r] * act_slope(a.activation, gv[r]) : 0.f;
-        dh[NF + f][r] = live ? dy[f][r] * act(a.activation, gv[r]) : 0.f;
+        dh[f][r] = live ? dy[f][r] * uv[r] * slope[r] : 0.f;
+        dh[NF + f][r] = live ? dy[f][r] * v[r] : 0.f;
       }
       db[f] += dh[f];
       db[NF + f] += dh[NF + f];
@@ -154,13 +175,17 @@ __global__ __launch_bounds__(256, 1) void narrow_backward(const Narrow a) {
     }
     if (a.dx) {
       const long row = t * 16 + i;
+      f4 v[ND];
+#pragma unroll
+      for (int d = 0; d < ND; ++d) v[d] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < 2 * NF; ++f)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) v[d] = mma4(wt[d][f][lane], dh[f], v[d]);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int f = 0; f < 2 * NF; ++f) v = mma4(wt[d][f][lane], dh[f], v);
         const int at = 16 * d + 4 * g;
-        if (row < a.N && at < a.D) store4(static_cast<T*>(a.dx) + row * a.D + at, v, a.D - at, a.dx_step);
+        if (row < a.N && at < a.D) store4(static_cast<T*>(a.dx) + row * a.D + at, v[d], a.D - at, a.dx_step);
       }
     }
     f4 xq[ND];
@@ -246,7 +271,7 @@ void launch(const Narrow& a, bool backward, unsigned groups, hipStream_t s) {
   if (backward)
     narrow_backward<T, ND, NF><<<groups, 256, 0, s>>>(a);
   else
-    narrow_forward<T, ND, NF><<<groups, 256, 0, s>>>(a);
+    narrow_forward<T, ND, NF><<<groups, 512, 0, s>>>(a);
 }
 template <typename T>
 void launch(const Narrow& a, bool backward, unsigned groups, hipStream_t s) {
@@ -269,9 +294,9 @@ int step_of(const void* p, long ld, int dtype) {
   return (at | ld) % 4 == 0 ? 4 : (at | ld) % 2 == 0 ? 2 : 1;
 }
 
-// Workgroups of four waves, each with 16 rows at least.
-unsigned groups_of(long N, unsigned most) {
-  const long n = (N + 63) / 64;
+// Workgroups, at most one per CU, for waves with 16 rows at least.
+unsigned groups_of(long N, int waves, unsigned most) {
+  const long n = (N + 16 * waves - 1) / (16 * waves);
   return (unsigned)(n < 1 ? 1 : n < most ? n : most);
 }
 
@@ -288,13 +313,13 @@ Narrow base(const cet_gated_desc& d, const void* x, const void* wg, const void* 
 
 bool narrow(const cet_gated_desc& d) { return d.D <= 64 && d.F <= 64; }
 
-size_t narrow_workspace(const cet_gated_desc& d, int cus) { return (size_t)groups_of(d.N, cus) * PART * sizeof(float); }
+size_t narrow_workspace(const cet_gated_desc& d, int cus) { return (size_t)groups_of(d.N, 4, cus) * PART * sizeof(float); }
 
 int narrow_forward_run(const cet_gated_desc& d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
                        void* out, int cus, hipStream_t s) {
   Narrow a = base(d, x, wg, wu, bg, bu);
   a.out = out, a.out_step = step_of(out, d.F, d.dtype);
-  launch(a, d.dtype, false, groups_of(d.N, 2 * cus), s);
+  launch(a, d.dtype, false, groups_of(d.N, 8, cus), s);
   CET_HIP(hipGetLastError());
   return CET_OK;
 }
@@ -305,7 +330,7 @@ int narrow_backward_run(const cet_gated_desc& d, const void* x, const void* wg, 
   a.dy = dy, a.ld_dy = d.ld_dy, a.dy_step = step_of(dy, d.ld_dy, d.dtype);
   a.dx = dx, a.dx_step = step_of(dx, d.D, d.dtype);
   a.part = dwg || dbg ? part : nullptr;
-  const unsigned groups = groups_of(d.N, cus);
+  const unsigned groups = groups_of(d.N, 4, cus);
   launch(a, d.dtype, true, groups, s);
   CET_HIP(hipGetLastError());
   if (a.part) {
