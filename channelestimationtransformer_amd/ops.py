@@ -295,9 +295,13 @@ def _seq_check(name, t, dtype, *shape):
     is contiguous."""
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(s is not None and int(d) != int(s) for d, s in zip(t.shape, shape)):
-        raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    have = t.shape
+    if len(have) != len(shape):
+        raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(have)}")
+    for s, d in zip(shape, have):
+        if s is not None and s != d:
+            raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(have)}")
+    return t if have[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def _seq_type(t):
@@ -351,6 +355,7 @@ def _at(t):
 
 
 _HERE = contextlib.nullcontext()
+_TWO = ctypes.c_int64 * 2
 
 
 def _on(dev):
@@ -359,7 +364,7 @@ def _on(dev):
 
 
 def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)  # torch.cuda.current_stream without the object (1.5 us)
 
 
 def run_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float,
@@ -454,13 +459,15 @@ linear_attention.register_autograd(_linattn_backward, setup_context=_linattn_set
 
 
 class LinearAttention(torch.autograd.Function):
-    """The same operator without the dispatcher (eager calls on plain tensors: a fifth of the host time)."""
-    forward = staticmethod(run_linear_attention)
+    """The same operator without the dispatcher (eager calls on plain tensors: a third of the host time; a forward
+    that takes `ctx` saves the binding of its arguments, 12 us)."""
 
     @staticmethod
-    def setup_context(ctx, inputs, output):
-        _linattn_setup(ctx, inputs, output)
+    def forward(ctx, *args):
+        output = run_linear_attention(*args)
+        _linattn_setup(ctx, args, output)
         ctx.mark_non_differentiable(output[2])
+        return output
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -483,7 +490,7 @@ def _step(q, k, v, log_decay, state, out_state, scale, slots):
     wide = 0
     if slots is not None:
         slots, wide = _index("slots", slots, B)
-    strides = [(ctypes.c_int64 * 2)(*t.stride()[:2]) for t in (q, k, v)]
+    strides = [_TWO(*t.stride()[:2]) for t in (q, k, v)]
     with _on(dev):
         rc = _cabi.lib().cet_linear_attention_step(
             code, B, H, K, V, *strides, _at(q), _at(k), _at(v), _at(log_decay), scale, _at(state), _at(out_state),
@@ -599,8 +606,11 @@ rotary.register_autograd(_rotary_backward, setup_context=_rotary_setup)
 
 
 class Rotary(torch.autograd.Function):
-    forward = staticmethod(run_rotary)
-    setup_context = staticmethod(_rotary_setup)
+    @staticmethod
+    def forward(ctx, *args):
+        output = run_rotary(*args)
+        _rotary_setup(ctx, args, output)
+        return output
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -704,8 +714,11 @@ gated_linear.register_autograd(_gated_backward, setup_context=_gated_setup)
 
 
 class GatedLinear(torch.autograd.Function):
-    forward = staticmethod(run_gated_linear)
-    setup_context = staticmethod(_gated_setup)
+    @staticmethod
+    def forward(ctx, *args):
+        output = run_gated_linear(*args)
+        _gated_setup(ctx, args, output)
+        return output
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -725,8 +738,17 @@ def step_in_place(q, k, v, log_decay, state, scale, slots):
 
 def direct(*tensors):
     """Whether a call may pass the dispatcher by: eager, and on plain tensors only (none of a tracer's)."""
-    return not torch.compiler.is_compiling() and all(type(t) in _PLAIN for t in tensors)
+    if torch.compiler.is_compiling():
+        return False
+    for t in tensors:
+        if type(t) not in _PLAIN:
+            return False
+    return True
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False

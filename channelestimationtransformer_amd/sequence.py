@@ -8,7 +8,8 @@ leaves a state of fixed size per head, `linear_attention_step` carries that stat
 
 All take CUDA (ROCm) tensors of one type (float32, bfloat16 or float16), run on the current stream
 and raise on anything the kernels do not serve. `rotary`, `linear_attention` and
-`gated_linear` have gradients (`rotary`'s can be differentiated again).
+`gated_linear` have gradients (`rotary`'s can be differentiated again; the transforms of torch.func are
+refused).
 """
 import math
 

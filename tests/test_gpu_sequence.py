@@ -169,3 +169,12 @@ def test_refusals_on_the_gpu():
         except RuntimeError:
             continue
         pytest.fail(f"call {n} was not refused")
+
+
+def test_function_transforms_are_refused():
+    """Not silently without gradients."""
+    q, dec = torch.randn(2, 5, 3, 8).cuda(), ref.geometric(3).cuda()
+    for call in (lambda t: cet.linear_attention(t, q, q, dec)[0].sum(), lambda t: cet.gated_linear(t[0, 0], q[0, 1], q[0, 2]).sum(),
+                 lambda t: cet.rotary(t, None, torch.arange(5, device="cuda"), cet.rotary_frequencies(8)[0])[0].sum()):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(call)(q)
