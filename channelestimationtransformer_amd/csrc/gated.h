@@ -149,18 +149,14 @@ struct Tile {
       const int r = r0 + i, kc = kk * 4 + g;
       return *reinterpret_cast<const Frag*>(t + r * 128 + ((kc ^ (r >> 1 & 7)) << 4));
     } else if constexpr (E == 2) {
+      // k = 32 kk + 8 g + 4 half + i / 4, whose turn is that of the lane alone; pieces of 16 indices: 2 X, 2 X + 1
       typedef __attribute__((address_space(3))) s4* lds_s4;
-      Frag f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int k = kk * 32 + 8 * g + 4 * half + (i >> 2), mc = r0 / 8 + (i >> 1 & 1);
-        const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(t + k * (ROWS * E) + ((mc ^ turn(k)) << 4) + (i & 1) * 8));
-        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-        const u2 w = __builtin_bit_cast(u2, v);
-        f[2 * half] = w[0];
-        f[2 * half + 1] = w[1];
-      }
-      return f;
+      typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+      const int th = (i >> 2) | (g & 1) << 2;
+      const char* p = t + (8 * g + (i >> 2)) * (ROWS * E) + (i & 1) * 8 + ((r0 / 16 ^ th) << 5) + ((i >> 1 & 1) << 4) + kk * 32 * ROWS * E;
+      const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
+      const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * ROWS * E)));
+      return Frag{a[0], a[1], b[0], b[1]};
     } else {
       Frag f;
 #pragma unroll
@@ -259,6 +255,11 @@ __device__ inline f4 load4(const T* p, int n, int step) {
   return v;
 }
 
+template <int N>
+struct Half {
+  static constexpr int value = N;
+};
+
 template <typename T, int BP, int BQ, int WP, int WQ, bool PC, bool QC, int KIND>
 __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const Args a) {
   constexpr int NT = 64 * WP * WQ, NPT = BP / WP / 16, NQT = BQ / WQ / 16;
@@ -304,28 +305,56 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
     return GATED ? (x < NPT / 2 ? wp * (BP / 2 / WP) + 16 * x : BP / 2 + wp * (BP / 2 / WP) + 16 * (x - NPT / 2)) : wp * (BP / WP) + 16 * x;
   };
 
+  // A tile is worked on in four steps: half of its 128 bytes of k and half of the wave's tiles of P each. The
+  // operands of a step travel from LDS into one set of registers while the matrix instructions work on the other,
+  // across the barrier too: before the last step of a tile the next tile has landed, this one is all in registers,
+  // and its buffer takes the rows of the tile after. (Whole steps of k need 32 registers more and spilled where
+  // operands are read by columns.)
+  constexpr int HP = NPT / 2;
+  Frag p0_[HP], p1_[HP], q0_[NQT], q1_[NQT];
+  auto load_p = [&](Frag (&fp)[HP], int buf, int kk, int half) {
+    const char* pt = lds + buf * BUF;
+#pragma unroll
+    for (int x = 0; x < HP; ++x) fp[x] = TP::read(pt, p_row(half * HP + x), kk, i, g);
+  };
+  auto load_q = [&](Frag (&fq)[NQT], int buf, int kk) {
+    const char* qt = lds + buf * BUF + TP::BYTES;
+#pragma unroll
+    for (int y = 0; y < NQT; ++y) fq[y] = TQ::read(qt, wq * (BQ / WQ) + 16 * y, kk, i, g);
+  };
+  auto multiply = [&](const Frag (&fp)[HP], const Frag (&fq)[NQT], auto half) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < HP; ++x)
+#pragma unroll
+      for (int y = 0; y < NQT; ++y) acc[decltype(half)::value * HP + x][y] = mma<T>(fp[x], fq[y], acc[decltype(half)::value * HP + x][y]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
   if (k_first < k_end) fetch(k_first, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  if (k_first + BK < k_end) fetch(k_first + BK, 1);
+  if (k_first < k_end) {
+    load_q(q0_, 0, 0);
+    load_p(p0_, 0, 0, 0);
+  }
   int buf = 0;
   for (int k0 = k_first; k0 < k_end; k0 += BK, buf ^= 1) {
-    if (k0 + BK < k_end) fetch(k0 + BK, buf ^ 1);
-    const char* pt = lds + buf * BUF;
-    const char* qt = pt + TP::BYTES;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      Frag fq[NQT];
-#pragma unroll
-      for (int y = 0; y < NQT; ++y) fq[y] = TQ::read(qt, wq * (BQ / WQ) + 16 * y, kk, i, g);
-#pragma unroll
-      for (int x = 0; x < NPT; ++x) {
-        const Frag fp = TP::read(pt, p_row(x), kk, i, g);
-#pragma unroll
-        for (int y = 0; y < NQT; ++y) acc[x][y] = mma<T>(fp, fq[y], acc[x][y]);
-      }
-    }
+    load_p(p1_, buf, 0, 1);
+    multiply(p0_, q0_, Half<0>());
+    load_q(q1_, buf, 1);
+    load_p(p0_, buf, 1, 0);
+    multiply(p1_, q0_, Half<1>());
+    load_p(p1_, buf, 1, 1);
+    multiply(p0_, q1_, Half<0>());
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+    if (k0 + 2 * BK < k_end) fetch(k0 + 2 * BK, buf);
+    if (k0 + BK < k_end) {
+      load_q(q0_, buf ^ 1, 0);
+      load_p(p0_, buf ^ 1, 0, 0);
+    }
+    multiply(p1_, q1_, Half<1>());
   }
 
   if constexpr (GATED) {
