@@ -54,6 +54,90 @@ __global__ __launch_bounds__(256) void pack_rows(const E* __restrict__ src, Stri
   }
 }
 
+// d = exp(log_decay) in two parts: a state that is multiplied slot by slot would hold a rounding of d raised to the
+// number of slots, 1e-4 of a weight 4,000 slots back.
+__device__ inline void decay_of(float log_decay, float& hi, float& lo) {
+  const double d = exp((double)log_decay);
+  hi = (float)d;
+  lo = (float)(d - (double)hi);
+}
+
+// Small heads (K and V up to 16) on many sequences, the predictors' own batches: a lane takes one column of V
+// of one head of one sequence, holds that column's state in K registers and walks the slots one by one; lanes of
+// a head read the same q and k. 100 instructions a head and 25 slots, where a wave with matrix instructions on a
+// head of its own took 1,180 and was bound by issuing them (4096 x 8 heads of 8, 25 slots, fp32: 67 us).
+template <typename IO, int KP>
+__global__ __launch_bounds__(256, 4) void columns(const Args a, int step_q, int step_k) {
+  const long c = (long)blockIdx.x * 256 + threadIdx.x;
+  const bool live = c < (long)a.B * a.H * a.V;
+  const unsigned bh = live ? (unsigned)(c / a.V) : 0;
+  const int vv = live ? (int)(c - (long)bh * a.V) : 0, b = bh / a.H, h = bh - b * a.H;
+  const int n = live ? row_count(a, b) : 0;
+  const long states = (long)a.K * a.V;
+  float S[KP];
+#pragma unroll
+  for (int k = 0; k < KP; ++k) S[k] = live && a.init && k < a.K ? a.init[bh * states + (long)k * a.init_k + (long)vv * a.init_v] : 0.f;
+  float d, d_lo;
+  decay_of(a.log_decay[h], d, d_lo);
+  const long from = a.reverse ? n - 1 : 0, dir = a.reverse ? -1 : 1;
+  const IO* q = static_cast<const IO*>(a.q) + b * a.sq.b + h * a.sq.h + from * a.sq.t;
+  const IO* k = static_cast<const IO*>(a.k) + b * a.sk.b + h * a.sk.h + from * a.sk.t;
+  const IO* v = static_cast<const IO*>(a.v) + b * a.sv.b + h * a.sv.h + from * a.sv.t + vv;
+  IO* const o0 = static_cast<IO*>(a.o) + b * a.so.b + h * a.so.h + vv;
+  IO* o = o0 + from * a.so.t;
+  auto row = [&](float (&x)[KP], const IO* p, int step) {
+    typedef typename Type<IO>::V4 V4;
+#pragma unroll
+    for (int j = 0; j < KP; j += 4) {
+      if (step == 4) {
+        V4 y = {};
+        if (j < a.K) y = *reinterpret_cast<const V4*>(p + j);  // K is a multiple of four
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[j + r] = (float)y[r];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[j + r] = j + r < a.K ? (float)p[j + r] : 0.f;
+      }
+    }
+  };
+  float qn[KP], kn[KP], vn = 0.f;  // the next slot's, on their way
+  if (n > 0) {
+    row(qn, q, step_q);
+    row(kn, k, step_k);
+    vn = (float)*v;
+  }
+  for (int t = 0; t < n; ++t) {
+    float qr[KP], kr[KP];
+    const float vr = vn * a.s_kv;
+#pragma unroll
+    for (int j = 0; j < KP; ++j) qr[j] = qn[j], kr[j] = kn[j];
+    if (t + 1 < n) {
+      q += dir * a.sq.t, k += dir * a.sk.t, v += dir * a.sv.t;
+      row(qn, q, step_q);
+      row(kn, k, step_k);
+      vn = (float)*v;
+    }
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < KP; ++j) {
+      S[j] = a.reverse ? fmaf(kr[j], vr, S[j]) : fmaf(S[j], d, fmaf(S[j], d_lo, kr[j] * vr));
+      sum[j & 3] = fmaf(qr[j], S[j], sum[j & 3]);
+    }
+    if (a.reverse) {
+#pragma unroll
+      for (int j = 0; j < KP; ++j) S[j] = fmaf(S[j], d, S[j] * d_lo);
+    }
+    *o = (IO)(((sum[0] + sum[1]) + (sum[2] + sum[3])) * a.s_inter);
+    o += dir * a.so.t;
+  }
+  if (!live) return;
+  for (long t = n; t < a.T; ++t) o0[t * a.so.t] = (IO)0.f;
+  if (a.fin)
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+      if (j < a.K) a.fin[bh * states + (long)j * a.V + vv] = S[j];
+}
+
 // One slot. A workgroup takes 4 TX (or TX, where rows of V are no multiple of four) columns of one head's
 // state of one stream; the rows of K are spread over TY = 256 / TX threads per column group, whose partial
 // sums of q S are added over the lanes of a wave and then over the four waves in LDS.
@@ -101,7 +185,8 @@ __global__ __launch_bounds__(256) void step(const Step<IO> a) {
       ks[tid] = (float)a.k[b * a.kb + h * a.kh + tid];
       qs[tid] = (float)a.q[b * a.qb + h * a.qh + tid] * a.scale;
     }
-    const float d = expf(a.log_decay[h]);
+    float d, d_lo;
+    decay_of(a.log_decay[h], d, d_lo);
     float v[W], acc[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
@@ -123,7 +208,7 @@ __global__ __launch_bounds__(256) void step(const Step<IO> a) {
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          s[w] = fmaf(s[w], d, ks[x] * v[w]);
+          s[w] = fmaf(s[w], d, fmaf(s[w], d_lo, ks[x] * v[w]));
           acc[w] = fmaf(qs[x], s[w], acc[w]);
         }
         if constexpr (W == 4) {
@@ -157,6 +242,8 @@ int cu_count() {
   return n;
 }
 
+bool by_columns(const cet_linattn_desc& d);
+
 struct Operand {
   const void* p;
   Strides s;
@@ -167,7 +254,7 @@ struct Operand {
     const int vec = 16 / elem_bytes(d.dtype);
     const bool wide = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && D % vec == 0 && (s.b % vec == 0 || d.B == 1) &&
                       (s.t % vec == 0 || d.T == 1) && (s.h % vec == 0 || d.H == 1);
-    if (!wide) copy = align_up((size_t)d.B * d.T * d.H * ((D + vec - 1) / vec) * 16);
+    if (!wide && !by_columns(d)) copy = align_up((size_t)d.B * d.T * d.H * ((D + vec - 1) / vec) * 16);
   }
   int pack(const cet_linattn_desc& d, char*& ws, hipStream_t stream) {
     if (!copy) return CET_OK;
@@ -196,7 +283,13 @@ struct Cut {
   size_t states;  // bytes of the states between segments, K x V per head
 };
 
+// A lane per column: small heads, as long as there are waves for two to every SIMD or too few slots to cut.
+bool by_columns(const cet_linattn_desc& d) {
+  return d.K <= 16 && d.V <= 16 && (d.T <= OUT_SLOTS || (long)d.B * d.H * std::min(d.K, d.V) >= 64L * 8 * cu_count());
+}
+
 Cut cut(const cet_linattn_desc& d) {
+  if (by_columns(d)) return Cut{1, std::max(d.T, 1), 0};
   const int cols = slice_columns(d.dtype, d.K, d.V);
   const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
   long nseg = tasks ? std::min<long>((2L * cu_count() + tasks - 1) / tasks, chunks / 2) : 1;
@@ -243,11 +336,33 @@ int segment_states(Args a, const Cut& c, int dtype, hipStream_t s) {
   return CET_OK;
 }
 
+template <typename IO>
+void launch_columns(const Args& a, hipStream_t s) {
+  const auto step = [&](const void* p, const Strides& t) {
+    return a.K % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * sizeof(IO)) == 0 && (t.b | t.t | t.h) % 4 == 0 ? 4 : 1;
+  };
+  const unsigned blocks = (unsigned)(((long)a.B * a.H * a.V + 255) / 256);
+  if (a.K <= 8)
+    columns<IO, 8><<<blocks, 256, 0, s>>>(a, step(a.q, a.sq), step(a.k, a.sk));
+  else
+    columns<IO, 16><<<blocks, 256, 0, s>>>(a, step(a.q, a.sq), step(a.k, a.sk));
+}
+
 // One pass of the recurrence, segments from their states in ws (transposed: of the operands' roles exchanged).
-int pass(Args a, const Cut& c, bool transposed, int dtype, hipStream_t s) {
+int pass(Args a, const Cut& c, bool columns, bool transposed, int dtype, hipStream_t s) {
   a.nseg = c.nseg, a.seg_len = c.seg_len;
   a.ws_k = a.init_k = transposed ? 1 : a.V;
   a.ws_v = a.init_v = transposed ? a.K : 1;
+  if (columns) {
+    if (dtype == CET_F32)
+      launch_columns<float>(a, s);
+    else if (dtype == CET_F16)
+      launch_columns<_Float16>(a, s);
+    else
+      launch_columns<__bf16>(a, s);
+    CET_HIP(hipGetLastError());
+    return CET_OK;
+  }
   const int cols = slice_columns(dtype, a.K, a.V);
   a.nslice = (a.V + cols - 1) / cols;
   a.vec_o = a.V % 4 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
@@ -331,6 +446,7 @@ int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k
   for (Operand* x : {&oq, &ok, &ov})
     if (const int rc = x->pack(*d, ws, s)) return rc;
   const Cut c = cut(*d);
+  const bool columns = by_columns(*d);
   Args a{};
   a.q = oq.p, a.k = ok.p, a.v = ov.p, a.o = o;
   a.sq = oq.s, a.sk = ok.s, a.sv = ov.s, a.so = contiguous(*d, d->V);
@@ -340,7 +456,7 @@ int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k
   a.B = d->B, a.T = d->T, a.H = d->H, a.K = d->K, a.V = d->V;
   a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
   if (const int rc = segment_states(a, c, d->dtype, s)) return rc;
-  return pass(a, c, false, d->dtype, s);
+  return pass(a, c, columns, false, d->dtype, s);
 }
 
 int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
@@ -362,6 +478,7 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   for (Operand* x : {&oq, &ok, &ov, &og})
     if (const int rc = x->pack(*d, ws, s)) return rc;
   const Cut c = cut(*d);
+  const bool columns = by_columns(*d);
   float* const forward = states ? const_cast<float*>(states) : reinterpret_cast<float*>(ws);  // only read where given
   float* const back = reinterpret_cast<float*>(ws + c.states);
   Args a{};
@@ -380,7 +497,7 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   a.o = dq;
   a.K = d->V, a.V = d->K;
   a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
-  if (const int rc = pass(a, c, true, d->dtype, s)) return rc;
+  if (const int rc = pass(a, c, columns, true, d->dtype, s)) return rc;
   // the gradients of the states, backward in time, which the two other passes share
   a.ws = back;
   a.init = d_final;
@@ -392,13 +509,13 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   a.q = ov.p, a.sq = ov.s, a.k = og.p, a.sk = og.s, a.v = oq.p, a.sv = oq.s;
   a.o = dk;
   a.K = d->V, a.V = d->K;
-  if (const int rc = pass(a, c, true, d->dtype, s)) return rc;
+  if (const int rc = pass(a, c, columns, true, d->dtype, s)) return rc;
   // dv: (k, q, do) backward in time; the carry at the end is the gradient of the first state
   a.q = ok.p, a.sq = ok.s, a.k = oq.p, a.sk = oq.s, a.v = og.p, a.sv = og.s;
   a.o = dv, a.so = contiguous(*d, d->V);
   a.K = d->K, a.V = d->V;
   a.fin = d_initial;
-  return pass(a, c, false, d->dtype, s);
+  return pass(a, c, columns, false, d->dtype, s);
 }
 
 int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64_t* q_strides, const int64_t* k_strides,

@@ -73,7 +73,8 @@ def check(x, dtype, scale=None, y=None):
 SHAPES = [  # B, T, H, K, V
     (2, 1, 2, 8, 8), (1, 2, 1, 1, 1), (3, 15, 2, 16, 16), (2, 16, 1, 32, 32), (2, 17, 3, 20, 24), (1, 31, 2, 8, 100), (2, 32, 2, 64, 64),
     (2, 33, 1, 40, 72), (1, 63, 2, 128, 128), (1, 64, 1, 128, 64), (2, 65, 1, 100, 33), (1, 80, 2, 256, 256),
-    (1, 129, 1, 256, 8), (1, 97, 1, 8, 256), (1, 200, 1, 192, 130), (1, 70, 1, 3, 5)]
+    (1, 129, 1, 256, 8), (1, 97, 1, 8, 256), (1, 200, 1, 192, 130), (1, 70, 1, 3, 5),
+    (9, 25, 3, 8, 8), (70, 32, 5, 16, 7), (5, 11, 2, 5, 16), (3, 33, 2, 16, 16)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -92,9 +93,10 @@ def test_time_axis_in_segments(shape, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T", [1, 40, 700])
-def test_ragged_lengths_and_what_lies_behind_them(dtype, T):
+@pytest.mark.parametrize("K, V", [(24, 40), (8, 12)])
+def test_ragged_lengths_and_what_lies_behind_them(dtype, T, K, V):
     """Lengths of zero, one, T and beyond both ends; NaN and infinity behind the last slot are not read."""
-    x = make(6, T, 2, 24, 40, dtype, seed=T, ragged=True)
+    x = make(6, T, 2, K, V, dtype, seed=T, ragged=True)
     x["lengths"][:4] = torch.tensor([0, 1, T, min(T, 33)])
     y = gpu(x, dtype)
     for n in ("q", "k", "v", "d_o"):
@@ -110,9 +112,10 @@ def test_ragged_lengths_and_what_lies_behind_them(dtype, T):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_strides_and_alignment(dtype):
+@pytest.mark.parametrize("T", [45, 29])
+def test_strides_and_alignment(dtype, T):
     """Slices of one packed projection, heads before slots, and rows that start off 16 bytes."""
-    B, T, H, K = 2, 45, 3, 16
+    B, H, K = 2, 3, 16
     x = make(B, T, H, K, K, dtype, seed=5)
     want = check(x, dtype)
     y = gpu(x, dtype)
@@ -142,6 +145,36 @@ def test_decays_at_their_ends(dtype):
     check(x, dtype)
     check(x, dtype, scale=-0.3)
     check(x, dtype, scale=0.0)
+
+
+def test_many_small_heads_over_many_slots():
+    """A lane per column also for long histories where there are heads enough for it; the far weights hold."""
+    B, T, H, K = 4200, 130, 4, 8
+    g = torch.Generator(device="cuda").manual_seed(16)
+    q, k, v = (torch.randn(B, T, H, K, generator=g, device="cuda") for _ in range(3))
+    dec = torch.log1p(-torch.exp2(-torch.tensor([5.0, 8.0, 11.0, 14.0], device="cuda")))
+    o, s = cet.linear_attention(q, k, v, dec, scale=0.3)
+    pick = [0, 1, 2099, 4198, 4199]
+    x = [t[pick].double().cpu() for t in (q, k, v)]
+    want, S = ref.linear_attention(*x, dec.cpu(), 0.3)
+    mass, mS = ref.linear_attention(*(t.abs() for t in x), dec.cpu(), 0.3)
+    c = 1.01 * (K + T + 64) * 2.0 ** -24
+    within(o[pick], want, c * mass, "o")
+    within(s[pick], S, c * mS, "state")
+
+
+def test_a_thousand_single_slots_keep_far_weights():
+    """The state after many steps against the recurrence: (steps + 64) fp32 roundings, none of them the decay's own
+    raised to the number of steps."""
+    H, K, n = 2, 4, 3000
+    dec = torch.log1p(-torch.exp2(-torch.tensor([12.0, 16.0], device="cuda")))
+    s = torch.ones(1, H, K, K, device="cuda")
+    z = torch.zeros(1, H, K, device="cuda")
+    for _ in range(n):
+        cet.linear_attention_step(z, z, z, dec, s, inplace=True)
+    want = (n * dec.double()).exp().cpu().view(1, H, 1, 1).expand(1, H, K, K)
+    # each step rounds twice: 2 n / 2 units of 2^-24 at the worst
+    within(s, want, n * 2.0 ** -24 * want, "state")
 
 
 def test_histories_without_slots():

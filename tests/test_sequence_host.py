@@ -9,9 +9,9 @@ from channelestimationtransformer_amd import _cabi
 
 
 def desc(**kw):
-    d = _cabi.LinattnDesc(0, 2, 8, 2, 16, 16, 0, 0.25)
+    d = _cabi.LinattnDesc(0, 2, 8, 2, 32, 32, 0, 0.25)
     for n in ("q", "k", "v", "d_o"):
-        getattr(d, n)[:] = (256, 32, 16)
+        getattr(d, n)[:] = (512, 64, 32)
     for n, v in kw.items():
         setattr(d, n, v)
     return d
@@ -56,7 +56,7 @@ def test_linear_attention_pointers():
         assert L.cet_linear_attention(desc(), P, P, P, P, off[0], None, P, None, off[1], off[2], 1 << 20, None) == 1
     assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, None, None, 0, None) == 1  # copy without workspace
     n = L.cet_linear_attention_workspace(desc(), P + 4, P, P, None, 0)
-    assert n >= 2 * 8 * 2 * 16 * 4
+    assert n >= 2 * 8 * 2 * 32 * 4
     assert L.cet_linear_attention(desc(), P + 4, P, P, P, None, None, P, None, None, P, n - 1, None) == 1
     assert L.cet_linear_attention(desc(B=0), None, None, None, None, None, None, None, None, None, None, 0, None) == 0
     for hole in range(8):
