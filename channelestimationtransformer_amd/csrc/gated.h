@@ -42,7 +42,7 @@ struct Args {
   const void *bias_g, *bias_u;
   const void* dy;
   long ld_dy;
-  int dy_step;        // elements that a row of dy can be read at once: 4, 2 or 1
+  int dy_step;        // elements that a row of dy can be read at once: 8, 4, 2 or 1
   void *out, *out1;   // out[q][p], rows from `out_split` on to out1
   long ld_out;
   int out_split, out_step;
@@ -117,31 +117,52 @@ struct Tile {
 
   __device__ static int turn(int k) { return E == 2 ? 2 * ((k & 3) | (k >> 3 & 1) << 2) : 4 * (k >> 2 & 3); }
 
-  // piece of memory that goes to place `at`: index i0.. of the operand, k0.. of the summed axis
-  __device__ static const char* source(const Operand& o, int at, int i0, int len, int k0, int k_end) {
+  // Rows: the addresses of this thread's pieces are carried along, 128 bytes a tile; all of them are the same piece
+  // kc of their rows (NT / 8 rows apart, a multiple of the permutation's period).
+  const char* row_at[COLS ? 1 : N];
+
+  __device__ static int piece() { return (threadIdx.x & 7) ^ (threadIdx.x >> 4 & 7); }
+  // The first tile to fetch starts at index i0 and k0.
+  __device__ void init(const Operand& o, int i0, int len, int k0) {
     if constexpr (!COLS) {
-      const int r = at / 8, kc = (at & 7) ^ (r >> 1 & 7), k = k0 + kc * VEC;
-      // BACKWARD and FORWARD take rows of both weights in one tile: the second half from p1
-      const bool second = o.split < ROWS && r >= o.split;
-      const int i = min(i0 + (second ? r - o.split : r), len - 1);
-      const T* p = static_cast<const T*>(second ? o.p1 : o.p) + (long)i * (second ? o.ld1 : o.ld) + k;
-      return k < k_end ? reinterpret_cast<const char*>(p) : reinterpret_cast<const char*>(&zeros);
-    } else {
-      const int kr = at / PER_ROW, mc = at % PER_ROW ^ turn(kr);
-      int k = k0 + kr;
-      const bool second = k >= o.split;
-      bool live = k < k_end;
-      if (second) k -= o.split;
-      live = live && k < o.part;
-      const int i = min(i0 + mc * VEC, (len - 1) / VEC * VEC);
-      const T* p = static_cast<const T*>(second ? o.p1 : o.p) + (long)k * (second ? o.ld1 : o.ld) + i;
-      return live ? reinterpret_cast<const char*>(p) : reinterpret_cast<const char*>(&zeros);
+      static_assert(NT % 128 == 0, "rows of a thread's pieces a multiple of 16 apart");
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        // FORWARD and BACKWARD take rows of both weights in one tile: the second half from p1
+        const int r = (u * NT + (int)threadIdx.x) / 8;
+        const bool second = o.split < ROWS && r >= o.split;
+        const int i = min(i0 + (second ? r - o.split : r), len - 1);
+        row_at[u] = reinterpret_cast<const char*>(static_cast<const T*>(second ? o.p1 : o.p) + (long)i * (second ? o.ld1 : o.ld) + k0 + piece() * VEC);
+      }
     }
   }
-  __device__ static void fetch(const Operand& o, unsigned lds, int i0, int len, int k0, int k_end) {
+  // piece of memory that goes to place `at`: index i0.. of the operand, k0.. of the summed axis
+  __device__ static const char* source(const Operand& o, int at, int i0, int len, int k0, int k_end) {
+    const int kr = at / PER_ROW, mc = at % PER_ROW ^ turn(kr);
+    int k = k0 + kr;
+    const bool second = k >= o.split;
+    bool live = k < k_end;
+    if (second) k -= o.split;
+    live = live && k < o.part;
+    const int i = min(i0 + mc * VEC, (len - 1) / VEC * VEC);
+    const T* p = static_cast<const T*>(second ? o.p1 : o.p) + (long)k * (second ? o.ld1 : o.ld) + i;
+    return live ? reinterpret_cast<const char*>(p) : reinterpret_cast<const char*>(&zeros);
+  }
+  // The tiles follow each other: k0 is BK behind that of the call before.
+  __device__ void fetch(const Operand& o, unsigned lds, int i0, int len, int k0, int k_end) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned to = lds + wave * 1024;
+    if constexpr (COLS) {
 #pragma unroll
-    for (int u = 0; u < N; ++u) dma16(source(o, u * NT + (int)threadIdx.x, i0, len, k0, k_end), lds + (u * NT + wave * 64) * 16);
+      for (int u = 0; u < N; ++u) dma16(source(o, u * NT + (int)threadIdx.x, i0, len, k0, k_end), to + u * NT * 16);
+    } else {
+      const bool live = k0 + piece() * VEC < k_end;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        dma16(live ? row_at[u] : reinterpret_cast<const char*>(&zeros), to + u * NT * 16);
+        row_at[u] += 128;
+      }
+    }
   }
   // indices r0..r0+15 of step kk (64 bytes of k) as an operand of the matrix instructions
   __device__ static Frag read(const char* t, int r0, int kk, int i, int g) {
@@ -225,7 +246,7 @@ template <typename T>
 __device__ inline void store4(T* p, const f4& v, int n, int step) {
   typedef T t4 __attribute__((ext_vector_type(4)));
   typedef T t2 __attribute__((ext_vector_type(2)));
-  if (n >= 4 && step == 4) {
+  if (n >= 4 && step >= 4) {
     *reinterpret_cast<t4*>(p) = t4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
   } else if (n >= 4 && step == 2) {
     *reinterpret_cast<t2*>(p) = t2{(T)v[0], (T)v[1]};
@@ -241,7 +262,7 @@ __device__ inline f4 load4(const T* p, int n, int step) {
   typedef T t4 __attribute__((ext_vector_type(4)));
   typedef T t2 __attribute__((ext_vector_type(2)));
   f4 v = {0.f, 0.f, 0.f, 0.f};
-  if (n >= 4 && step == 4) {
+  if (n >= 4 && step >= 4) {
     const t4 x = *reinterpret_cast<const t4*>(p);
     v = f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
   } else if (n >= 4 && step == 2) {
@@ -253,6 +274,41 @@ __device__ inline f4 load4(const T* p, int n, int step) {
       if (r < n) v[r] = (float)p[r];
   }
   return v;
+}
+
+// n values of a 16-byte piece at a time: whole where rows start on 16 bytes (step 16 / sizeof(T)), in 4 bytes or singly
+template <typename T>
+__device__ inline uint4 load_piece(const T* p, int n, int step) {
+  constexpr int VEC = 16 / sizeof(T), W = 4 / sizeof(T);
+  if (n >= VEC && step >= VEC) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (n >= VEC && step >= W) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const uint32_t*>(p)[j];
+  } else {
+    T e[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = j < n ? p[j] : (T)0.f;
+    __builtin_memcpy(w, e, 16);
+  }
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+template <typename T>
+__device__ inline void store_piece(T* p, const uint4& raw, int n, int step) {
+  constexpr int VEC = 16 / sizeof(T), W = 4 / sizeof(T);
+  if (n >= VEC && step >= VEC) {
+    *reinterpret_cast<uint4*>(p) = raw;
+  } else if (n >= VEC && step >= W) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(p)[j] = w[j];
+  } else {
+    T e[VEC];
+    __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (j < n) p[j] = e[j];
+  }
 }
 
 template <int N>
@@ -296,10 +352,12 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
 #pragma unroll
     for (int y = 0; y < NQT; ++y) acc[x][y] = f4{0.f, 0.f, 0.f, 0.f};
 
-  auto fetch = [&](int k0, int buf) {
-    TP::fetch(a.P, base + buf * BUF, p0, a.np, k0, k_end);
-    TQ::fetch(a.Q, base + buf * BUF + TP::BYTES, q0, a.nq, k0, k_end);
-  };
+  TP from_p;
+  TQ from_q;
+  from_p.init(a.P, p0, a.np, k_first);
+  from_q.init(a.Q, q0, a.nq, k_first);
+  auto fetch_p = [&](int k0, int buf) { from_p.fetch(a.P, base + buf * BUF, p0, a.np, k0, k_end); };
+  auto fetch_q = [&](int k0, int buf) { from_q.fetch(a.Q, base + buf * BUF + TP::BYTES, q0, a.nq, k0, k_end); };
   // first row of the wave's tile x of P: gate rows, then the up rows of the same features
   auto p_row = [&](int x) {
     return GATED ? (x < NPT / 2 ? wp * (BP / 2 / WP) + 16 * x : BP / 2 + wp * (BP / 2 / WP) + 16 * (x - NPT / 2)) : wp * (BP / WP) + 16 * x;
@@ -308,7 +366,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
   // A tile is worked on in four steps: half of its 128 bytes of k and half of the wave's tiles of P each. The
   // operands of a step travel from LDS into one set of registers while the matrix instructions work on the other,
   // across the barrier too: before the last step of a tile the next tile has landed, this one is all in registers,
-  // and its buffer takes the rows of the tile after. (Whole steps of k need 32 registers more and spilled where
+  // and its buffer takes the rows of the tile after, P's at once and Q's behind the next step (3 % over both at once). (Whole steps of k need 32 registers more and spilled where
   // operands are read by columns.)
   constexpr int HP = NPT / 2;
   Frag p0_[HP], p1_[HP], q0_[NQT], q1_[NQT];
@@ -330,10 +388,13 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
       for (int y = 0; y < NQT; ++y) acc[decltype(half)::value * HP + x][y] = mma<T>(fp[x], fq[y], acc[decltype(half)::value * HP + x][y]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (k_first < k_end) fetch(k_first, 0);
+  if (k_first < k_end) {
+    fetch_p(k_first, 0);
+    fetch_q(k_first, 0);
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (k_first + BK < k_end) fetch(k_first + BK, 1);
+  if (k_first + BK < k_end) fetch_p(k_first + BK, 1);
   if (k_first < k_end) {
     load_q(q0_, 0, 0);
     load_p(p0_, 0, 0, 0);
@@ -341,6 +402,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
   int buf = 0;
   for (int k0 = k_first; k0 < k_end; k0 += BK, buf ^= 1) {
     load_p(p1_, buf, 0, 1);
+    if (k0 + BK < k_end) fetch_q(k0 + BK, buf ^ 1);
     multiply(p0_, q0_, Half<0>());
     load_q(q1_, buf, 1);
     load_p(p0_, buf, 1, 0);
@@ -349,7 +411,7 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
     multiply(p0_, q1_, Half<0>());
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (k0 + 2 * BK < k_end) fetch(k0 + 2 * BK, buf);
+    if (k0 + 2 * BK < k_end) fetch_p(k0 + 2 * BK, buf);
     if (k0 + BK < k_end) {
       load_q(q0_, buf ^ 1, 0);
       load_p(p0_, buf ^ 1, 0, 0);
@@ -358,58 +420,89 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
   }
 
   if constexpr (GATED) {
+    // Results (and dy on its way in) go through LDS, so that memory sees whole pieces of 16 bytes along the rows: a
+    // lane holds 4 features of a row, 16 rows apart from its neighbours'. (dy and dh read and written from the
+    // accumulators' places: 66 us over the forward product's time at 8192 x 1024 x 2730, this way 30.) Rows of 256
+    // bytes at most, so fp32 takes two rounds in the large tile.
+    constexpr int E = Type<T>::E, VEC = 16 / E, XT = NPT / 2 * E > 8 ? 2 : NPT / 2, ROUNDS = NPT / 2 / XT;
+    constexpr int PIECES = WP * 16 * XT / VEC, SHARE = 16 / PIECES;
+    static_assert(2 * BQ * PIECES * 16 <= 2 * BUF, "two tiles of results in the operands' buffers");
+    char* const first = lds;
+    char* const second = lds + BQ * PIECES * 16;
+    auto turn = [](int row) { return row / SHARE & (PIECES - 1); };
+    // feature behind p0 of piece p in a round
+    auto feature = [](int p, int round) { return p * VEC / (16 * XT) * (BP / 2 / WP) + round * 16 * XT + p * VEC % (16 * XT); };
+    for (int round = 0; round < ROUNDS; ++round) {
+      if (round) __syncthreads();
+      if constexpr (KIND == BACKWARD) {
+        for (int at = threadIdx.x; at < BQ * PIECES; at += NT) {
+          const int row = at / PIECES, p = at % PIECES, q = q0 + row, f = p0 + feature(p, round), n = a.F - f;
+          uint4 raw = {0, 0, 0, 0};
+          if (q < a.nq && n > 0) raw = load_piece(static_cast<const T*>(a.dy) + (long)q * a.ld_dy + f, n, a.dy_step);
+          *reinterpret_cast<uint4*>(first + (row * PIECES + (p ^ turn(row))) * 16) = raw;
+        }
+        __syncthreads();
+      }
 #pragma unroll
-    for (int x = 0; x < NPT / 2; ++x) {
-      const int f = p0 + wp * (BP / 2 / WP) + 16 * x + 4 * g, n = a.F - f;
-      f4 bg = {0.f, 0.f, 0.f, 0.f}, bu = bg, sg = bg, su = bg;
-      if (a.bias_g) bg = load4(static_cast<const T*>(a.bias_g) + f, n, 1);
-      if (a.bias_u) bu = load4(static_cast<const T*>(a.bias_u) + f, n, 1);
+      for (int xr = 0; xr < NPT / 2; ++xr) {
+        if (xr / XT != round) continue;
+        const int f = p0 + wp * (BP / 2 / WP) + 16 * xr + 4 * g, n = a.F - f;
+        const int byte = (wp * 16 * XT + 16 * (xr % XT) + 4 * g) * E;
+        f4 bg = {0.f, 0.f, 0.f, 0.f}, bu = bg, sg = bg, su = bg;
+        if (a.bias_g) bg = load4(static_cast<const T*>(a.bias_g) + f, n, 1);
+        if (a.bias_u) bu = load4(static_cast<const T*>(a.bias_u) + f, n, 1);
 #pragma unroll
-      for (int y = 0; y < NQT; ++y) {
-        const int q = q0 + wq * (BQ / WQ) + 16 * y + i;
-        f4 gv = acc[x][y] + bg, uv = acc[x + NPT / 2][y] + bu;
-        if constexpr (KIND == FORWARD) {
-          f4 v, slope;
+        for (int y = 0; y < NQT; ++y) {
+          const int row = wq * (BQ / WQ) + 16 * y + i;
+          T* const place = reinterpret_cast<T*>(first + (row * PIECES + (byte / 16 ^ turn(row))) * 16 + byte % 16);
+          f4 gv = acc[xr][y] + bg, uv = acc[xr + NPT / 2][y] + bu, v, slope;
           act4(a.activation, gv, v, slope);
-          if (q < a.nq && n > 0) store4(static_cast<T*>(a.out) + (long)q * a.ld_out + f, v * uv, n, a.out_step);
-        } else {
-          f4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
-          if (q < a.nq && n > 0) {
-            const f4 d = load4(static_cast<const T*>(a.dy) + (long)q * a.ld_dy + f, n, a.dy_step);
-            f4 v, slope;
-            act4(a.activation, gv, v, slope);
+          if constexpr (KIND == FORWARD) {
+            store4(place, v * uv, 4, 4);
+          } else {
+            const f4 d = load4(place, 4, 4);
+            f4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              if (r < n) {
+              if (r < n && q0 + row < a.nq) {  // columns behind F are summed over in the products behind this one: zero
                 dg[r] = d[r] * uv[r] * slope[r];
                 du[r] = d[r] * v[r];
               }
             }
+            sg += dg;
+            su += du;
+            store4(place, dg, 4, 4);
+            store4(reinterpret_cast<T*>(reinterpret_cast<char*>(place) + (second - first)), du, 4, 4);
           }
-          sg += dg;
-          su += du;
-          // dh is summed over in the two products behind this one: its columns behind F are zero
-          if (q < a.nq && f < a.Fp) {
-            T* to = static_cast<T*>(a.out) + (long)q * a.ld_out + f;
-            store4(to, dg, 4, 4);
-            store4(to + a.Fp, du, 4, 4);
+        }
+        if constexpr (KIND == BACKWARD) {
+          if (a.part) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int off = 1; off < 16; off *= 2) {
+                sg[r] += __shfl_xor(sg[r], off);
+                su[r] += __shfl_xor(su[r], off);
+              }
+            if (i == 0 && f < a.Fp) {
+              float* to = a.part + (long)(tq * WQ + wq) * 2 * a.Fp + f;
+              *reinterpret_cast<f4*>(to) = sg;
+              *reinterpret_cast<f4*>(to + a.Fp) = su;
+            }
           }
         }
       }
-      if constexpr (KIND == BACKWARD) {
-        if (a.part) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int off = 1; off < 16; off *= 2) {
-              sg[r] += __shfl_xor(sg[r], off);
-              su[r] += __shfl_xor(su[r], off);
-            }
-          if (i == 0 && f < a.Fp) {
-            float* to = a.part + (long)(tq * WQ + wq) * 2 * a.Fp + f;
-            *reinterpret_cast<f4*>(to) = sg;
-            *reinterpret_cast<f4*>(to + a.Fp) = su;
-          }
+      __syncthreads();
+      for (int at = threadIdx.x; at < BQ * PIECES; at += NT) {
+        const int row = at / PIECES, p = at % PIECES, q = q0 + row, f = p0 + feature(p, round);
+        const int from = (row * PIECES + (p ^ turn(row))) * 16;
+        if (q >= a.nq) continue;
+        if constexpr (KIND == FORWARD) {
+          if (f < a.F) store_piece(static_cast<T*>(a.out) + (long)q * a.ld_out + f, *reinterpret_cast<const uint4*>(first + from), a.F - f, a.out_step);
+        } else if (f < a.Fp) {
+          T* to = static_cast<T*>(a.out) + (long)q * a.ld_out + f;
+          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(first + from);
+          *reinterpret_cast<uint4*>(to + a.Fp) = *reinterpret_cast<const uint4*>(second + from);
         }
       }
     }

@@ -226,7 +226,7 @@ struct Matrix {
 
 int step_of(const void* p, long ld, int dtype) {  // elements that a row can be read or written at once
   const uintptr_t at = reinterpret_cast<uintptr_t>(p) / elem_bytes(dtype);
-  return (at | ld) % 4 == 0 ? 4 : (at | ld) % 2 == 0 ? 2 : 1;
+  return (at | ld) % 8 == 0 ? 8 : (at | ld) % 4 == 0 ? 4 : (at | ld) % 2 == 0 ? 2 : 1;
 }
 
 constexpr int FEW = 64;
