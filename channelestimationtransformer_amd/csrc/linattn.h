@@ -246,6 +246,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
   const int end = min(rows, first + a.seg_len);
   const int c0 = slice * SL, col = c0 + wc * 16 * NV;  // first column of V: of the workgroup, of the wave
   const int k0 = kh * NKW * 16;                        // first row of the wave's part of S
+  const bool busy = col < a.V;  // the last slice may leave waves with nothing but their share of rows and scores
 
   const IO* q = static_cast<const IO*>(a.q) + b * a.sq.b + h * a.sq.h;
   const IO* k = static_cast<const IO*>(a.k) + b * a.sk.b + h * a.sk.h;
@@ -337,7 +338,10 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
                   TK::rows(qt, 16 * tb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x + 16, i, g), p);
     } else {
 #pragma unroll
-      for (int x = 0; x < NK; ++x) p = mma16(TK::rows(kt, 16 * sb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x, i, g), p);
+      for (int x = 0; x < NK; ++x) {
+        if (16 * x >= a.K) break;  // in fp32 the matrix instructions are what counts: none for columns that do not exist
+        p = mma16(TK::rows(kt, 16 * sb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x, i, g), p);
+      }
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) p[r] = sb == tb ? (i >= 4 * g + r ? p[r] * wd[r] : 0.f) : p[r] * wo[r];
@@ -385,12 +389,13 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
       for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
         for (int y = 0; y < NV; ++y) acc[tb][y] = f4{0.f, 0.f, 0.f, 0.f};
-      if (have) {
+      if (have && busy) {
         // the state enters this product rounded to bf16 (where the tensors are), the only place where it is: an
         // error of at most half a step of the output's own type on its share of the sum
         const float dm = pw_fast(g2, m);
 #pragma unroll
-        for (int x = 0; x < NKW; x += Ty::BF ? 2 : 1)
+        for (int x = 0; x < NKW; x += Ty::BF ? 2 : 1) {
+          if (!Ty::BF && k0 + 16 * x >= a.K) break;
 #pragma unroll
           for (int tb = 0; tb < NB; ++tb) {
             if constexpr (Ty::BF) {
@@ -403,6 +408,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
               for (int y = 0; y < NV; ++y) acc[tb][y] = mma16(S[x][y], q0, acc[tb][y]);
             }
           }
+        }
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb)
 #pragma unroll
@@ -414,7 +420,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
       }
     }
 
-    if (!OUT || at + C < end || a.fin) {  // nobody reads the state behind the last slot otherwise
+    if (busy && (!OUT || at + C < end || a.fin)) {  // nobody reads the state behind the last slot otherwise
       float w[NB][4];
       if (slow) {
         if (fabsf(g2) * (float)(m + C) > 20.f) {
@@ -474,6 +480,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
             for (int r = 0; r < 4; ++r) vw[y][r] = vf[sb][y][r] * w[sb][r];
 #pragma unroll
           for (int x = 0; x < NKW; ++x) {
+            if (k0 + 16 * x >= a.K) break;
             const f4 kq = TK::cols(kt, 16 * sb, k0 + 16 * x, i, g);
 #pragma unroll
             for (int y = 0; y < NV; ++y) S[x][y] = mma16(kq, vw[y], S[x][y]);
@@ -497,7 +504,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
     if (at + BUFS * C < end) fetch(at + BUFS * C, buf);
     buf = buf == BUFS - 1 ? 0 : buf + 1;
 
-    if (OUT) {
+    if (OUT && busy) {
       if constexpr (SHARE) {
 #pragma unroll
         for (int x = 0; x < BLOCKS; ++x) pf[x] = ps[flip][x][lane];
