@@ -147,25 +147,31 @@ struct Tile {
     const int u = r / SHARE256;  // rows of this many share the banks' 256 bytes
     return E == 2 ? ((u & (PB / 2 - 1)) << 1 | (r >> 3 & 1)) & (PB - 1) : u & (PB - 1);
   }
-  __device__ static Quad rows(const char* t, int r0, int c0, int i, int g) {
-    const int r = r0 + i;
-    const char* p = E == 2 ? t + r * (COLS * E) + ((c0 / VEC + (g >> 1) ^ turn(r)) << 4) + (g & 1) * 8
-                           : t + r * (COLS * E) + ((c0 / VEC + g ^ turn(r)) << 4);
-    return Type<IO>::quad(*reinterpret_cast<const V4*>(p));
+  // A lane's address for the 16 x 16 tile (sb, x): rows 16 sb.., columns 16 x... The pieces of column tile x differ from
+  // those of tile 0 in bits that the permutation only flips, so one address per operand and an exclusive or serve
+  // all of them (addresses kept for each tile took a hundred registers).
+  static constexpr int ROW = COLS * E, SHIFT = E == 2 ? 5 : 6;
+  template <typename X>
+  __device__ static X at(unsigned p) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) X*>(p);
   }
-  __device__ static Quad cols(const char* t, int r0, int c0, int i, int g) {
+  __device__ static unsigned rows_base(int i, int g) {
+    return E == 2 ? i * ROW + (((g >> 1) ^ turn(i)) << 4) + (g & 1) * 8 : i * ROW + ((g ^ turn(i)) << 4);
+  }
+  __device__ static unsigned cols_base(int i, int g, int j) {  // fp32: one for each of the four rows
+    const int r = 4 * g + (E == 2 ? i >> 2 : j);
+    return E == 2 ? r * ROW + (((i >> 1 & 1) ^ turn(r)) << 4) + (i & 1) * 8 : r * ROW + (((i >> 2) ^ turn(r)) << 4) + (i & 3) * 4;
+  }
+  __device__ static Quad rows(unsigned base, int sb, int x) { return Type<IO>::quad(at<V4>((base ^ x << SHIFT) + sb * 16 * ROW)); }
+  __device__ static Quad cols(const unsigned (&base)[E == 2 ? 1 : 4], int sb, int x) {
     if constexpr (E == 2) {
       typedef __attribute__((address_space(3))) s4* lds_s4;
-      const int r = r0 + 4 * g + (i >> 2);
-      const char* p = t + r * (COLS * E) + ((c0 / VEC + (i >> 1 & 1) ^ turn(r)) << 4) + (i & 1) * 8;
-      return Type<IO>::quad(__builtin_bit_cast(V4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p)));
+      const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)((base[0] ^ x << SHIFT) + sb * 16 * ROW));
+      return Type<IO>::quad(__builtin_bit_cast(V4, r));
     } else {
       f4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = r0 + 4 * g + j, c = c0 + i;
-        v[j] = *reinterpret_cast<const float*>(t + r * (COLS * E) + ((c / VEC ^ turn(r)) << 4) + (c & 3) * 4);
-      }
+      for (int j = 0; j < 4; ++j) v[j] = at<float>((base[j] ^ x << SHIFT) + sb * 16 * ROW);
       return v;
     }
   }
@@ -329,18 +335,16 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
     for (int r = 0; r < 4; ++r) wk[sb][r] = slow ? pw(g2, -(16 * sb + 4 * g + r + e)) * a.s_kv : 0.f;
 
   // block (tb, sb) of the scores, decayed, as an operand
-  auto scores = [&](const char* qt, const char* kt, int tb, int sb) {
+  auto scores = [&](unsigned qr, unsigned kr, int tb, int sb) {
     f4 p = f4{0.f, 0.f, 0.f, 0.f};
     if constexpr (Ty::BF) {
 #pragma unroll
-      for (int x = 0; x < NK; x += 2)
-        p = mma32(TK::rows(kt, 16 * sb, 16 * x, i, g), TK::rows(kt, 16 * sb, 16 * x + 16, i, g),
-                  TK::rows(qt, 16 * tb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x + 16, i, g), p);
+      for (int x = 0; x < NK; x += 2) p = mma32(TK::rows(kr, sb, x), TK::rows(kr, sb, x + 1), TK::rows(qr, tb, x), TK::rows(qr, tb, x + 1), p);
     } else {
 #pragma unroll
       for (int x = 0; x < NK; ++x) {
         if (16 * x >= a.K) break;  // in fp32 the matrix instructions are what counts: none for columns that do not exist
-        p = mma16(TK::rows(kt, 16 * sb, 16 * x, i, g), TK::rows(qt, 16 * tb, 16 * x, i, g), p);
+        p = mma16(TK::rows(kr, sb, x), TK::rows(qr, tb, x), p);
       }
     }
 #pragma unroll
@@ -361,16 +365,24 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  constexpr int CB = sizeof(IO) == 2 ? 1 : 4;
+  const unsigned row_lane = TK::rows_base(i, g);
+  unsigned k_lane[CB], v_lane[CB];
+#pragma unroll
+  for (int j = 0; j < CB; ++j) k_lane[j] = TK::cols_base(i, g, j), v_lane[j] = TV::cols_base(i, g, j);
   int buf = 0;
   for (int at = first; at < end; at += C) {
     const int n = min(C, end - at);
-    const char *kt = tiles[buf], *vt = kt + TK::BYTES, *qt = vt + TV::BYTES;
+    const unsigned kt = lds + buf * BUF, vt = kt + TK::BYTES, kr = kt + row_lane, qr = vt + TV::BYTES + row_lane;
+    unsigned kc[CB], vc[CB];
+#pragma unroll
+    for (int j = 0; j < CB; ++j) kc[j] = kt + k_lane[j], vc[j] = vt + v_lane[j];
 
     Quad vf[NB][NV];
 #pragma unroll
     for (int sb = 0; sb < NB; ++sb)
 #pragma unroll
-      for (int y = 0; y < NV; ++y) vf[sb][y] = TV::cols(vt, 16 * sb, wc * 16 * NV + 16 * y, i, g);
+      for (int y = 0; y < NV; ++y) vf[sb][y] = TV::cols(vc, sb, wc * NV + y);
 
     f4 acc[OUT ? NB : 1][NV];
     Quad pf[OUT ? BLOCKS : 1];
@@ -380,9 +392,9 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
 #pragma unroll
       for (int x = 0; x < BLOCKS; ++x) {
         if constexpr (SHARE) {
-          if (x % NW == wave) ps[flip][x][lane] = scores(qt, kt, TB[x], SB[x]);
+          if (x % NW == wave) ps[flip][x][lane] = scores(qr, kr, TB[x], SB[x]);
         } else {
-          pf[x] = scores(qt, kt, TB[x], SB[x]);
+          pf[x] = scores(qr, kr, TB[x], SB[x]);
         }
       }
 #pragma unroll
@@ -399,11 +411,11 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
 #pragma unroll
           for (int tb = 0; tb < NB; ++tb) {
             if constexpr (Ty::BF) {
-              const Quad q0 = TK::rows(qt, 16 * tb, k0 + 16 * x, i, g), q1 = TK::rows(qt, 16 * tb, k0 + 16 * x + 16, i, g);
+              const Quad q0 = TK::rows(qr, tb, k0 / 16 + x), q1 = TK::rows(qr, tb, k0 / 16 + x + 1);
 #pragma unroll
               for (int y = 0; y < NV; ++y) acc[tb][y] = mma32(to_bf(S[x][y]), to_bf(S[x + 1][y]), q0, q1, acc[tb][y]);
             } else {
-              const Quad q0 = TK::rows(qt, 16 * tb, k0 + 16 * x, i, g);
+              const Quad q0 = TK::rows(qr, tb, k0 / 16 + x);
 #pragma unroll
               for (int y = 0; y < NV; ++y) acc[tb][y] = mma16(S[x][y], q0, acc[tb][y]);
             }
@@ -460,7 +472,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
           }
 #pragma unroll
         for (int x = 0; x < NKW; ++x) {
-          const bf4 kq0 = TK::cols(kt, 16 * sb, k0 + 16 * x, i, g), kq1 = TK::cols(kt, 16 * sb + 16, k0 + 16 * x, i, g);
+          const bf4 kq0 = TK::cols(kc, sb, k0 / 16 + x), kq1 = TK::cols(kc, sb + 1, k0 / 16 + x);
 #pragma unroll
           for (int y = 0; y < NV; ++y) {
             S[x][y] = mma32(kq0, kq1, t2[0][y], t2[1][y], S[x][y]);
@@ -481,7 +493,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
 #pragma unroll
           for (int x = 0; x < NKW; ++x) {
             if (k0 + 16 * x >= a.K) break;
-            const f4 kq = TK::cols(kt, 16 * sb, k0 + 16 * x, i, g);
+            const f4 kq = TK::cols(kc, sb, k0 / 16 + x);
 #pragma unroll
             for (int y = 0; y < NV; ++y) S[x][y] = mma16(kq, vw[y], S[x][y]);
           }
