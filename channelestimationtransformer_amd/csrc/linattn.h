@@ -196,6 +196,13 @@ __device__ inline Source source(const IO* p, long st, int rows, int end, int rev
   return Source{reinterpret_cast<const char*>(p + c0 + (reverse ? (rows - 1) * st : 0)), (reverse ? -st : st) * (long)sizeof(IO), end, cols - c0};
 }
 
+// Columns of the staged rows of q and k: a power of two, for the permutation, and 64 bytes at least.
+constexpr int row_width(int nk, size_t bytes) {
+  int w = bytes == 2 ? 32 : 16;
+  while (w < 16 * nk) w *= 2;
+  return w;
+}
+
 template <int NK, int NV>
 __device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
 #pragma unroll
@@ -212,11 +219,11 @@ __device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
 // column each finishes the outputs of one block of 16 slots, with the other's half of q S for it, which comes
 // through LDS behind the same barrier.
 template <typename IO, int NK, int NV, int WC, int KH, bool OUT>
-__global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(const Args a) {
+__global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) void chunks(const Args a) {
   typedef Type<IO> Ty;
   typedef typename Ty::Quad Quad;
-  constexpr int C = OUT ? OUT_SLOTS : STATE_SLOTS, NB = C / 16;
-  constexpr int NW = WC * KH, DK = 16 * NK, NKW = NK / KH, SL = 16 * NV * WC;
+  constexpr int C = OUT || (WC == 8 && sizeof(IO) == 4) ? OUT_SLOTS : STATE_SLOTS, NB = C / 16;  // two workgroups on a CU
+  constexpr int NW = WC * KH, DK = row_width(NK, sizeof(IO)), NKW = NK / KH, SL = 16 * NV * WC;
   constexpr bool SHARE = NW > 1;  // one wave keeps its scores
   constexpr int BLOCKS = NB * (NB + 1) / 2, MINE = KH == 2 ? 1 : NB;
   static_assert((!OUT || NB == 2) && KH <= 2 && NK % KH == 0, "two blocks of slots in a chunk with outputs");
@@ -234,15 +241,18 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
 
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, kh = wave / WC;
-  // Workgroups go to the 8 XCDs in turn: an XCD is given one run of them, so that the slices of a head, which
-  // read the same q and k, share its L2.
+  // Workgroups go to the 8 XCDs in turn: the slices of a segment, which read the same q and k, are given to one, and
+  // share its L2; the segments of one sequence are spread over all, so that long ones keep no XCD busy alone (32
+  // sequences, the first four full and the others of 64 slots, 16 heads, bf16: 200 us, by runs of workgroups 263).
   unsigned id = blockIdx.x;
-  {
-    const unsigned per = gridDim.x / 8, rest = gridDim.x % 8, xcd = id % 8;
-    id = xcd * per + min(xcd, rest) + id / 8;
+  int slice;
+  if (const unsigned eight = 8 * a.nslice, whole = gridDim.x / eight * eight; id < whole) {
+    slice = id / 8 % a.nslice;
+    id = id / eight * 8 + id % 8;
+  } else {
+    slice = id % a.nslice;
+    id /= a.nslice;
   }
-  const int slice = id % a.nslice;
-  id /= a.nslice;
   const int nseg_here = OUT ? a.nseg : a.nseg - 1;  // without outputs the last segment has nothing to add
   const int seg = id % nseg_here;
   const long bh = id / nseg_here;
@@ -342,10 +352,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
       for (int x = 0; x < NK; x += 2) p = mma32(TK::rows(kr, sb, x), TK::rows(kr, sb, x + 1), TK::rows(qr, tb, x), TK::rows(qr, tb, x + 1), p);
     } else {
 #pragma unroll
-      for (int x = 0; x < NK; ++x) {
-        if (16 * x >= a.K) break;  // in fp32 the matrix instructions are what counts: none for columns that do not exist
-        p = mma16(TK::rows(kr, sb, x), TK::rows(qr, tb, x), p);
-      }
+      for (int x = 0; x < NK; ++x) p = mma16(TK::rows(kr, sb, x), TK::rows(qr, tb, x), p);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) p[r] = sb == tb ? (i >= 4 * g + r ? p[r] * wd[r] : 0.f) : p[r] * wo[r];
@@ -407,7 +414,6 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
         const float dm = pw_fast(g2, m);
 #pragma unroll
         for (int x = 0; x < NKW; x += Ty::BF ? 2 : 1) {
-          if (!Ty::BF && k0 + 16 * x >= a.K) break;
 #pragma unroll
           for (int tb = 0; tb < NB; ++tb) {
             if constexpr (Ty::BF) {
@@ -492,7 +498,6 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
             for (int r = 0; r < 4; ++r) vw[y][r] = vf[sb][y][r] * w[sb][r];
 #pragma unroll
           for (int x = 0; x < NKW; ++x) {
-            if (k0 + 16 * x >= a.K) break;
             const f4 kq = TK::cols(kc, sb, k0 / 16 + x);
 #pragma unroll
             for (int y = 0; y < NV; ++y) S[x][y] = mma16(kq, vw[y], S[x][y]);
@@ -557,11 +562,19 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
   }
 
   if (OUT) {
-    // slots behind the sequence's end
-    const int from = max(rows, first), to = min(a.T, first + a.seg_len);
-    const int wide = min(a.V, c0 + SL) - c0;
-    for (long at = (long)from * wide + threadIdx.x; at < (long)to * wide; at += 64 * NW)
-      Ty::store(o + at / wide * a.so.t + c0 + at % wide, 0.f);
+    // slots behind the sequence's end: four columns a thread
+    constexpr int LPR = SL / 4;
+    const int to = min(a.T, first + a.seg_len), vv = c0 + 4 * (int)(threadIdx.x % LPR);
+    for (int at = max(rows, first) + (int)(threadIdx.x / LPR); at < to; at += 64 * NW / LPR) {
+      IO* p = o + at * a.so.t + vv;
+      if (a.vec_o && vv + 4 <= a.V) {
+        Ty::store4(p, f4{0.f, 0.f, 0.f, 0.f});
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (vv + r < a.V) Ty::store(p + r, 0.f);
+      }
+    }
   }
   if (m) multiply_out(S, pw(g2, m));
   float* to = nullptr;
@@ -586,13 +599,14 @@ __global__ __launch_bounds__(64 * WC * KH, WC * KH == 1 ? 1 : 2) void chunks(con
 }
 
 // Columns of V that a workgroup takes: 16 (one wave, as long as that wave can bring in the rows of K in few
-// instructions); 128 in bf16 up to K = 128, where four waves hold their state in 64 registers each; else 64, and 32
-// where rows of 256 fp32 fill LDS. (bf16, 128 x 128, 8 x 16 heads x 2048 slots: 82 us a pass; 64 columns by eight
-// waves, two to the K of a column, 101 us, and 119 us with one workgroup per CU and no segments.)
+// instructions); 128 in bf16 up to K = 128, where four waves hold their state in 64 registers each, and in fp32 up to
+// K = 64, by eight waves; else 64, and 32 where rows of 256 fp32 fill LDS. (bf16, 128 x 128, 8 x 16 heads x 2048
+// slots: 82 us a pass; 64 columns by eight waves, two to the K of a column, 101 us, and 119 us with one workgroup per
+// CU and no segments. fp32, 40 x 72, 16 x 6 heads of up to 777 slots: 35 us, by slices of 64 columns 50.)
 inline int slice_columns(int dtype, int K, int V) {
   if (V <= 16 && K <= 64) return 16;
   if (K > 128 && dtype != CET_BF16) return 32;
-  return V > 64 && K <= 128 && dtype == CET_BF16 ? 128 : 64;
+  return V > 64 && K <= (dtype == CET_BF16 ? 128 : 64) ? 128 : 64;
 }
 
 template <typename IO, int NK, bool OUT>
@@ -601,29 +615,49 @@ inline void launch_k(const Args& a, unsigned blocks, hipStream_t s) {
   const int cols = slice_columns(BF ? CET_BF16 : CET_F32, a.K, a.V);
   if constexpr (NK <= 4)
     if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(a);
+  if constexpr (NK <= 4 && !BF)
+    if (cols == 128) return chunks<IO, NK, 1, 8, 1, OUT><<<blocks, 512, 0, s>>>(a);
   if constexpr (NK <= 8 && BF)
     if (cols == 128) return chunks<IO, NK, 2, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
   if constexpr (NK <= 4)
     chunks<IO, NK, 1, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
-  else if constexpr (NK == 16 && !BF)
+  else if constexpr (NK > 8 && !BF)
     chunks<IO, NK, 1, 2, 2, OUT><<<blocks, 256, 0, s>>>(a);
   else
     chunks<IO, NK, 1, 4, 2, OUT><<<blocks, 512, 0, s>>>(a);
 }
 
+// K in blocks of 16. In fp32 the matrix instructions are what counts, and there are more sizes than powers of two:
+// none is issued for blocks that do not exist (16 x 6 heads of up to 777 slots, K = 40: 35 us a pass, as K = 64 38).
 template <typename IO, bool OUT>
 inline void launch(const Args& a, unsigned blocks, hipStream_t s) {
-  // 2-byte rows of 16 would be smaller than the 1024 bytes that an instruction brings: 32 at least
-  if (sizeof(IO) == 4 && a.K <= 16)
-    launch_k<IO, sizeof(IO) == 4 ? 1 : 2, OUT>(a, blocks, s);
-  else if (a.K <= 32)
-    launch_k<IO, 2, OUT>(a, blocks, s);
-  else if (a.K <= 64)
-    launch_k<IO, 4, OUT>(a, blocks, s);
-  else if (a.K <= 128)
-    launch_k<IO, 8, OUT>(a, blocks, s);
-  else
-    launch_k<IO, 16, OUT>(a, blocks, s);
+  if constexpr (Type<IO>::BF) {
+    if (a.K <= 32)
+      launch_k<IO, 2, OUT>(a, blocks, s);
+    else if (a.K <= 64)
+      launch_k<IO, 4, OUT>(a, blocks, s);
+    else if (a.K <= 128)
+      launch_k<IO, 8, OUT>(a, blocks, s);
+    else
+      launch_k<IO, 16, OUT>(a, blocks, s);
+  } else {
+    if (a.K <= 16)
+      launch_k<IO, 1, OUT>(a, blocks, s);
+    else if (a.K <= 32)
+      launch_k<IO, 2, OUT>(a, blocks, s);
+    else if (a.K <= 48)
+      launch_k<IO, 3, OUT>(a, blocks, s);
+    else if (a.K <= 64)
+      launch_k<IO, 4, OUT>(a, blocks, s);
+    else if (a.K <= 96)
+      launch_k<IO, 6, OUT>(a, blocks, s);
+    else if (a.K <= 128)
+      launch_k<IO, 8, OUT>(a, blocks, s);
+    else if (a.K <= 192)
+      launch_k<IO, 12, OUT>(a, blocks, s);
+    else
+      launch_k<IO, 16, OUT>(a, blocks, s);
+  }
 }
 
 // one translation unit each

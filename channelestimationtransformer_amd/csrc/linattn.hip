@@ -275,9 +275,10 @@ struct Operand {
 };
 
 // How the time axis is cut: into segments where heads, sequences and slices alone are fewer than two workgroups
-// per CU, none shorter than 128 slots. Forward and backward cut it alike, and share the segments' states. (16 x 6
-// heads of up to 777 slots, fp32: two segments 66 us a pass, three 56, four 70, five 57; three or four workgroups per
-// CU cost the bf16 training pass 20 to 25 %.)
+// per CU, none shorter than 128 slots, as many as make the workgroups' rounds over the chip times the length of a
+// segment least (12 x 16 heads x 2048 slots, bf16, 128 x 128: two segments in one round 190 us with the states
+// between them, three in two rounds 206). Forward and backward cut it alike, and share the segments' states. (Three
+// or four workgroups per CU cost the bf16 training pass of 8 x 16 heads 20 to 25 %.)
 struct Cut {
   int nseg, seg_len;
   size_t states;  // bytes of the states between segments, K x V per head
@@ -292,10 +293,12 @@ Cut cut(const cet_linattn_desc& d) {
   if (by_columns(d)) return Cut{1, std::max(d.T, 1), 0};
   const int cols = slice_columns(d.dtype, d.K, d.V);
   const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
-  long nseg = tasks ? std::min<long>((2L * cu_count() + tasks - 1) / tasks, chunks / 2) : 1;
-  if (tasks >= 2L * cu_count()) nseg = 1;
-  nseg = std::max<long>(nseg, 1);
-  const long per = (std::max<long>(chunks, 1) + nseg - 1) / nseg;
+  const long room = 2L * cu_count();
+  long per = std::max<long>(chunks, 1), best = (tasks + room - 1) / room * per;
+  for (long n = 2; tasks && n <= (room + tasks - 1) / tasks && 2 * n <= chunks; ++n) {
+    const long p = (chunks + n - 1) / n, cost = (tasks * ((chunks + p - 1) / p) + room - 1) / room * p;
+    if (cost < best) per = p, best = cost;
+  }
   Cut c;
   c.seg_len = (int)(per * STATE_SLOTS);
   c.nseg = (int)std::max<long>((chunks + per - 1) / per, 1);
