@@ -295,7 +295,9 @@ Cut cut(const cet_linattn_desc& d) {
   const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
   const long room = 2L * cu_count();
   long per = std::max<long>(chunks, 1), best = (tasks + room - 1) / room * per;
-  for (long n = 2; tasks && n <= (room + tasks - 1) / tasks && 2 * n <= chunks; ++n) {
+  for (const long most : {tasks ? room / tasks : 1, tasks ? (room + tasks - 1) / tasks : 1}) {  // within a round, and one more
+    const long n = std::min(most, chunks / 2);
+    if (n < 2) continue;
     const long p = (chunks + n - 1) / n, cost = (tasks * ((chunks + p - 1) / p) + room - 1) / room * p;
     if (cost < best) per = p, best = cost;
   }
