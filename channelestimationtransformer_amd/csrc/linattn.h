@@ -82,8 +82,15 @@ __device__ inline int row_count(const Args& a, int b) {
 // The arithmetic of a tensor type. float32 and float16 tensors are multiplied in fp32 (a float16
 // state or score would leave that type's range on long histories), bfloat16 ones in bf16.
 
-// Slots of a chunk: 32 with outputs, 64 where only states are formed (fewer barriers; no scores to hold).
+// Slots of a chunk: 32 with outputs, 64 where only states are formed (fewer barriers; no scores to hold). In fp32 half
+// as many or fewer as soon as the rows are long: two workgroups (K up to 128) or three buffers then fit a CU's LDS, and
+// one wave holds all of K (2 x 6 heads of 128 x 128, 4096 slots: 59 us; 32 slots, K in halves by two waves and one
+// workgroup of 64 columns per CU 75; 186 heads of 256 x 256, 702 slots: 560 us, by slices of 32 columns 870).
 constexpr int OUT_SLOTS = 32, STATE_SLOTS = 64;
+constexpr int chunk_slots(bool bf, bool out, int nk, int wc) {
+  if (out) return bf || nk <= 4 ? 32 : 16;
+  return bf ? 64 : nk > 8 ? 16 : nk > 4 || wc == 8 ? 32 : 64;
+}
 
 template <typename IO>
 struct Type {
@@ -219,24 +226,27 @@ __device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
 // column each finishes the outputs of one block of 16 slots, with the other's half of q S for it, which comes
 // through LDS behind the same barrier.
 template <typename IO, int NK, int NV, int WC, int KH, bool OUT>
-__global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) void chunks(const Args a) {
+__global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1 ? 1 : 2) void chunks(const Args a) {
   typedef Type<IO> Ty;
   typedef typename Ty::Quad Quad;
-  constexpr int C = OUT || (WC == 8 && sizeof(IO) == 4) ? OUT_SLOTS : STATE_SLOTS, NB = C / 16;  // two workgroups on a CU
+  constexpr int C = chunk_slots(Ty::BF, OUT, NK, WC), NB = C / 16;
   constexpr int NW = WC * KH, DK = row_width(NK, sizeof(IO)), NKW = NK / KH, SL = 16 * NV * WC;
   constexpr bool SHARE = NW > 1;  // one wave keeps its scores
   constexpr int BLOCKS = NB * (NB + 1) / 2, MINE = KH == 2 ? 1 : NB;
-  static_assert((!OUT || NB == 2) && KH <= 2 && NK % KH == 0, "two blocks of slots in a chunk with outputs");
+  // The scores of a chunk of 16 slots are one block: the waves take its K in parts, and each adds the parts up.
+  constexpr bool SPLIT = OUT && NB == 1;
+  constexpr int SCORES = SPLIT ? (NK < NW ? NK : NW) : BLOCKS;
+  static_assert(KH <= 2 && NK % KH == 0 && (!OUT || NB == 2 || (NB == 1 && KH == 1 && SHARE)), "one or two blocks of slots in a chunk with outputs");
   typedef Tile<IO, DK, C> TK;
   typedef Tile<IO, SL, C> TV;
   // Buffers in a ring: rows of chunk c + BUFS are asked for when everybody has left chunk c.
   constexpr int BUF = (OUT ? 2 : 1) * TK::BYTES + TV::BYTES;
   // Three where that leaves room for two workgroups on a CU, or where two would not either.
-  constexpr int REST = (OUT && SHARE ? 2 * BLOCKS * 64 * (int)sizeof(Quad) : 0) + (OUT && KH == 2 ? 2 * NW * NV * 1024 : 0) + 2048;
+  constexpr int REST = (OUT && SHARE ? 2 * SCORES * 64 * (int)sizeof(Quad) : 0) + (OUT && KH == 2 ? 2 * NW * NV * 1024 : 0);
   constexpr int BUFS = SHARE && (3 * BUF + REST <= 81920 || (2 * BUF + REST > 81920 && 3 * BUF + REST <= 163840)) ? 3 : 2;
   constexpr int PARTS = BUF / 1024, PER = PARTS / NW, EXTRA = PARTS % NW;  // of a chunk; of each wave; of the first waves
   __shared__ __align__(1024) char tiles[BUFS][BUF];
-  __shared__ Quad ps[2][OUT && SHARE ? BLOCKS : 1][64];
+  __shared__ Quad ps[2][OUT && SHARE ? SCORES : 1][64];
   __shared__ f4 xs[2][OUT && KH == 2 ? NW : 1][NV][64];
 
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -331,7 +341,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) v
     wd[r] = i >= s ? pw(g2, i - s) * a.s_intra : 0.f;
     wo[r] = pw(g2, 16 + i - s) * a.s_intra;
   }
-  const float rf[OUT_SLOTS / 16] = {pw(g2, i + e) * a.s_inter, pw(g2, 16 + i + e) * a.s_inter};
+  const float rf[2] = {pw(g2, i + e) * a.s_inter, pw(g2, 16 + i + e) * a.s_inter};
   // A state that fades slowly is kept as S / d^m, m slots since it was last multiplied out: a chunk then adds
   // its keys and values by the weights d^-(m + 1 + j) and touches no element of S otherwise, and the weight of
   // a slot far back is not rounded once per chunk. It is multiplied out when d^m would leave 2^+-20. Where 2^-16
@@ -396,8 +406,15 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) v
     const int flip = (at / C) & 1;
     if (OUT) {
       constexpr int TB[3] = {0, 1, 1}, SB[3] = {0, 0, 1};  // the blocks on and below the diagonal
+      if constexpr (SPLIT) {
+        f4 p = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < BLOCKS; ++x) {
+        for (int u = 0; u < NK; u += NW)
+          if (u + wave < NK) p = mma16(TK::rows(kr, 0, u + wave), TK::rows(qr, 0, u + wave), p);
+        if (wave < SCORES) ps[flip][wave][lane] = p;
+      }
+#pragma unroll
+      for (int x = 0; x < (SPLIT ? 0 : BLOCKS); ++x) {
         if constexpr (SHARE) {
           if (x % NW == wave) ps[flip][x][lane] = scores(qr, kr, TB[x], SB[x]);
         } else {
@@ -434,7 +451,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) v
       }
       if constexpr (KH == 2) {
 #pragma unroll
-        for (int y = 0; y < NV; ++y) xs[flip][wave][y][lane] = kh ? acc[0][y] : acc[1][y];
+        for (int y = 0; y < NV; ++y) xs[flip][wave][y][lane] = kh ? acc[0][y] : acc[NB - 1][y];
       }
     }
 
@@ -522,7 +539,14 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) v
     buf = buf == BUFS - 1 ? 0 : buf + 1;
 
     if (OUT && busy) {
-      if constexpr (SHARE) {
+      if constexpr (SPLIT) {
+        f4 p = ps[flip][0][lane];
+#pragma unroll
+        for (int x = 1; x < SCORES; ++x) p += ps[flip][x][lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = i >= 4 * g + r ? p[r] * wd[r] : 0.f;
+        pf[0] = p;
+      } else if constexpr (SHARE) {
 #pragma unroll
         for (int x = 0; x < BLOCKS; ++x) pf[x] = ps[flip][x][lane];
       }
@@ -533,14 +557,18 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) v
         f4 out[NV];
 #pragma unroll
         for (int y = 0; y < NV; ++y) {
-          out[y] = KH == 2 ? (kh ? acc[1][y] : acc[0][y]) : acc[t][y];
+          out[y] = KH == 2 ? (kh ? acc[NB - 1][y] : acc[0][y]) : acc[t][y];
           if constexpr (KH == 2) out[y] += xs[flip][kh ? wave - WC : wave + WC][y][lane];
           if constexpr (Ty::BF) {
             const bf4 none = bf4{(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
             out[y] = mma32(vf[0][y], tb ? vf[1][y] : none, tb ? pf[1] : pf[0], tb ? pf[2] : none, out[y]);
           } else {
-            out[y] = mma16(vf[0][y], tb ? pf[1] : pf[0], out[y]);
-            if (tb) out[y] = mma16(vf[1][y], pf[2], out[y]);
+            if constexpr (NB == 1) {
+              out[y] = mma16(vf[0][y], pf[0], out[y]);
+            } else {
+              out[y] = mma16(vf[0][y], tb ? pf[1] : pf[0], out[y]);
+              if (tb) out[y] = mma16(vf[1][y], pf[2], out[y]);
+            }
           }
         }
         if (16 * tb + i < n) {
@@ -605,8 +633,14 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 ? 4 : WC * KH == 1 ? 1 : 2) v
 // CU and no segments. fp32, 40 x 72, 16 x 6 heads of up to 777 slots: 35 us, by slices of 64 columns 50.)
 inline int slice_columns(int dtype, int K, int V) {
   if (V <= 16 && K <= 64) return 16;
-  if (K > 128 && dtype != CET_BF16) return 32;
-  return V > 64 && K <= (dtype == CET_BF16 ? 128 : 64) ? 128 : 64;
+  return V > 64 && (dtype != CET_BF16 || K <= 128) ? 128 : 64;
+}
+
+// How many of them a CU holds at once and keeps busy: single waves as many as LDS takes; one where rows of 256 fill
+// it, two otherwise.
+inline int workgroups_per_cu(int dtype, int K, int V) {
+  if (slice_columns(dtype, K, V) == 16) return K > 32 ? 4 : 8;
+  return K > 128 && (dtype == CET_BF16 || V > 64) ? 1 : 2;
 }
 
 template <typename IO, int NK, bool OUT>
@@ -615,14 +649,12 @@ inline void launch_k(const Args& a, unsigned blocks, hipStream_t s) {
   const int cols = slice_columns(BF ? CET_BF16 : CET_F32, a.K, a.V);
   if constexpr (NK <= 4)
     if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(a);
-  if constexpr (NK <= 4 && !BF)
+  if constexpr (!BF)
     if (cols == 128) return chunks<IO, NK, 1, 8, 1, OUT><<<blocks, 512, 0, s>>>(a);
   if constexpr (NK <= 8 && BF)
     if (cols == 128) return chunks<IO, NK, 2, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
-  if constexpr (NK <= 4)
+  if constexpr (NK <= 4 || (!BF && (OUT || NK <= 8)))
     chunks<IO, NK, 1, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
-  else if constexpr (NK > 8 && !BF)
-    chunks<IO, NK, 1, 2, 2, OUT><<<blocks, 256, 0, s>>>(a);
   else
     chunks<IO, NK, 1, 4, 2, OUT><<<blocks, 512, 0, s>>>(a);
 }

@@ -293,7 +293,7 @@ Cut cut(const cet_linattn_desc& d) {
   if (by_columns(d)) return Cut{1, std::max(d.T, 1), 0};
   const int cols = slice_columns(d.dtype, d.K, d.V);
   const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
-  const long room = 2L * cu_count();
+  const long room = (long)cu_count() * workgroups_per_cu(d.dtype, d.K, d.V);
   long per = std::max<long>(chunks, 1), best = (tasks + room - 1) / room * per;
   for (const long most : {tasks ? room / tasks : 1, tasks ? (room + tasks - 1) / tasks : 1}) {  // within a round, and one more
     const long n = std::min(most, chunks / 2);
