@@ -52,6 +52,12 @@ struct Args {
   float s_inter, s_intra, s_kv;
 };
 
+// Passes of one shape in one launch (the gradients).
+struct Passes {
+  Args a[3];
+  int n;
+};
+
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -103,8 +109,11 @@ struct Type {
     else
       return f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
   }
-  __device__ static void store(IO* p, float v) { *p = (IO)v; }
-  __device__ static void store4(IO* p, const f4& v) { *reinterpret_cast<V4*>(p) = V4{(IO)v[0], (IO)v[1], (IO)v[2], (IO)v[3]}; }
+  // said to be global memory: stores through a generic pointer are waited for with the LDS reads
+  __device__ static void store(IO* p, float v) { *(__attribute__((address_space(1))) IO*)p = (IO)v; }
+  __device__ static void store4(IO* p, const f4& v) {
+    *(__attribute__((address_space(1))) V4*)p = V4{(IO)v[0], (IO)v[1], (IO)v[2], (IO)v[3]};
+  }
 };
 
 // acc += A B over 16 values of k in one tile (fp32: four instructions of k = 4)
@@ -173,7 +182,7 @@ struct Tile {
   __device__ static Quad cols(const unsigned (&base)[E == 2 ? 1 : 4], int sb, int x) {
     if constexpr (E == 2) {
       typedef __attribute__((address_space(3))) s4* lds_s4;
-      const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)((base[0] ^ x << SHIFT) + sb * 16 * ROW));
+      const s4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(unsigned long)((base[0] ^ x << SHIFT) + sb * 16 * ROW));
       return Type<IO>::quad(__builtin_bit_cast(V4, r));
     } else {
       f4 v;
@@ -226,7 +235,7 @@ __device__ inline void multiply_out(f4 (&S)[NK][NV], float f) {
 // column each finishes the outputs of one block of 16 slots, with the other's half of q S for it, which comes
 // through LDS behind the same barrier.
 template <typename IO, int NK, int NV, int WC, int KH, bool OUT>
-__global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1 ? 1 : 2) void chunks(const Args a) {
+__global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1 ? 1 : 2) void chunks(const Passes passes) {
   typedef Type<IO> Ty;
   typedef typename Ty::Quad Quad;
   constexpr int C = chunk_slots(Ty::BF, OUT, NK, WC), NB = C / 16;
@@ -251,18 +260,22 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
 
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, kh = wave / WC;
-  // Workgroups go to the 8 XCDs in turn: the slices of a segment, which read the same q and k, are given to one, and
-  // share its L2; the segments of one sequence are spread over all, so that long ones keep no XCD busy alone (32
-  // sequences, the first four full and the others of 64 slots, 16 heads, bf16: 200 us, by runs of workgroups 263).
+  // Workgroups go to the 8 XCDs in turn: the slices and passes of a segment, which read the same rows, are given to
+  // one, and share its L2 (the three gradients of 8 x 16 heads of 128 x 128, bf16: @@ us, one after the other 245);
+  // the segments of a sequence are spread over all, so that long ones keep no XCD busy alone (32 sequences, the
+  // first four full and the others of 64 slots, 16 heads, bf16: 200 us, by runs of workgroups 263).
+  const int inner = passes.n * passes.a[0].nslice;
   unsigned id = blockIdx.x;
   int slice;
-  if (const unsigned eight = 8 * a.nslice, whole = gridDim.x / eight * eight; id < whole) {
-    slice = id / 8 % a.nslice;
+  if (const unsigned eight = 8 * inner, whole = gridDim.x / eight * eight; id < whole) {
+    slice = id / 8 % inner;
     id = id / eight * 8 + id % 8;
   } else {
-    slice = id % a.nslice;
-    id /= a.nslice;
+    slice = id % inner;
+    id /= inner;
   }
+  const Args a = passes.a[slice / passes.a[0].nslice];
+  slice %= passes.a[0].nslice;
   const int nseg_here = OUT ? a.nseg : a.nseg - 1;  // without outputs the last segment has nothing to add
   const int seg = id % nseg_here;
   const long bh = id / nseg_here;
@@ -644,58 +657,62 @@ inline int workgroups_per_cu(int dtype, int K, int V) {
 }
 
 template <typename IO, int NK, bool OUT>
-inline void launch_k(const Args& a, unsigned blocks, hipStream_t s) {
+inline void launch_k(const Passes& p, unsigned blocks, hipStream_t s) {
   constexpr bool BF = Type<IO>::BF;
-  const int cols = slice_columns(BF ? CET_BF16 : CET_F32, a.K, a.V);
+  const int cols = slice_columns(BF ? CET_BF16 : CET_F32, p.a[0].K, p.a[0].V);
   if constexpr (NK <= 4)
-    if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(a);
+    if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(p);
   if constexpr (!BF)
-    if (cols == 128) return chunks<IO, NK, 1, 8, 1, OUT><<<blocks, 512, 0, s>>>(a);
+    if (cols == 128) return chunks<IO, NK, 1, 8, 1, OUT><<<blocks, 512, 0, s>>>(p);
   if constexpr (NK <= 8 && BF)
-    if (cols == 128) return chunks<IO, NK, 2, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
+    if (cols == 128) return chunks<IO, NK, 2, 4, 1, OUT><<<blocks, 256, 0, s>>>(p);
   if constexpr (NK <= 4 || (!BF && (OUT || NK <= 8)))
-    chunks<IO, NK, 1, 4, 1, OUT><<<blocks, 256, 0, s>>>(a);
+    chunks<IO, NK, 1, 4, 1, OUT><<<blocks, 256, 0, s>>>(p);
   else
-    chunks<IO, NK, 1, 4, 2, OUT><<<blocks, 512, 0, s>>>(a);
+    chunks<IO, NK, 1, 4, 2, OUT><<<blocks, 512, 0, s>>>(p);
 }
 
 // K in blocks of 16. In fp32 the matrix instructions are what counts, and there are more sizes than powers of two:
 // none is issued for blocks that do not exist (16 x 6 heads of up to 777 slots, K = 40: 35 us a pass, as K = 64 38).
+inline int k_blocks(int dtype, int K) {
+  const int n = (K + 15) / 16;
+  if (dtype == CET_BF16) return n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
+  return n <= 4 ? n : n <= 6 ? 6 : n <= 8 ? 8 : n <= 12 ? 12 : 16;
+}
+// Passes of one launch have the same kernel and slices.
+inline bool alike(int dtype, const Args& a, const Args& b) {
+  const int cols = slice_columns(dtype, a.K, a.V);
+  return k_blocks(dtype, a.K) == k_blocks(dtype, b.K) && cols == slice_columns(dtype, b.K, b.V) &&
+         (a.V + cols - 1) / cols == (b.V + cols - 1) / cols;
+}
+
 template <typename IO, bool OUT>
-inline void launch(const Args& a, unsigned blocks, hipStream_t s) {
-  if constexpr (Type<IO>::BF) {
-    if (a.K <= 32)
-      launch_k<IO, 2, OUT>(a, blocks, s);
-    else if (a.K <= 64)
-      launch_k<IO, 4, OUT>(a, blocks, s);
-    else if (a.K <= 128)
-      launch_k<IO, 8, OUT>(a, blocks, s);
-    else
-      launch_k<IO, 16, OUT>(a, blocks, s);
-  } else {
-    if (a.K <= 16)
-      launch_k<IO, 1, OUT>(a, blocks, s);
-    else if (a.K <= 32)
-      launch_k<IO, 2, OUT>(a, blocks, s);
-    else if (a.K <= 48)
-      launch_k<IO, 3, OUT>(a, blocks, s);
-    else if (a.K <= 64)
-      launch_k<IO, 4, OUT>(a, blocks, s);
-    else if (a.K <= 96)
-      launch_k<IO, 6, OUT>(a, blocks, s);
-    else if (a.K <= 128)
-      launch_k<IO, 8, OUT>(a, blocks, s);
-    else if (a.K <= 192)
-      launch_k<IO, 12, OUT>(a, blocks, s);
-    else
-      launch_k<IO, 16, OUT>(a, blocks, s);
+inline void launch(const Passes& p, unsigned blocks, hipStream_t s) {
+  constexpr bool BF = Type<IO>::BF;
+  switch (k_blocks(BF ? CET_BF16 : CET_F32, p.a[0].K)) {
+    case 1:
+      if constexpr (!BF) launch_k<IO, 1, OUT>(p, blocks, s);
+      break;
+    case 2: launch_k<IO, 2, OUT>(p, blocks, s); break;
+    case 3:
+      if constexpr (!BF) launch_k<IO, 3, OUT>(p, blocks, s);
+      break;
+    case 4: launch_k<IO, 4, OUT>(p, blocks, s); break;
+    case 6:
+      if constexpr (!BF) launch_k<IO, 6, OUT>(p, blocks, s);
+      break;
+    case 8: launch_k<IO, 8, OUT>(p, blocks, s); break;
+    case 12:
+      if constexpr (!BF) launch_k<IO, 12, OUT>(p, blocks, s);
+      break;
+    default: launch_k<IO, 16, OUT>(p, blocks, s);
   }
 }
 
 // one translation unit each
-void launch_f32(const Args& a, bool out, unsigned blocks, hipStream_t s);
-void launch_f16(const Args& a, bool out, unsigned blocks, hipStream_t s);
-void launch_bf16(const Args& a, bool out, unsigned blocks, hipStream_t s);
+void launch_f32(const Passes& p, bool out, unsigned blocks, hipStream_t s);
+void launch_f16(const Passes& p, bool out, unsigned blocks, hipStream_t s);
+void launch_bf16(const Passes& p, bool out, unsigned blocks, hipStream_t s);
 
 }  // namespace la
 }  // namespace cet

@@ -308,20 +308,20 @@ Cut cut(const cet_linattn_desc& d) {
   return c;
 }
 
-int launch(const Args& a, bool out, unsigned blocks, int dtype, hipStream_t s) {
+// A launch of passes of one shape; `nseg`: segments that have work.
+int launch(Passes& p, bool out, int nseg, int dtype, hipStream_t s) {
+  const Args& a = p.a[0];
+  const int cols = slice_columns(dtype, a.K, a.V);
+  for (int i = 0; i < p.n; ++i) p.a[i].nslice = (a.V + cols - 1) / cols;
+  const unsigned blocks = (unsigned)((long)a.B * a.H * nseg * a.nslice * p.n);
   if (dtype == CET_F32)
-    launch_f32(a, out, blocks, s);
+    launch_f32(p, out, blocks, s);
   else if (dtype == CET_F16)
-    launch_f16(a, out, blocks, s);
+    launch_f16(p, out, blocks, s);
   else
-    launch_bf16(a, out, blocks, s);
+    launch_bf16(p, out, blocks, s);
   CET_HIP(hipGetLastError());
   return CET_OK;
-}
-
-unsigned blocks(const Args& a, int dtype, int nseg) {
-  const int cols = slice_columns(dtype, a.K, a.V);
-  return (unsigned)((long)a.B * a.H * nseg * ((a.V + cols - 1) / cols));
 }
 
 // The states between segments from (k, v) into ws, as K x V.
@@ -329,9 +329,8 @@ int segment_states(Args a, const Cut& c, int dtype, hipStream_t s) {
   if (c.nseg == 1) return CET_OK;
   a.nseg = c.nseg, a.seg_len = c.seg_len;
   a.ws_k = a.V, a.ws_v = 1;
-  const int cols = slice_columns(dtype, a.K, a.V);
-  a.nslice = (a.V + cols - 1) / cols;
-  if (const int rc = launch(a, false, blocks(a, dtype, c.nseg - 1), dtype, s)) return rc;
+  Passes p{{a}, 1};
+  if (const int rc = launch(p, false, c.nseg - 1, dtype, s)) return rc;
   const unsigned heads = (unsigned)((long)a.B * a.H), states = (unsigned)(a.K * a.V);
   if (states % 4 == 0 && (reinterpret_cast<uintptr_t>(a.init) & 15) == 0)
     join_segments<4><<<dim3((states / 4 + 255) / 256, heads), 256, 0, s>>>(a);
@@ -353,33 +352,47 @@ void launch_columns(const Args& a, hipStream_t s) {
     columns<IO, 16><<<blocks, 256, 0, s>>>(a, step(a.q, a.sq), step(a.k, a.sk));
 }
 
-// One pass of the recurrence, segments from their states in ws (transposed: of the operands' roles exchanged).
-int pass(Args a, const Cut& c, bool columns, bool transposed, int dtype, hipStream_t s) {
-  a.nseg = c.nseg, a.seg_len = c.seg_len;
-  a.ws_k = a.init_k = transposed ? 1 : a.V;
-  a.ws_v = a.init_v = transposed ? a.K : 1;
-  if (columns) {
-    if (dtype == CET_F32)
-      launch_columns<float>(a, s);
-    else if (dtype == CET_F16)
-      launch_columns<_Float16>(a, s);
-    else
-      launch_columns<__bf16>(a, s);
-    CET_HIP(hipGetLastError());
-    return CET_OK;
+// Passes of the recurrence, segments from their states in ws (`transposed`: of the operands' roles exchanged). Those of
+// one shape share a launch.
+double threads(const Args& a, int nseg) { return (double)a.B * a.H * nseg * ((a.V + 63) / 64) * 512; }  // at most
+struct Run {
+  Args a;
+  bool transposed;
+};
+int run(Run* r, int n, const Cut& c, bool columns, int dtype, hipStream_t s) {
+  Passes p{};
+  for (int i = 0; i < n; ++i) {
+    Args& a = r[i].a;
+    a.nseg = c.nseg, a.seg_len = c.seg_len;
+    a.ws_k = a.init_k = r[i].transposed ? 1 : a.V;
+    a.ws_v = a.init_v = r[i].transposed ? a.K : 1;
+    a.vec_o = a.V % 4 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
+    if (columns) {
+      if (dtype == CET_F32)
+        launch_columns<float>(a, s);
+      else if (dtype == CET_F16)
+        launch_columns<_Float16>(a, s);
+      else
+        launch_columns<__bf16>(a, s);
+      CET_HIP(hipGetLastError());
+      continue;
+    }
+    p.a[p.n++] = a;
+    if (i + 1 < n && alike(dtype, a, r[i + 1].a) && threads(a, c.nseg) * (p.n + 1) < 4294967296.) continue;
+    if (const int rc = launch(p, true, c.nseg, dtype, s)) return rc;
+    p.n = 0;
   }
-  const int cols = slice_columns(dtype, a.K, a.V);
-  a.nslice = (a.V + cols - 1) / cols;
-  a.vec_o = a.V % 4 == 0 && (reinterpret_cast<uintptr_t>(a.o) & 15) == 0;
-  return launch(a, true, blocks(a, dtype, c.nseg), dtype, s);
+  return CET_OK;
 }
 
 bool bad_desc(const cet_linattn_desc* d) {
   return !d || d->dtype < CET_F32 || d->dtype > CET_F16 || d->B < 0 || d->T < 0 || d->H < 0 || d->K < 1 || d->V < 1 ||
          d->T > (1 << 30) || !std::isfinite(d->scale);
 }
-// (a launch holds fewer than 2^32 threads: 256 for each head of each sequence and slice)
-bool too_large(const cet_linattn_desc& d) { return d.K > 256 || d.V > 256 || (double)d.B * d.H > (1 << 22); }
+// (a launch holds fewer than 2^32 threads: at most 512 for each head of each sequence and 64 columns)
+bool too_large(const cet_linattn_desc& d) {
+  return d.K > 256 || d.V > 256 || (double)d.B * d.H * ((std::max(d.K, d.V) + 63) / 64) > (1 << 22);
+}
 Strides contiguous(const cet_linattn_desc& d, int D) { return Strides{(long)d.T * d.H * D, (long)d.H * D, D}; }
 
 template <typename IO, int W>
@@ -461,7 +474,8 @@ int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k
   a.B = d->B, a.T = d->T, a.H = d->H, a.K = d->K, a.V = d->V;
   a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
   if (const int rc = segment_states(a, c, d->dtype, s)) return rc;
-  return pass(a, c, columns, false, d->dtype, s);
+  Run r{a, false};
+  return run(&r, 1, c, columns, d->dtype, s);
 }
 
 int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
@@ -497,12 +511,13 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
     a.K = d->K, a.V = d->V, a.s_kv = 1.f;
     if (const int rc = segment_states(a, c, d->dtype, s)) return rc;
   }
+  Run r[3];
   // dq: (do, v, k) forward in time, states transposed
   a.q = og.p, a.sq = og.s, a.k = ov.p, a.sk = ov.s, a.v = ok.p, a.sv = ok.s;
   a.o = dq;
   a.K = d->V, a.V = d->K;
   a.s_inter = a.s_intra = d->scale, a.s_kv = 1.f;
-  if (const int rc = pass(a, c, columns, true, d->dtype, s)) return rc;
+  r[0] = Run{a, true};
   // the gradients of the states, backward in time, which the two other passes share
   a.ws = back;
   a.init = d_final;
@@ -514,13 +529,14 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   a.q = ov.p, a.sq = ov.s, a.k = og.p, a.sk = og.s, a.v = oq.p, a.sv = oq.s;
   a.o = dk;
   a.K = d->V, a.V = d->K;
-  if (const int rc = pass(a, c, columns, true, d->dtype, s)) return rc;
+  r[1] = Run{a, true};
   // dv: (k, q, do) backward in time; the carry at the end is the gradient of the first state
   a.q = ok.p, a.sq = ok.s, a.k = oq.p, a.sk = oq.s, a.v = og.p, a.sv = og.s;
   a.o = dv, a.so = contiguous(*d, d->V);
   a.K = d->K, a.V = d->V;
   a.fin = d_initial;
-  return pass(a, c, columns, false, d->dtype, s);
+  r[2] = Run{a, false};
+  return run(r, 3, c, columns, d->dtype, s);
 }
 
 int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64_t* q_strides, const int64_t* k_strides,

@@ -4,11 +4,11 @@
 namespace cet {
 namespace la {
 
-void launch_bf16(const Args& a, bool out, unsigned blocks, hipStream_t s) {
+void launch_bf16(const Passes& p, bool out, unsigned blocks, hipStream_t s) {
   if (out)
-    launch<__bf16, true>(a, blocks, s);
+    launch<__bf16, true>(p, blocks, s);
   else
-    launch<__bf16, false>(a, blocks, s);
+    launch<__bf16, false>(p, blocks, s);
 }
 
 }  // namespace la

@@ -4,11 +4,11 @@
 namespace cet {
 namespace la {
 
-void launch_f16(const Args& a, bool out, unsigned blocks, hipStream_t s) {
+void launch_f16(const Passes& p, bool out, unsigned blocks, hipStream_t s) {
   if (out)
-    launch<_Float16, true>(a, blocks, s);
+    launch<_Float16, true>(p, blocks, s);
   else
-    launch<_Float16, false>(a, blocks, s);
+    launch<_Float16, false>(p, blocks, s);
 }
 
 }  // namespace la

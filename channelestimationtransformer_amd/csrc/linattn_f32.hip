@@ -4,11 +4,11 @@
 namespace cet {
 namespace la {
 
-void launch_f32(const Args& a, bool out, unsigned blocks, hipStream_t s) {
+void launch_f32(const Passes& p, bool out, unsigned blocks, hipStream_t s) {
   if (out)
-    launch<float, true>(a, blocks, s);
+    launch<float, true>(p, blocks, s);
   else
-    launch<float, false>(a, blocks, s);
+    launch<float, false>(p, blocks, s);
 }
 
 }  // namespace la
