@@ -213,8 +213,8 @@ __device__ inline void act1(float g, float& a, float& slope) {
     a = g * p;
     slope = fmaf(g * 0.39894228040143267794f, e, p);
   } else {
-    a = fmaxf(g, 0.f);
-    slope = g > 0.f ? 1.f : 0.f;
+    a = g <= 0.f ? 0.f : g;  // (a NaN stays one)
+    slope = g <= 0.f ? 0.f : 1.f;
   }
 }
 __device__ inline void act4(int kind, const f4& g, f4& a, f4& slope) {
@@ -317,7 +317,7 @@ struct Half {
 };
 
 template <typename T, int BP, int BQ, int WP, int WQ, bool PC, bool QC, int KIND>
-__global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const Args a) {
+__global__ __launch_bounds__(64 * WP * WQ, 2) void product(const Args a) {
   constexpr int NT = 64 * WP * WQ, NPT = BP / WP / 16, NQT = BQ / WQ / 16;
   constexpr bool GATED = KIND == FORWARD || KIND == BACKWARD;
   typedef Tile<T, BP, NT, PC> TP;
@@ -366,8 +366,8 @@ __global__ __launch_bounds__(64 * WP * WQ, BP == 256 ? 2 : 2) void product(const
   // A tile is worked on in four steps: half of its 128 bytes of k and half of the wave's tiles of P each. The
   // operands of a step travel from LDS into one set of registers while the matrix instructions work on the other,
   // across the barrier too: before the last step of a tile the next tile has landed, this one is all in registers,
-  // and its buffer takes the rows of the tile after, P's at once and Q's behind the next step (3 % over both at once). (Whole steps of k need 32 registers more and spilled where
-  // operands are read by columns.)
+  // and its buffer takes the rows of the tile after, P's at once and Q's behind the next step (3 % over both at
+  // once). (Whole steps of k need 32 registers more and spilled where operands are read by columns.)
   constexpr int HP = NPT / 2;
   Frag p0_[HP], p1_[HP], q0_[NQT], q1_[NQT];
   auto load_p = [&](Frag (&fp)[HP], int buf, int kk, int half) {

@@ -97,7 +97,6 @@ __global__ __launch_bounds__(512) void few_rows(const Args a) {
   for (int y = 0; y < NQT; ++y) ag[y] = au[y] = f4{0.f, 0.f, 0.f, 0.f};
   const Frag none = {0, 0, 0, 0};
   const int steps = (a.nk + STEP - 1) / STEP;
-#pragma unroll 4
   for (int s = wave; s < steps; s += 8) {
     const int k = s * STEP + g * VEC;
     const bool live = k < a.nk;  // whole pieces: rows are padded to them

@@ -10,6 +10,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 
@@ -740,6 +741,8 @@ def direct(*tensors):
     """Whether a call may pass the dispatcher by: eager, and on plain tensors only (none of a tracer's)."""
     if torch.compiler.is_compiling():
         return False
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("forward-mode differentiation is not supported")  # the tangents would be dropped in silence
     for t in tensors:
         if type(t) not in _PLAIN:
             return False

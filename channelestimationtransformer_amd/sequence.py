@@ -8,8 +8,9 @@ leaves a state of fixed size per head, `linear_attention_step` carries that stat
 
 All take CUDA (ROCm) tensors of one type (float32, bfloat16 or float16), run on the current stream
 and raise on anything the kernels do not serve. `rotary`, `linear_attention` and
-`gated_linear` have gradients (`rotary`'s can be differentiated again; the transforms of torch.func are
-refused).
+`gated_linear` have gradients (`rotary`'s can be differentiated again; the transforms of torch.func and
+forward-mode differentiation are refused). All can be captured into graphs; a training step is captured whole, with
+no eager graph of the same leaves alive, as torch asks.
 """
 import math
 
@@ -29,7 +30,9 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     everywhere if None, values outside [0, T] taken as the nearer end): slots at and behind a sequence's
     length are not read, their o and their gradients are zero, and the state stops before them. The
     decay is a constant: it has no gradient and is refused if it wants one. Any strides with a
-    contiguous last axis are read in place where rows start on 16 bytes, copied once otherwise."""
+    contiguous last axis are read in place where rows start on 16 bytes, copied once otherwise. Slots are
+    taken in chunks of up to 32: an infinity or NaN in a slot within its sequence's length can reach the
+    outputs of the slots of its chunk before it, too."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0
     if log_decay.requires_grad and torch.is_grad_enabled():

@@ -196,3 +196,14 @@ def test_graphs_and_streams():
             torch.cuda.synchronize()
             for j, out in enumerate(outs):
                 assert all(torch.equal(a, b) for a, b in zip(out, want[(turn + j) % 2]))
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("N, D, F", [(9, 40, 24), (40, 100, 130), (300, 136, 150)])
+def test_nan_is_not_swallowed(N, D, F, kind):
+    """A NaN in a weight of the gate reaches its column of the result, whatever the activation, and no other."""
+    x, wg, wu, _, _, _ = make(N, D, F, torch.float32, False, seed=8)
+    wg[3, 5] = float("nan")
+    out = cet.gated_linear(x, wg, wu, activation=kind)
+    assert torch.isnan(out[:, 3]).all()
+    assert torch.isfinite(out[:, [c for c in range(F) if c != 3]]).all()

@@ -84,6 +84,22 @@ def test_forward_and_gradients(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [12, 50, 130])
+@pytest.mark.parametrize("K", [10, 24, 40, 56, 72, 100, 160, 200])
+def test_every_number_of_blocks(K, V, dtype):
+    """Each number of blocks of K that a kernel is built for with each width of its slices, in segments, to ragged
+    lengths; the gradients are the same with K and V exchanged."""
+    check(make(2, 270, 1, K, V, dtype, seed=K + V, ragged=True), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K, V", [(100, 128), (40, 33), (256, 200), (130, 70)])
+def test_gradients_that_share_a_launch(K, V, dtype):
+    """Heads whose K and V differ but are served by one kernel, and some where only two of the gradients are."""
+    check(make(2, 150, 2, K, V, dtype, seed=K, ragged=True), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(2, 700, 1, 32, 16), (1, 1500, 2, 64, 64), (1, 1031, 1, 128, 128), (1, 900, 1, 16, 16)])
 def test_time_axis_in_segments(shape, dtype):
     """Few sequences and heads: the time axis is cut and the pieces' states are joined."""

@@ -178,3 +178,14 @@ def test_function_transforms_are_refused():
                  lambda t: cet.rotary(t, None, torch.arange(5, device="cuda"), cet.rotary_frequencies(8)[0])[0].sum()):
         with pytest.raises(RuntimeError):
             torch.func.grad(call)(q)
+
+
+def test_forward_mode_differentiation_is_refused():
+    """Not silently without tangents."""
+    q, dec = torch.randn(2, 5, 3, 8).cuda(), ref.geometric(3).cuda()
+    with torch.autograd.forward_ad.dual_level():
+        t = torch.autograd.forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: cet.linear_attention(t, q, q, dec), lambda: cet.gated_linear(t[0, 0], q[0, 1], q[0, 2]),
+                     lambda: cet.rotary(t, None, torch.arange(5, device="cuda"), cet.rotary_frequencies(8)[0])):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
