@@ -308,7 +308,8 @@ int cet_qpsk_bit_errors(const float* x_hat, const float* x_true, double* out, lo
 enum { CET_F32 = 0, CET_BF16 = 1, CET_F16 = 2 };
 
 /* Sizes and layouts of linear attention over B sequences of at most T slots, H heads, K features of
- * queries and keys and V of values per head (1 <= K, V <= 256). Strides: {sequence, slot, head}. */
+ * queries and keys and V of values per head (1 <= K, V <= 256, B H ceil(max(K, V) / 64) <= 2^22, else
+ * CET_ERR_UNSUPPORTED). Strides: {sequence, slot, head}. */
 typedef struct cet_linattn_desc {
   int32_t dtype, B, T, H, K, V;
   int32_t lengths64; /* `lengths` holds int64, not int32 */
@@ -350,7 +351,7 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
 
 /* One slot of B streams: q, k [B,H,K], v [B,H,V] (strides {stream, head} in elements), o [B,H,V]
  * contiguous. state_in, state_out: device float32 [rows,H,K,V], the same array (updated in place) or
- * disjoint ones. slots == NULL: stream b owns row b (rows >= B). With slots (device [B] int32, or int64
+ * disjoint ones; B H <= 2^21. slots == NULL: stream b owns row b (rows >= B). With slots (device [B] int32, or int64
  * where slots64) the arrays are the same and stream b owns row slots[b]; a negative slot is an idle
  * stream (its o is zero), and a slot beyond the array or one that an earlier stream of the call already
  * has gives an o of NaN and leaves the state alone. */
@@ -383,7 +384,7 @@ int cet_rotary(const cet_rotary_desc* d, const void* q, const void* k, const voi
  * out [N,F] contiguous. Products and the activation are formed in fp32, out is rounded once. */
 typedef struct cet_gated_desc {
   int32_t dtype;
-  int32_t activation; /* 0 silu, 1 gelu (exact erf form), 2 relu */
+  int32_t activation; /* 0 silu, 1 gelu (erf form, to 1e-7), 2 relu */
   int32_t N, D, F;
   int64_t ld_x, ld_gate, ld_up;
   int64_t ld_dy; /* backward only */
@@ -398,7 +399,7 @@ int cet_gated_linear(const cet_gated_desc* d, const void* x, const void* w_gate,
 
 /* Gradients from dy [N,F] (rows at ld_dy); the projections are formed again. dx [N,D], dw_* [F,D], db_* [F],
  * contiguous; dx, both dw or both db may be NULL (not wanted). The gradients of the projections are rounded to
- * the tensors' type once before the products that dx and dw are; db is summed from them in fp32. */
+ * the tensors' type once before the products that dx and dw are; db is summed in fp32 before that. */
 int cet_gated_linear_backward(const cet_gated_desc* d, const void* x, const void* w_gate, const void* w_up,
                               const void* b_gate, const void* b_up, const void* dy, void* dx, void* dw_gate,
                               void* dw_up, void* db_gate, void* db_up, void* workspace, size_t workspace_bytes,
