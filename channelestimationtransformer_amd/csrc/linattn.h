@@ -261,9 +261,9 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, kh = wave / WC;
   // Workgroups go to the 8 XCDs in turn: the slices and passes of a segment, which read the same rows, are given to
-  // one, and share its L2 (the three gradients of 8 x 16 heads of 128 x 128, bf16: @@ us, one after the other 245);
-  // the segments of a sequence are spread over all, so that long ones keep no XCD busy alone (32 sequences, the
-  // first four full and the others of 64 slots, 16 heads, bf16: 200 us, by runs of workgroups 263).
+  // one, and share its L2 (the three gradients of 8 x 16 heads of 128 x 128, 2048 slots, bf16: 234 us, one after the
+  // other 251); the segments of a sequence are spread over all, so that long ones keep no XCD busy alone (32
+  // sequences, the first four full and the others of 64 slots, 16 heads, bf16: 200 us, by runs of workgroups 263).
   const int inner = passes.n * passes.a[0].nslice;
   unsigned id = blockIdx.x;
   int slice;

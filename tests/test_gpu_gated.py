@@ -207,3 +207,11 @@ def test_nan_is_not_swallowed(N, D, F, kind):
     out = cet.gated_linear(x, wg, wu, activation=kind)
     assert torch.isnan(out[:, 3]).all()
     assert torch.isfinite(out[:, [c for c in range(F) if c != 3]]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("F", [129, 255, 257, 263, 1299])
+def test_rows_of_an_odd_number_of_features(F, dtype):
+    """Rows that start between two words, over one tile and several, with whole and broken last pieces."""
+    check(make(300, 72, F, dtype, True, seed=F), "silu", dtype)
+    check(make(4100, 40, F, dtype, False, seed=F), "relu", dtype)
