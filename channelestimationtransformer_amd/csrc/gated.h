@@ -115,7 +115,7 @@ struct Tile {
   static constexpr int PER_ROW = COLS ? ROWS / VEC : 8, TOTAL = ROWS * 8, N = TOTAL / NT, BYTES = ROWS * 128;
   static_assert(TOTAL % NT == 0, "whole pieces per thread");
 
-  __device__ static int turn(int k) { return E == 2 ? 2 * ((k & 3) | (k >> 3 & 1) << 2) : 4 * (k >> 2 & 3); }
+  __device__ static int turn(int k) { return (E == 2 ? 2 * ((k & 3) | (k >> 3 & 1) << 2) : 4 * (k >> 2 & 3)) & (PER_ROW - 1); }
 
   // Rows: the addresses of this thread's pieces are carried along, 128 bytes a tile; all of them are the same piece
   // kc of their rows (NT / 8 rows apart, a multiple of the permutation's period).
@@ -173,7 +173,7 @@ struct Tile {
       // k = 32 kk + 8 g + 4 half + i / 4, whose turn is that of the lane alone; pieces of 16 indices: 2 X, 2 X + 1
       typedef __attribute__((address_space(3))) s4* lds_s4;
       typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-      const int th = (i >> 2) | (g & 1) << 2;
+      const int th = ((i >> 2) | (g & 1) << 2) & (PER_ROW / 2 - 1);
       const char* p = t + (8 * g + (i >> 2)) * (ROWS * E) + (i & 1) * 8 + ((r0 / 16 ^ th) << 5) + ((i >> 1 & 1) << 4) + kk * 32 * ROWS * E;
       const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
       const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 4 * ROWS * E)));
@@ -553,9 +553,9 @@ __global__ __launch_bounds__(64 * WP * WQ, 2) void product(const Args a) {
   }
 }
 
-int run_f32(const Args& a, int kind, bool large, hipStream_t s);
-int run_bf16(const Args& a, int kind, bool large, hipStream_t s);
-int run_f16(const Args& a, int kind, bool large, hipStream_t s);
+int run_f32(const Args& a, int kind, int tile, hipStream_t s);
+int run_bf16(const Args& a, int kind, int tile, hipStream_t s);
+int run_f16(const Args& a, int kind, int tile, hipStream_t s);
 
 // Which product: KIND and the operands' layouts go together.
 enum { STEP_FORWARD, STEP_DH, STEP_DX, STEP_DW, STEP_DW_PARTIAL, STEP_DX_PARTIAL };
@@ -581,8 +581,8 @@ inline int run2(const Args& a, int step, hipStream_t s) {
   }
 }
 template <typename T>
-inline int run(const Args& a, int step, bool large, hipStream_t s) {
-  return large ? run2<T, 256, 256, 2, 4>(a, step, s) : run2<T, 128, 128, 2, 2>(a, step, s);
+inline int run(const Args& a, int step, int tile, hipStream_t s) {
+  return tile == 256 ? run2<T, 256, 256, 2, 4>(a, step, s) : tile == 128 ? run2<T, 128, 128, 2, 2>(a, step, s) : run2<T, 64, 64, 2, 2>(a, step, s);
 }
 
 }  // namespace gated

@@ -149,33 +149,42 @@ int cu_count() {
   return n;
 }
 
-// Tiles of 256 x 256 (one workgroup per CU) or 128 x 128 (two), and for sums that may be split, in how many
-// pieces: the cheapest by whole rounds of workgroups, the small tile at 3/4 of the large one's rate, the
-// splits' partial products written and read at 8 TB/s, as they stay in the caches between. (dx of 8192 x 1024 from
-// 2 x 2730 columns, bf16: large tiles in two pieces 98 + 13 us, small ones whole 120 us.)
+// Tiles of 256 x 256 (one workgroup per CU), 128 x 128 (two) or 64 x 64 (four), and for sums that may be split, in how
+// many pieces: the least estimate, from times measured per tile and 128 bytes of k, of a workgroup alone on its CU
+// (its latency) and of one among several (its share of the CU), and per tile's results; 1.3 times as much where operands
+// are read by columns, half of the results' time where they are stored as they are; the splits' partial products
+// written and read at 8 TB/s, as they stay in the caches between. Forward times in us by 256, 128 and 64: bf16 500 rows,
+// 2048 to 759: 55, 30, 21; 1073 rows, 1024 to 2177: 35, 24, 27; 8192 rows, 1024 to 2730: 115, 133, 179; fp32 1262 rows,
+// 2048 to 1925: 490, 278, 213; 20,000 rows, 500 to 1001: 414, 391, 423.
 struct Cut {
-  bool large;
+  int tile;
   int splits, k_per_split;
   size_t ws;
 };
+struct TileTimes {
+  long b;
+  double alone, shared, results;  // us
+};
+constexpr TileTimes TIMES[2][3] = {{{256, 1.55, 1.55, 10}, {128, 0.85, 0.58, 2.6}, {64, 0.58, 0.23, 1.1}},
+                                   {{256, 7.5, 7.5, 20}, {128, 2.1, 2.1, 4}, {64, 0.65, 0.65, 1}}};  // fp32
+
 Cut cut(int dtype, long np, long nq, long nk, bool gated, bool may_split, int cus) {
-  const double rate = (dtype == CET_F32 ? 120e12 : 1000e12) / cus;
   const int bk = 128 / elem_bytes(dtype);
-  Cut best{false, 1, 0, 0};
+  Cut best{128, 1, 0, 0};
   double cost = 1e30;
-  for (int large = 0; large < 2; ++large) {
-    const long b = large ? 256 : 128, bp = gated ? b / 2 : b;
-    const long tiles = ((np + bp - 1) / bp) * ((nq + b - 1) / b), slots = large ? cus : 2L * cus;
+  for (const TileTimes& x : TIMES[dtype == CET_F32]) {
+    const long bp = gated ? x.b / 2 : x.b, tiles = ((np + bp - 1) / bp) * ((nq + x.b - 1) / x.b), slots = cus * (256 / x.b);
     for (int s = 1; s <= (may_split ? 512 : 1); s += s < 32 ? 1 : s / 8) {
       const long per = std::max<long>(((nk + s - 1) / s + bk - 1) / bk * bk, bk);
       const long used = std::max<long>((nk + per - 1) / per, 1);
       if (used != s) continue;
-      const double rounds = (double)((tiles * s + slots - 1) / slots);
-      double t = rounds * 2.0 * b * b * per / (large ? rate : 0.75 * rate / 2) + 3e-6;
-      if (s > 1) t += 8.0 * s * np * nq / 8e12 + 4e-6;
+      const double rounds = (double)((tiles * s + slots - 1) / slots), share = (double)((tiles * s + cus - 1) / cus);
+      const double steps = (double)(per / bk) * (gated ? 1 : 1.3);
+      double t = std::max(rounds * steps * x.alone, share * steps * x.shared) + share * x.results * (gated ? 1 : 0.5);
+      if (s > 1) t += 8.0 * s * np * nq / 8e6 + 4;
       if (t < cost) {
         cost = t;
-        best = Cut{large != 0, s, (int)per, s > 1 ? align_up((size_t)s * np * nq * sizeof(float)) : 0};
+        best = Cut{(int)x.b, s, (int)per, s > 1 ? align_up((size_t)s * np * nq * sizeof(float)) : 0};
       }
     }
   }
@@ -183,7 +192,7 @@ Cut cut(int dtype, long np, long nq, long nk, bool gated, bool may_split, int cu
 }
 
 void set_tiles(Args& a, const Cut& c, bool gated) {
-  const int b = c.large ? 256 : 128, bp = gated ? b / 2 : b;
+  const int b = c.tile, bp = gated ? b / 2 : b;
   a.tiles_p = (a.np + bp - 1) / bp;
   a.tiles_q = (a.nq + b - 1) / b;
   a.splits = c.splits;
@@ -191,8 +200,8 @@ void set_tiles(Args& a, const Cut& c, bool gated) {
   if (gated) a.P.split = b / 2;
 }
 
-int run(int dtype, const Args& a, int step, bool large, hipStream_t s) {
-  return dtype == CET_F32 ? run_f32(a, step, large, s) : dtype == CET_F16 ? run_f16(a, step, large, s) : run_bf16(a, step, large, s);
+int run(int dtype, const Args& a, int step, int tile, hipStream_t s) {
+  return dtype == CET_F32 ? run_f32(a, step, tile, s) : dtype == CET_F16 ? run_f16(a, step, tile, s) : run_bf16(a, step, tile, s);
 }
 
 // A row-major matrix that the products read: in place where its rows are whole 16-byte pieces, else copied.
@@ -258,8 +267,8 @@ struct Plan {
       dx = cut(d.dtype, d.D, d.N, 2L * Fp, false, true, cus);
       dw = cut(d.dtype, d.D, 2L * Fp, d.N, false, true, cus);
       dh = align_up((size_t)d.N * 2 * Fp * elem_bytes(d.dtype));
-      // one row of column sums per tile and wave along the rows (4 waves in the large tile, 2 in the small)
-      block_rows = forward.large ? (d.N + 255L) / 256 * 4 : (d.N + 127L) / 128 * 2;
+      // one row of column sums per tile and wave along the rows (4 waves in the largest tile, 2 in the others)
+      block_rows = ((long)d.N + forward.tile - 1) / forward.tile * (forward.tile == 256 ? 4 : 2);
       blocks = align_up((size_t)block_rows * 2 * Fp * sizeof(float));
       splits = std::max(dx.ws, dw.ws);
     }
@@ -280,11 +289,11 @@ void launch_sum_splits(const Args& a, hipStream_t s) {
 // A product of `dh` with another operand, split over the summed axis where the plan says so.
 int product_of_dh(int dtype, Args a, const Cut& c, int step, int step_partial, float* splits, hipStream_t s) {
   set_tiles(a, c, false);
-  if (c.splits == 1) return run(dtype, a, step, c.large, s);
+  if (c.splits == 1) return run(dtype, a, step, c.tile, s);
   a.part = splits;
   Args b = a;
   b.ld_out = a.np;
-  if (const int rc = run(dtype, b, step_partial, c.large, s)) return rc;
+  if (const int rc = run(dtype, b, step_partial, c.tile, s)) return rc;
   if (dtype == CET_F32)
     launch_sum_splits<float>(a, s);
   else if (dtype == CET_F16)
@@ -348,7 +357,7 @@ int cet_gated_linear(const cet_gated_desc* d, const void* x, const void* w_gate,
     return CET_OK;
   }
   set_tiles(a, p.forward, true);
-  return run(d->dtype, a, STEP_FORWARD, p.forward.large, s);
+  return run(d->dtype, a, STEP_FORWARD, p.forward.tile, s);
 }
 
 int cet_gated_linear_backward(const cet_gated_desc* d, const void* x, const void* w_gate, const void* w_up,
@@ -380,7 +389,7 @@ int cet_gated_linear_backward(const cet_gated_desc* d, const void* x, const void
     a.out = dh, a.ld_out = 2L * p.Fp;
     a.part = db_gate ? blocks : nullptr;
     set_tiles(a, p.forward, true);
-    if (const int rc = run(d->dtype, a, STEP_DH, p.forward.large, s)) return rc;
+    if (const int rc = run(d->dtype, a, STEP_DH, p.forward.tile, s)) return rc;
   }
   if (db_gate) {
     if (d->dtype == CET_F32)

@@ -4,7 +4,7 @@
 namespace cet {
 namespace gated {
 
-int run_bf16(const Args& a, int step, bool large, hipStream_t s) { return run<__bf16>(a, step, large, s); }
+int run_bf16(const Args& a, int step, int tile, hipStream_t s) { return run<__bf16>(a, step, tile, s); }
 
 }  // namespace gated
 }  // namespace cet

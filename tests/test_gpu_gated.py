@@ -215,3 +215,10 @@ def test_rows_of_an_odd_number_of_features(F, dtype):
     """Rows that start between two words, over one tile and several, with whole and broken last pieces."""
     check(make(300, 72, F, dtype, True, seed=F), "silu", dtype)
     check(make(4100, 40, F, dtype, False, seed=F), "relu", dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N, D, F", [(90, 130, 70), (1073, 264, 2177), (600, 2056, 300), (3000, 128, 66)])
+def test_tiles_of_every_size(N, D, F, dtype):
+    """Few tiles (the smallest), several rounds of them, long sums in pieces."""
+    check(make(N, D, F, dtype, True, seed=N), "gelu", dtype)
