@@ -173,3 +173,11 @@ def test_graph_replays():
         want = cet.rotary(q + turn, k, pos + 1000 * turn, freq)
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shape", [(3, 50, 4, 2, 48, 12), (2, 31, 6, 1, 80, 40), (2, 17, 2, 2, 20, 4), (1, 40, 3, 1, 36, 36), (2, 9, 2, 2, 96, 24)])
+def test_pieces_of_every_width(shape, layout, dtype):
+    """Turned parts whose halves are whole numbers of 8, 4 and 2 values only."""
+    test_against_the_definition(shape, layout, dtype)
