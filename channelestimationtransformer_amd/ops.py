@@ -34,7 +34,8 @@ def _f32(name, t, *shape):
     the kernels index raw pointers, so a wrong dtype or a short buffer would read out of bounds."""
     if t.dtype != torch.float32:
         raise RuntimeError(f"{name} must be float32, got {t.dtype}")
-    if t.dim() != len(shape) or any(s is not None and int(d) != int(s) for d, s in zip(t.shape, shape)):
+    if t.shape != shape and (  # (the comparison alone where every size is given)
+            t.dim() != len(shape) or any(s is not None and int(d) != int(s) for d, s in zip(t.shape, shape))):
         raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t  # a slice may start anywhere; the C ABI wants 16 B
@@ -297,11 +298,16 @@ def _seq_check(name, t, dtype, *shape):
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be {dtype}, got {t.dtype}")
     have = t.shape
-    if len(have) != len(shape):
+    if have != shape and (len(have) != len(shape) or any(s is not None and s != d for s, d in zip(shape, have))):
         raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(have)}")
-    for s, d in zip(shape, have):
-        if s is not None and s != d:
-            raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(have)}")
+    return t if have[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _seq_first(name, t, dim):
+    """The tensor that gives a call its type and sizes."""
+    have = t.shape
+    if len(have) != dim:
+        raise RuntimeError(f"{name} must have shape {[None] * dim}, got {list(have)}")
     return t if have[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
@@ -322,7 +328,7 @@ def _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o=None):
     """Checked operands of the linear attention calls and their descriptor."""
     dev = _dev_check(*(t for t in (q, k, v, log_decay, initial_state, lengths, d_o) if t is not None))
     code = _seq_type(q)
-    q = _seq_check("q", q, q.dtype, None, None, None, None)
+    q = _seq_first("q", q, 4)
     B, T, H, K = q.shape
     k = _seq_check("k", k, q.dtype, B, T, H, K)
     v = _seq_check("v", v, q.dtype, B, T, H, None)
@@ -477,9 +483,9 @@ class LinearAttention(torch.autograd.Function):
 
 
 def _step(q, k, v, log_decay, state, out_state, scale, slots):
-    dev = _dev_check(*(t for t in (q, k, v, log_decay, state, slots) if t is not None))
+    dev = _dev_check(q, k, v, log_decay, state) if slots is None else _dev_check(q, k, v, log_decay, state, slots)
     code = _seq_type(q)
-    q = _seq_check("q", q, q.dtype, None, None, None)
+    q = _seq_first("q", q, 3)
     B, H, K = q.shape
     k = _seq_check("k", k, q.dtype, B, H, K)
     v = _seq_check("v", v, q.dtype, B, H, None)
@@ -487,15 +493,15 @@ def _step(q, k, v, log_decay, state, out_state, scale, slots):
     if not (1 <= K <= 256 and 1 <= V <= 256):
         raise RuntimeError(f"head sizes from 1 to 256 are served, got K = {K}, V = {V}")
     log_decay = _f32("log_decay", log_decay, H)
-    o = torch.empty((B, H, V), dtype=q.dtype, device=dev)
+    o = q.new_empty((B, H, V))
     wide = 0
     if slots is not None:
         slots, wide = _index("slots", slots, B)
     strides = [_TWO(*t.stride()[:2]) for t in (q, k, v)]
     with _on(dev):
         rc = _cabi.lib().cet_linear_attention_step(
-            code, B, H, K, V, *strides, _at(q), _at(k), _at(v), _at(log_decay), scale, _at(state), _at(out_state),
-            state.shape[0], _at(slots), wide, _at(o), _stream(dev))
+            code, B, H, K, V, *strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), scale,
+            state.data_ptr(), out_state.data_ptr(), state.shape[0], _at(slots), wide, o.data_ptr(), _stream(dev))
     _cabi.check(rc, "cet_linear_attention_step")
     return o
 
@@ -542,9 +548,9 @@ def run_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tens
            gain: float, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """q [B,T,Hq,D], k [B,T,Hk,D] or None, positions int32 / int64 [T] or [B,T], inv_freq float64 [pairs]
     -> the turned q and k (empty without k)."""
-    dev = _dev_check(*(t for t in (q, k, positions, inv_freq) if t is not None))
+    dev = _dev_check(q, positions, inv_freq) if k is None else _dev_check(q, k, positions, inv_freq)
     code = _seq_type(q)
-    q = _seq_check("q", q, q.dtype, None, None, None, None)
+    q = _seq_first("q", q, 4)
     B, T, Hq, D = q.shape
     if k is not None:
         k = _seq_check("k", k, q.dtype, B, T, None, D)
@@ -552,7 +558,7 @@ def run_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tens
         raise RuntimeError(f"inv_freq must be float64 [pairs] with 1 <= pairs <= D / 2, got {inv_freq.dtype} "
                            f"{list(inv_freq.shape)} for D = {D}")
     inv_freq = inv_freq.contiguous()
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((T,), (B, T)):
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape not in ((T,), (B, T)):
         raise RuntimeError(f"positions must be int32 or int64 [{T}] or [{B}, {T}], got {positions.dtype} {list(positions.shape)}")
     if not math.isfinite(gain):
         raise RuntimeError(f"gain must be finite, got {gain}")
@@ -564,11 +570,11 @@ def run_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tens
     if k is not None:
         d.k[:] = k.stride()[:3]
     d.pos[:] = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
-    qo = torch.empty((B, T, Hq, D), dtype=q.dtype, device=dev)
-    ko = torch.empty((B, T, Hk, D) if k is not None else (0,), dtype=q.dtype, device=dev)
+    qo = q.new_empty((B, T, Hq, D))
+    ko = q.new_empty((B, T, Hk, D) if k is not None else (0,))
     with _on(dev):
-        rc = _cabi.lib().cet_rotary(d, _at(q), _at(k), _at(positions), _at(inv_freq), int(inverse), _at(qo), _at(ko),
-                                    _stream(dev))
+        rc = _cabi.lib().cet_rotary(d, q.data_ptr(), _at(k), positions.data_ptr(), inv_freq.data_ptr(), int(inverse),
+                                    qo.data_ptr(), ko.data_ptr(), _stream(dev))
     _cabi.check(rc, "cet_rotary")
     return qo, ko
 
@@ -632,7 +638,7 @@ def _gated(x, w_gate, w_up, b_gate, b_up, activation, dy=None):
     code = _seq_type(x)
     if activation not in GATED_ACTIVATIONS:
         raise RuntimeError(f"activation must be one of {sorted(GATED_ACTIVATIONS)}, got {activation!r}")
-    x = _seq_check("x", x, x.dtype, None, None)
+    x = _seq_first("x", x, 2)
     N, D = x.shape
     w_gate = _seq_check("w_gate", w_gate, x.dtype, None, D)
     F = w_gate.shape[0]
@@ -651,12 +657,12 @@ def run_gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, 
                  b_up: Optional[torch.Tensor], activation: str) -> torch.Tensor:
     """x [N,D], w_gate, w_up [F,D], b_gate, b_up [F] or None -> act(x w_gate^T + b_gate) * (x w_up^T + b_up) [N,F]."""
     dev, d, x, w_gate, w_up, b_gate, b_up, _ = _gated(x, w_gate, w_up, b_gate, b_up, activation)
-    out = torch.empty((d.N, d.F), dtype=x.dtype, device=dev)
+    out = x.new_empty((d.N, d.F))
     L = _cabi.lib()
     with _on(dev):
-        n = L.cet_gated_linear_workspace(d, _at(x), _at(w_gate), _at(w_up), 0)
+        n = L.cet_gated_linear_workspace(d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), 0)
         ws = _workspace(n, dev)
-        rc = L.cet_gated_linear(d, _at(x), _at(w_gate), _at(w_up), _at(b_gate), _at(b_up), _at(out), _at(ws), n,
+        rc = L.cet_gated_linear(d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _at(b_gate), _at(b_up), out.data_ptr(), _at(ws), n,
                                 _stream(dev))
     _cabi.check(rc, "cet_gated_linear")
     return out
