@@ -326,7 +326,7 @@ def _index(name, t, n):
 
 def _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o=None):
     """Checked operands of the linear attention calls and their descriptor."""
-    dev = _dev_check(*(t for t in (q, k, v, log_decay, initial_state, lengths, d_o) if t is not None))
+    dev = _dev_check(*[t for t in (q, k, v, log_decay, initial_state, lengths, d_o) if t is not None])
     code = _seq_type(q)
     q = _seq_first("q", q, 4)
     B, T, H, K = q.shape
@@ -346,9 +346,9 @@ def _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o=None):
     if d_o is not None:
         d_o = _seq_check("d_o", d_o, q.dtype, B, T, H, V)
     d = _cabi.LinattnDesc(code, B, T, H, K, V, wide, scale)
-    for name, t in (("q", q), ("k", k), ("v", v), ("d_o", d_o)):
-        if t is not None:
-            getattr(d, name)[:] = t.stride()[:3]
+    d.q[:], d.k[:], d.v[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    if d_o is not None:
+        d.d_o[:] = d_o.stride()[:3]
     return dev, d, q, k, v, log_decay, initial_state, lengths, d_o
 
 
@@ -380,7 +380,7 @@ def run_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     """q, k [B,T,H,K], v [B,T,H,V] -> o [B,T,H,V], state float32 [B,H,K,V], and with `keep` the states between
     segments of a long time axis for the backward call (else empty)."""
     dev, d, q, k, v, log_decay, s0, lengths, _ = _linattn(q, k, v, log_decay, scale, initial_state, lengths)
-    o = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
+    o = q.new_empty((d.B, d.T, d.H, d.V))
     state = torch.empty((d.B, d.H, d.K, d.V), dtype=torch.float32, device=dev)
     L = _cabi.lib()
     with _on(dev):
@@ -414,8 +414,7 @@ def run_linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     if d_state is not None:
         _dev_check(q, d_state)
         d_state = _f32("d_state", d_state, d.B, d.H, d.K, d.V)
-    dq, dk = (torch.empty((d.B, d.T, d.H, d.K), dtype=q.dtype, device=dev) for _ in range(2))
-    dv = torch.empty((d.B, d.T, d.H, d.V), dtype=q.dtype, device=dev)
+    dq, dk, dv = q.new_empty(q.shape), q.new_empty(q.shape), q.new_empty(v.shape)
     ds = torch.empty((d.B, d.H, d.K, d.V) if want_initial else (0,), dtype=torch.float32, device=dev)
     L = _cabi.lib()
     with _on(dev):
@@ -634,7 +633,7 @@ GATED_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 
 def _gated(x, w_gate, w_up, b_gate, b_up, activation, dy=None):
     """Checked operands of the gated projection and their descriptor; x and dy as matrices."""
-    dev = _dev_check(*(t for t in (x, w_gate, w_up, b_gate, b_up, dy) if t is not None))
+    dev = _dev_check(*[t for t in (x, w_gate, w_up, b_gate, b_up, dy) if t is not None])
     code = _seq_type(x)
     if activation not in GATED_ACTIVATIONS:
         raise RuntimeError(f"activation must be one of {sorted(GATED_ACTIVATIONS)}, got {activation!r}")
@@ -645,7 +644,8 @@ def _gated(x, w_gate, w_up, b_gate, b_up, activation, dy=None):
     w_up = _seq_check("w_up", w_up, x.dtype, F, D)
     if D < 1 or F < 1 or D > 1 << 20 or F > 1 << 20 or N > 1 << 28:
         raise RuntimeError(f"x [N, D] and weights [F, D] with N up to 2^28, D and F from 1 to 2^20 are served, got {N}, {D}, {F}")
-    b_gate, b_up = (None if b is None else _seq_check(n, b, x.dtype, F) for n, b in (("b_gate", b_gate), ("b_up", b_up)))
+    b_gate = None if b_gate is None else _seq_check("b_gate", b_gate, x.dtype, F)
+    b_up = None if b_up is None else _seq_check("b_up", b_up, x.dtype, F)
     if dy is not None:
         dy = _seq_check("dy", dy, x.dtype, N, F)
     d = _cabi.GatedDesc(code, GATED_ACTIVATIONS[activation], N, D, F, x.stride(0), w_gate.stride(0), w_up.stride(0),
@@ -681,16 +681,16 @@ def run_gated_linear_backward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch
                           want_b: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """-> dx, dw_gate, dw_up, db_gate, db_up; empty where not wanted."""
     dev, d, x, w_gate, w_up, b_gate, b_up, dy = _gated(x, w_gate, w_up, b_gate, b_up, activation, dy)
-    new = lambda want, *shape: torch.empty(shape if want else (0,), dtype=x.dtype, device=dev)  # noqa: E731
+    new = lambda want, *shape: x.new_empty(shape if want else (0,))  # noqa: E731
     dx, dw_gate, dw_up = new(want_x, d.N, d.D), new(want_w, d.F, d.D), new(want_w, d.F, d.D)
     db_gate, db_up = new(want_b, d.F), new(want_b, d.F)
     L = _cabi.lib()
     with _on(dev):
-        n = L.cet_gated_linear_workspace(d, _at(x), _at(w_gate), _at(w_up), 1)
+        n = L.cet_gated_linear_workspace(d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), 1)
         ws = _workspace(n, dev)
-        rc = L.cet_gated_linear_backward(d, _at(x), _at(w_gate), _at(w_up), _at(b_gate), _at(b_up), _at(dy), _at(dx),
-                                         _at(dw_gate), _at(dw_up), _at(db_gate), _at(db_up), _at(ws), n,
-                                         _stream(dev))
+        rc = L.cet_gated_linear_backward(
+            d, x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), _at(b_gate), _at(b_up), dy.data_ptr(), dx.data_ptr(),
+            dw_gate.data_ptr(), dw_up.data_ptr(), db_gate.data_ptr(), db_up.data_ptr(), _at(ws), n, _stream(dev))
     _cabi.check(rc, "cet_gated_linear_backward")
     return dx, dw_gate, dw_up, db_gate, db_up
 
