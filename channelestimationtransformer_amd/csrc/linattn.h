@@ -640,13 +640,13 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
 }
 
 // Columns of V that a workgroup takes: 16 (one wave, as long as that wave can bring in the rows of K in few
-// instructions); 128 in bf16 up to K = 128, where four waves hold their state in 64 registers each, and in fp32 up to
-// K = 64, by eight waves; else 64, and 32 where rows of 256 fp32 fill LDS. (bf16, 128 x 128, 8 x 16 heads x 2048
-// slots: 82 us a pass; 64 columns by eight waves, two to the K of a column, 101 us, and 119 us with one workgroup per
-// CU and no segments. fp32, 40 x 72, 16 x 6 heads of up to 777 slots: 35 us, by slices of 64 columns 50.)
+// instructions), else 64 or, from 65 on, 128: in bf16 up to K = 128 by four waves that hold their state in 64 registers
+// each, otherwise by eight. (bf16, 128 x 128, 8 x 16 heads x 2048 slots: 82 us a pass; 64 columns by eight waves, two to
+// the K of a column, 101 us, and 119 us with one workgroup per CU and no segments. bf16, 256 x 256, 16 x 6 heads x
+// 2048 slots: 241 us, by slices of 64 columns 320. fp32, 40 x 72, 16 x 6 heads of up to 777 slots: 35 us, by 64 50.)
 inline int slice_columns(int dtype, int K, int V) {
   if (V <= 16 && K <= 64) return 16;
-  return V > 64 && (dtype != CET_BF16 || K <= 128) ? 128 : 64;
+  return V > 64 ? 128 : 64;
 }
 
 // How many of them a CU holds at once and keeps busy: single waves as many as LDS takes; one where rows of 256 fill
@@ -662,7 +662,7 @@ inline void launch_k(const Passes& p, unsigned blocks, hipStream_t s) {
   const int cols = slice_columns(BF ? CET_BF16 : CET_F32, p.a[0].K, p.a[0].V);
   if constexpr (NK <= 4)
     if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(p);
-  if constexpr (!BF)
+  if constexpr (!BF || NK > 8)
     if (cols == 128) return chunks<IO, NK, 1, 8, 1, OUT><<<blocks, 512, 0, s>>>(p);
   if constexpr (NK <= 8 && BF)
     if (cols == 128) return chunks<IO, NK, 2, 4, 1, OUT><<<blocks, 256, 0, s>>>(p);
@@ -676,7 +676,7 @@ inline void launch_k(const Passes& p, unsigned blocks, hipStream_t s) {
 // none is issued for blocks that do not exist (16 x 6 heads of up to 777 slots, K = 40: 35 us a pass, as K = 64 38).
 inline int k_blocks(int dtype, int K) {
   const int n = (K + 15) / 16;
-  if (dtype == CET_BF16) return n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
+  if (dtype == CET_BF16) return n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : n <= 12 ? 12 : 16;
   return n <= 4 ? n : n <= 6 ? 6 : n <= 8 ? 8 : n <= 12 ? 12 : 16;
 }
 // Passes of one launch have the same kernel and slices.
@@ -702,9 +702,7 @@ inline void launch(const Passes& p, unsigned blocks, hipStream_t s) {
       if constexpr (!BF) launch_k<IO, 6, OUT>(p, blocks, s);
       break;
     case 8: launch_k<IO, 8, OUT>(p, blocks, s); break;
-    case 12:
-      if constexpr (!BF) launch_k<IO, 12, OUT>(p, blocks, s);
-      break;
+    case 12: launch_k<IO, 12, OUT>(p, blocks, s); break;
     default: launch_k<IO, 16, OUT>(p, blocks, s);
   }
 }
