@@ -644,7 +644,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
 // each, otherwise by eight. (bf16, 128 x 128, 8 x 16 heads x 2048 slots: 82 us a pass; 64 columns by eight waves, two to
 // the K of a column, 101 us, and 119 us with one workgroup per CU and no segments. bf16, 256 x 256, 16 x 6 heads x
 // 2048 slots: 241 us, by slices of 64 columns 320. fp32, 40 x 72, 16 x 6 heads of up to 777 slots: 35 us, by 64 50.)
-inline int slice_columns(int dtype, int K, int V) {
+inline int slice_columns(int K, int V) {
   if (V <= 16 && K <= 64) return 16;
   return V > 64 ? 128 : 64;
 }
@@ -652,14 +652,14 @@ inline int slice_columns(int dtype, int K, int V) {
 // How many of them a CU holds at once and keeps busy: single waves as many as LDS takes; one where rows of 256 fill
 // it, two otherwise.
 inline int workgroups_per_cu(int dtype, int K, int V) {
-  if (slice_columns(dtype, K, V) == 16) return K > 32 ? 4 : 8;
+  if (slice_columns(K, V) == 16) return K > 32 ? 4 : 8;
   return K > 128 && (dtype == CET_BF16 || V > 64) ? 1 : 2;
 }
 
 template <typename IO, int NK, bool OUT>
 inline void launch_k(const Passes& p, unsigned blocks, hipStream_t s) {
   constexpr bool BF = Type<IO>::BF;
-  const int cols = slice_columns(BF ? CET_BF16 : CET_F32, p.a[0].K, p.a[0].V);
+  const int cols = slice_columns(p.a[0].K, p.a[0].V);
   if constexpr (NK <= 4)
     if (cols == 16) return chunks<IO, NK, 1, 1, 1, OUT><<<blocks, 64, 0, s>>>(p);
   if constexpr (!BF || NK > 8)
@@ -681,8 +681,8 @@ inline int k_blocks(int dtype, int K) {
 }
 // Passes of one launch have the same kernel and slices.
 inline bool alike(int dtype, const Args& a, const Args& b) {
-  const int cols = slice_columns(dtype, a.K, a.V);
-  return k_blocks(dtype, a.K) == k_blocks(dtype, b.K) && cols == slice_columns(dtype, b.K, b.V) &&
+  const int cols = slice_columns(a.K, a.V);
+  return k_blocks(dtype, a.K) == k_blocks(dtype, b.K) && cols == slice_columns(b.K, b.V) &&
          (a.V + cols - 1) / cols == (b.V + cols - 1) / cols;
 }
 

@@ -291,7 +291,7 @@ bool by_columns(const cet_linattn_desc& d) {
 
 Cut cut(const cet_linattn_desc& d) {
   if (by_columns(d)) return Cut{1, std::max(d.T, 1), 0};
-  const int cols = slice_columns(d.dtype, d.K, d.V);
+  const int cols = slice_columns(d.K, d.V);
   const long tasks = (long)d.B * d.H * ((d.V + cols - 1) / cols), chunks = (d.T + STATE_SLOTS - 1) / STATE_SLOTS;
   const long room = (long)cu_count() * workgroups_per_cu(d.dtype, d.K, d.V);
   long per = std::max<long>(chunks, 1), best = (tasks + room - 1) / room * per;
@@ -311,7 +311,7 @@ Cut cut(const cet_linattn_desc& d) {
 // A launch of passes of one shape; `nseg`: segments that have work.
 int launch(Passes& p, bool out, int nseg, int dtype, hipStream_t s) {
   const Args& a = p.a[0];
-  const int cols = slice_columns(dtype, a.K, a.V);
+  const int cols = slice_columns(a.K, a.V);
   for (int i = 0; i < p.n; ++i) p.a[i].nslice = (a.V + cols - 1) / cols;
   const unsigned blocks = (unsigned)((long)a.B * a.H * nseg * a.nslice * p.n);
   if (dtype == CET_F32)
