@@ -103,6 +103,7 @@ struct Type {
   typedef IO V4 __attribute__((ext_vector_type(4)));
   static constexpr bool BF = __is_same(IO, __bf16);
   typedef typename Pick<BF, bf4, f4>::T Quad;  // four values of an operand: k = 4g..4g+3
+  typedef typename Pick<BF, bf8, f4>::T Score; // four fp32 values as an operand: in bf16 two terms of each, x and what is left
   __device__ static Quad quad(const V4& v) {
     if constexpr (BF || __is_same(IO, float))
       return v;
@@ -130,6 +131,15 @@ __device__ inline f4 mma32(const bf4& a0, const bf4& a1, const bf4& b0, const bf
 }
 __device__ inline bf4 to_bf(const f4& v) { return bf4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}; }
 __device__ inline f4 to_f(const bf4& v) { return f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
+// An fp32 operand of bf16 products in two terms, 2^-16 of it at most left out: scores and states are sums in fp32, and
+// rounded to one term they made the outputs' error 1.4 times that of their own rounding. (8 x 16 heads x 2048 slots of
+// 128 x 128: 134 us forward and 308 for the gradients, with one term 119 and 271; 96 heads of 256 x 256: 276, 229.)
+__device__ inline bf8 two_terms(const f4& v) {
+  const bf4 hi = to_bf(v);
+  return __builtin_shufflevector(hi, to_bf(v - to_f(hi)), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ inline bf4 first_term(const bf8& v) { return __builtin_shufflevector(v, v, 0, 1, 2, 3); }
+__device__ inline bf4 second_term(const bf8& v) { return __builtin_shufflevector(v, v, 4, 5, 6, 7); }
 
 __device__ inline unsigned lds_address(const void* p) {
   return (unsigned)(unsigned long)(const __attribute__((address_space(3))) char*)p;
@@ -238,6 +248,7 @@ template <typename IO, int NK, int NV, int WC, int KH, bool OUT>
 __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1 ? 1 : 2) void chunks(const Passes passes) {
   typedef Type<IO> Ty;
   typedef typename Ty::Quad Quad;
+  typedef typename Ty::Score Score;
   constexpr int C = chunk_slots(Ty::BF, OUT, NK, WC), NB = C / 16;
   constexpr int NW = WC * KH, DK = row_width(NK, sizeof(IO)), NKW = NK / KH, SL = 16 * NV * WC;
   constexpr bool SHARE = NW > 1;  // one wave keeps its scores
@@ -251,11 +262,11 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
   // Buffers in a ring: rows of chunk c + BUFS are asked for when everybody has left chunk c.
   constexpr int BUF = (OUT ? 2 : 1) * TK::BYTES + TV::BYTES;
   // Three where that leaves room for two workgroups on a CU, or where two would not either.
-  constexpr int REST = (OUT && SHARE ? 2 * SCORES * 64 * (int)sizeof(Quad) : 0) + (OUT && KH == 2 ? 2 * NW * NV * 1024 : 0);
+  constexpr int REST = (OUT && SHARE ? 2 * SCORES * 64 * (int)sizeof(Score) : 0) + (OUT && KH == 2 ? 2 * NW * NV * 1024 : 0);
   constexpr int BUFS = SHARE && (3 * BUF + REST <= 81920 || (2 * BUF + REST > 81920 && 3 * BUF + REST <= 163840)) ? 3 : 2;
   constexpr int PARTS = BUF / 1024, PER = PARTS / NW, EXTRA = PARTS % NW;  // of a chunk; of each wave; of the first waves
   __shared__ __align__(1024) char tiles[BUFS][BUF];
-  __shared__ Quad ps[2][OUT && SHARE ? SCORES : 1][64];
+  __shared__ Score ps[2][OUT && SHARE ? SCORES : 1][64];
   __shared__ f4 xs[2][OUT && KH == 2 ? NW : 1][NV][64];
 
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -380,7 +391,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
 #pragma unroll
     for (int r = 0; r < 4; ++r) p[r] = sb == tb ? (i >= 4 * g + r ? p[r] * wd[r] : 0.f) : p[r] * wo[r];
     if constexpr (Ty::BF)
-      return to_bf(p);  // rounded to the tensors' type for the second product, as its sum will be
+      return two_terms(p);
     else
       return p;
   };
@@ -415,7 +426,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
       for (int y = 0; y < NV; ++y) vf[sb][y] = TV::cols(vc, sb, wc * NV + y);
 
     f4 acc[OUT ? NB : 1][NV];
-    Quad pf[OUT ? BLOCKS : 1];
+    Score pf[OUT ? BLOCKS : 1];
     const int flip = (at / C) & 1;
     if (OUT) {
       constexpr int TB[3] = {0, 1, 1}, SB[3] = {0, 0, 1};  // the blocks on and below the diagonal
@@ -439,18 +450,23 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
 #pragma unroll
         for (int y = 0; y < NV; ++y) acc[tb][y] = f4{0.f, 0.f, 0.f, 0.f};
       if (have && busy) {
-        // the state enters this product rounded to bf16 (where the tensors are), the only place where it is: an
-        // error of at most half a step of the output's own type on its share of the sum
         const float dm = pw_fast(g2, m);
 #pragma unroll
         for (int x = 0; x < NKW; x += Ty::BF ? 2 : 1) {
+          if constexpr (Ty::BF) {
 #pragma unroll
-          for (int tb = 0; tb < NB; ++tb) {
-            if constexpr (Ty::BF) {
-              const Quad q0 = TK::rows(qr, tb, k0 / 16 + x), q1 = TK::rows(qr, tb, k0 / 16 + x + 1);
+            for (int y = 0; y < NV; ++y) {
+              const bf8 s0 = two_terms(S[x][y]), s1 = two_terms(S[x + 1][y]);
 #pragma unroll
-              for (int y = 0; y < NV; ++y) acc[tb][y] = mma32(to_bf(S[x][y]), to_bf(S[x + 1][y]), q0, q1, acc[tb][y]);
-            } else {
+              for (int tb = 0; tb < NB; ++tb) {
+                const Quad q0 = TK::rows(qr, tb, k0 / 16 + x), q1 = TK::rows(qr, tb, k0 / 16 + x + 1);
+                acc[tb][y] = mma32(second_term(s0), second_term(s1), q0, q1, acc[tb][y]);
+                acc[tb][y] = mma32(first_term(s0), first_term(s1), q0, q1, acc[tb][y]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int tb = 0; tb < NB; ++tb) {
               const Quad q0 = TK::rows(qr, tb, k0 / 16 + x);
 #pragma unroll
               for (int y = 0; y < NV; ++y) acc[tb][y] = mma16(S[x][y], q0, acc[tb][y]);
@@ -573,8 +589,10 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
           out[y] = KH == 2 ? (kh ? acc[NB - 1][y] : acc[0][y]) : acc[t][y];
           if constexpr (KH == 2) out[y] += xs[flip][kh ? wave - WC : wave + WC][y][lane];
           if constexpr (Ty::BF) {
-            const bf4 none = bf4{(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f};
-            out[y] = mma32(vf[0][y], tb ? vf[1][y] : none, tb ? pf[1] : pf[0], tb ? pf[2] : none, out[y]);
+            const bf4 none = bf4{(__bf16)0.f, (__bf16)0.f, (__bf16)0.f, (__bf16)0.f}, v1 = tb ? vf[1][y] : none;
+            const Score p0 = tb ? pf[1] : pf[0];
+            out[y] = mma32(vf[0][y], v1, second_term(p0), tb ? second_term(pf[2]) : none, out[y]);
+            out[y] = mma32(vf[0][y], v1, first_term(p0), tb ? first_term(pf[2]) : none, out[y]);
           } else {
             if constexpr (NB == 1) {
               out[y] = mma16(vf[0][y], pf[0], out[y]);

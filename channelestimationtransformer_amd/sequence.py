@@ -32,7 +32,8 @@ def linear_attention(q, k, v, log_decay, scale=None, initial_state=None, lengths
     decay is a constant: it has no gradient and is refused if it wants one. Any strides with a
     contiguous last axis are read in place where rows start on 16 bytes, copied once otherwise. Slots are
     taken in chunks of up to 32: an infinity or NaN in a slot within its sequence's length can reach the
-    outputs of the slots of its chunk before it, too."""
+    outputs of the slots of its chunk before it, too (an infinity as NaN). Sums and states are float32, and o and the
+    gradients are rounded once; for bfloat16 tensors scores and states enter their products with 16 bits."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0
     if log_decay.requires_grad and torch.is_grad_enabled():

@@ -334,6 +334,8 @@ size_t cet_linear_attention_states(const cet_linattn_desc* d);
  * either may be NULL (zero; not wanted). o: device [B,T,H,V] contiguous, every element is written.
  * states: NULL, or cet_linear_attention_states() bytes that keep the states between segments for the backward call.
  * initial and states start on 16 bytes.
+ * o is rounded once; of bfloat16 tensors the scores and the state enter their products in two terms (2^-16 of them left
+ * out), the states that are kept and returned are sums of exact products in fp32. The gradients are formed alike.
  * Slots of q, k and v at or behind lengths[b] are not read. The workspace is 16-byte aligned and used by
  * this call until it has run on the stream. */
 int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
