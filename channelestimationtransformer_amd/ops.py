@@ -478,7 +478,7 @@ class LinearAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_state, _):
-        return _linattn_backward(ctx, d_o, d_state, None, run_linear_attention_backward)
+        return _linattn_backward(ctx, d_o, d_state, None, run_linear_attention_backward if direct(d_o, d_state) else linear_attention_backward)
 
 
 def _step(q, k, v, log_decay, state, out_state, scale, slots):
@@ -620,7 +620,7 @@ class Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        return _rotary_backward(ctx, dq, dk, direct_rotary)
+        return _rotary_backward(ctx, dq, dk, direct_rotary if direct(dq, dk) else rotary)
 
 
 def direct_rotary(q, k, *rest):
@@ -730,7 +730,7 @@ class GatedLinear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _gated_backward(ctx, dy, run_gated_linear_backward)
+        return _gated_backward(ctx, dy, run_gated_linear_backward if direct(dy) else gated_linear_backward)
 
 
 _PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
@@ -743,9 +743,18 @@ def step_in_place(q, k, v, log_decay, state, scale, slots):
     return o
 
 
+def _modes():
+    """Whether a mode wants to see the calls (a default device does not)."""
+    return any(not isinstance(torch._C._get_function_stack_at(n), torch.utils._device.DeviceContext)
+               for n in range(torch._C._len_torch_function_stack()))
+
+
 def direct(*tensors):
-    """Whether a call may pass the dispatcher by: eager, and on plain tensors only (none of a tracer's)."""
-    if torch.compiler.is_compiling():
+    """Whether a call may pass the dispatcher by: eager, on plain tensors, with no tracer and no mode active (they
+    would see the allocations of the results and not what fills them)."""
+    if torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
+        return False
+    if torch._C._len_torch_function_stack() and _modes():
         return False
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("forward-mode differentiation is not supported")  # the tangents would be dropped in silence
