@@ -74,8 +74,8 @@ def rotary_frequencies(dim, base=10000.0, scaling="none", factor=1.0, original_l
     * "ntk": the base times factor ** (dim / (dim - 2)), so that the slowest pair is stretched by
       `factor` and the fastest keeps its rate;
     * "yarn": pairs that turn more than turns[0] times within `original_length` keep their rate, those
-      below turns[1] are divided by `factor`, a linear ramp over the pairs between; gain
-      0.1 ln(factor) + 1."""
+      below turns[1] are divided by `factor`, a linear ramp over the pairs between, from the last of the
+      former to the first of the latter (which may lie behind the last pair); gain 0.1 ln(factor) + 1."""
     dim = int(dim)
     if dim < 2 or dim % 2:
         raise RuntimeError(f"dim must be even and positive, got {dim}")
@@ -93,8 +93,9 @@ def rotary_frequencies(dim, base=10000.0, scaling="none", factor=1.0, original_l
         if not original_length or original_length <= 0 or not turns[0] > turns[1] > 0:
             raise RuntimeError("yarn needs original_length > 0 and turns[0] > turns[1] > 0")
         pair = [dim * math.log(original_length / (n * 2 * math.pi)) / (2 * math.log(base)) for n in turns]
-        low, high = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), dim // 2 - 1)
+        low, high = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), dim - 1)
         ramp = ((j - low) / max(high - low, 0.001)).clamp(0, 1)
+        ramp[j >= pair[1]] = 1.0  # (all of them where even the first turns less than turns[1] times)
         freq = freq / factor * ramp + freq * (1 - ramp)
         gain = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
     return freq.to(device), gain
