@@ -195,9 +195,9 @@ enum { SILU, GELU, RELU };
 __device__ inline float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 
 // The activation and its slope. silu: s = 1 / (1 + e^-g). gelu: the normal distribution's density e = e^(-g^2/2) and
-// its tail by the rational form of Abramowitz and Stegun 7.1.26, |error| < 0.75e-7 of the distribution and, unlike
-// 1 + erf, without a branch between two ranges (erff took half the time of a narrow layer's pass). Exponential and
-// reciprocal are the hardware's, 1 ulp each.
+// its tail P(-|g|) = e R(|g|), R a polynomial of t = 1 / (1 + 0.3 |g|) fitted by least maximum of its relative error (1.5e-7 for |g| up to
+// 14), so that the tail keeps its bits as far as e does; without a branch between two ranges (erff took half the
+// time of a narrow layer's pass). Exponential and reciprocal are the hardware's, 1 ulp each.
 template <int KIND>
 __device__ inline void act1(float g, float& a, float& slope) {
   if constexpr (KIND == SILU) {
@@ -206,9 +206,12 @@ __device__ inline void act1(float g, float& a, float& slope) {
     slope = s * fmaf(g, 1.f - s, 1.f);
   } else if constexpr (KIND == GELU) {
     const float e = fast_exp(-0.5f * g * g);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752440f, fabsf(g), 1.f));
-    const float tail = 0.5f * t * e *
-                       fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(g), 1.f));
+    float r = fmaf(t, 0.035674780f, -0.15720310f);
+    r = fmaf(t, fmaf(t, r, 0.20635351f), -0.053683635f);
+    r = fmaf(t, fmaf(t, r, 0.12856161f), 0.099913498f);
+    r = fmaf(t, fmaf(t, r, 0.12075395f), 0.11962930f);
+    const float tail = e * (t * r);
     const float p = g < 0.f ? tail : 1.f - tail;
     a = g * p;
     slope = fmaf(g * 0.39894228040143267794f, e, p);

@@ -386,7 +386,7 @@ int cet_rotary(const cet_rotary_desc* d, const void* q, const void* k, const voi
  * out [N,F] contiguous. Products and the activation are formed in fp32, out is rounded once. */
 typedef struct cet_gated_desc {
   int32_t dtype;
-  int32_t activation; /* 0 silu, 1 gelu (erf form, to 1e-7), 2 relu */
+  int32_t activation; /* 0 silu, 1 gelu (erf form, to (1.5 g^2 + 24) 2^-24 of itself), 2 relu */
   int32_t N, D, F;
   int64_t ld_x, ld_gate, ld_up;
   int64_t ld_dy; /* backward only */

@@ -1,0 +1,55 @@
+"""The activation of the gated projection by itself: one feature of x holds the gate's value, the up projection is 1.
+
+gelu(g) = g Phi(g) and, at the negative side, Phi(g) = e R with e = exp(-g^2 / 2): in units of 2^-24 of the value the exponent's two
+roundings and its constant's are 3 (g^2 / 2), exponential and reciprocal 2 each and another 1 in the reciprocal's argument, R's fit
+2.5, its eight steps 8, the products with e, g and the up projection 3, and the output's own 1: below 1.5 g^2 + 24. The slope
+g phi(g) + Phi(g) is off by that of its two terms. silu: 2 |g| for the exponent, then 2 + 2 + 4. Behind g = -13.2 e is
+below fp32's smallest normal number and taken as zero."""
+import math
+
+import pytest
+import torch
+
+import channelestimationtransformer_amd as cet
+import seq_ref as ref
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def gelu(g):
+    tail = 0.5 * torch.special.erfc(g.abs() / math.sqrt(2.0))
+    p = torch.where(g < 0, tail, 1 - tail)
+    phi = torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+    return g * p, g * phi + p, (1.5 * g * g + 24) * (g * p).abs(), (1.5 * g * g + 24) * ((g * phi).abs() + p)
+
+
+def silu(g):
+    s = 1 / (1 + torch.exp(-g))
+    return g * s, s * (1 + g * (1 - s)), (2 * g.abs() + 9) * (g * s).abs(), (2 * g.abs() + 24) * s * (1 + g.abs())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["gelu", "silu"])
+@pytest.mark.parametrize("N, D", [(4000, 1), (2000, 40), (60, 72), (1999, 72), (20000, 264)])
+def test_values_and_slopes_over_the_whole_range(N, D, kind, dtype):
+    """Narrow layers, few rows and tiles; the negative tail to a bound relative to itself."""
+    g = torch.cat([torch.linspace(-14.0, 14.0, N - N // 2), torch.linspace(-8.0, 0.0, N // 2)]).to(dtype)
+    F = 1 if D == 1 else D
+    x = torch.zeros(N, D)
+    x[:, 0] = g.float()
+    w_gate = torch.zeros(F, D)
+    w_gate[:, 0] = 1.0
+    x, w_gate = x.to(dtype).cuda().requires_grad_(), w_gate.to(dtype).cuda()
+    w_up, one = torch.zeros_like(w_gate), torch.ones(F, dtype=dtype, device="cuda")
+    out = cet.gated_linear(x, w_gate, w_up, None, one, activation=kind)
+    dy = torch.zeros_like(out)
+    dy[:, F - 1] = 1.0
+    dx, = torch.autograd.grad(out, x, dy)
+    a, slope, off, slope_off = (gelu if kind == "gelu" else silu)(g.double())
+    h, tiny = ref.half_step(dtype), 6e-8 if dtype == torch.float16 else 3e-37
+    # the slope is rounded to the tensors' type twice: as the projection's gradient and as dx
+    for got, want, lim, roundings in ((out.detach().cpu(), a, off, 1), (dx[:, :1].cpu(), slope, slope_off, 2)):
+        lim = (1.01 * (U * lim + roundings * h * want.abs()) + tiny)[:, None]
+        err = (got.double() - want[:, None]).abs()
+        assert (err <= lim).all(), (float((err / lim).max()), float(g[(err / lim).max(1)[0].argmax()]))
