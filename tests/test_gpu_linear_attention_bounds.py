@@ -1,4 +1,5 @@
-"""Linear attention within bounds that leave no room for operands of fewer bits.
+"""Linear attention within bounds that leave no room for operands of fewer bits, and with heads that remember
+thousands of slots.
 
 An output or gradient element is off by one rounding to the tensors' type and by (K + T + 64) fp32 roundings of the sum of
 the terms' absolute values (the same recurrence on absolute values, "mass"). In bfloat16 every term of the sum holds a score or a
@@ -9,7 +10,8 @@ import torch
 
 import channelestimationtransformer_amd as cet
 import seq_ref as ref
-from test_gpu_linear_attention import gpu, make, within
+from channelestimationtransformer_amd import _cabi
+from test_gpu_linear_attention import TYPES, gpu, make, within
 
 pytestmark = pytest.mark.gpu
 
@@ -42,8 +44,48 @@ def check(x, dtype, y=None, pick=None):
         within(a.detach(), b, c, n)
 
 
+def segments(dtype, B, T, H, K, V):
+    d = _cabi.LinattnDesc({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], B, T, H, K, V, 0, 1.0)
+    return _cabi.lib().cet_linear_attention_states(d) > 0
+
+
 @pytest.mark.parametrize("shape", [(2, 40, 2, 16, 16), (2, 100, 2, 24, 40), (2, 65, 2, 64, 64), (1, 33, 3, 128, 128), (2, 130, 2, 100, 130),
                                    (1, 200, 2, 40, 200), (1, 97, 1, 160, 50), (2, 70, 1, 192, 256), (1, 300, 1, 256, 256), (3, 500, 1, 64, 16)])
 def test_bfloat16_is_rounded_once(shape):
     """Scores and states keep more bits than the tensors, in the outputs and in all gradients."""
     check(make(*shape, torch.bfloat16, seed=sum(shape)), torch.bfloat16)
+
+SLOW = torch.log1p(-torch.exp2(-torch.tensor([8.0, 9.0, 10.0, 12.0])))  # 256 to 4096 slots
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("K, V", [(24, 40), (128, 128), (16, 8)])
+def test_far_weights_over_segments(K, V, ragged, dtype):
+    """The time axis cut into segments whose joined states still weigh in the outputs, the last state and its
+    gradient; one head forgets nothing."""
+    B, T = (2, 1100) if K < 128 else (1, 700)
+    x = make(B, T, 5, K, V, dtype, seed=K + V, ragged=ragged)
+    x["g"] = torch.cat([SLOW, torch.zeros(1)])
+    if ragged:
+        x["lengths"][0] = T - 37
+    assert segments(dtype, B, T, 5, K, V)
+    check(x, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B, K, V", [(128, 20, 40), (128, 100, 33), (512, 40, 16)])
+def test_a_state_multiplied_out_within_a_segment(B, K, V, dtype):
+    """Enough heads that the axis is not cut: decays that make the kept state's factor leave its range
+    several times, once, and never within the history."""
+    T, pick = 700, [0, B // 2, B - 1]
+    g = torch.Generator().manual_seed(B + K)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x = {"q": r(B, T, 4, K), "k": r(B, T, 4, K), "v": r(B, T, 4, V), "d_o": r(B, T, 4, V)}
+    x = {n: t.to(dtype) for n, t in x.items()}
+    x.update(s0=r(B, 4, K, V), d_state=r(B, 4, K, V), lengths=torch.randint(0, T + 1, (B,), generator=g),
+             g=torch.cat([torch.log(torch.tensor([0.75, 0.97])), SLOW[:1], torch.zeros(1)]))
+    x["lengths"][pick[0]], x["lengths"][pick[1]] = T, T - 19
+    assert not segments(dtype, B, T, 4, K, V)
+    y = {n: t.cuda() for n, t in x.items()}
+    check({n: t.double() if n not in ("g", "lengths") else t for n, t in x.items()}, dtype, y=y, pick=pick)
