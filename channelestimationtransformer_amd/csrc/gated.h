@@ -6,6 +6,10 @@
 //     dx = [dg du] [Wg; Wu]                                                             (backward 2)
 //     [dWg; dWu] = [dg du]^T x,   [dbg; dbu] = column sums of [dg du]                   (backward 3)
 //
+// dg and du are rounded to the tensors' type once, as the operands that the matrix instructions take: 0.0023 of a bf16
+// gradient against 0.0017 by its own rounding alone. In two terms they would double both products behind them (8192 x
+// 1024 to 2730: 210 us more of 480) and the bytes of dh. In fp16 they have that type's range, which callers are told.
+//
 // One product form: out[q][p] = sum_k P[p][k] Q[q][k], 16 x 16 tiles with p along the four registers of a
 // lane, so that a lane stores four neighbours of a row. Either operand may lie in memory with k contiguous
 // (rows) or with its own index contiguous (columns: dx reads the weights as they are, backward 3 both dh and x).

@@ -121,7 +121,10 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     layout of `torch.nn.Linear`, or two halves of one [2F, D]), biases [F] or None, one type for all;
     returns [..., F]. `activation`: "silu", "gelu" (erf form) or "relu". Projections and activation are
     formed in float32 and the result is rounded once; the projections are not kept for the gradient but
-    formed again, their gradients are rounded to the tensors' type before the last products."""
+    formed again. Their gradients are rounded to the tensors' type before the products that dx and the weights'
+    gradients are (an error of the size of the results' own rounding); in float16 they have that type's range, infinite
+    beyond 65504 and zero below 3e-8, which is what loss scaling is for. Layers with D and F up to 64 keep them in
+    float32."""
     if x.dim() < 1:
         raise RuntimeError("x must be [..., D]")
     args = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x, w_gate, w_up, b_gate, b_up, activation

@@ -53,3 +53,28 @@ def test_values_and_slopes_over_the_whole_range(N, D, kind, dtype):
         lim = (1.01 * (U * lim + roundings * h * want.abs()) + tiny)[:, None]
         err = (got.double() - want[:, None]).abs()
         assert (err <= lim).all(), (float((err / lim).max()), float(g[(err / lim).max(1)[0].argmax()]))
+
+
+@pytest.mark.parametrize("N, D, F", [(40, 8, 8), (40, 72, 80), (300, 72, 80)])
+def test_the_range_of_float16_gradients(N, D, F):
+    """dy u = 400 * 200 leaves float16: narrow layers keep the projections' gradients in float32 and give the
+    finite dx; wider ones store them, and what is out of range is infinite in every gradient that it enters, so that a
+    loss scaler sees it. The other rows and features are not touched."""
+    x = torch.zeros(N, D, dtype=torch.float16, device="cuda").requires_grad_()
+    w = torch.zeros(F, D, dtype=torch.float16, device="cuda")
+    w[3, 2] = 2.0 ** -10
+    w = [w.clone().requires_grad_() for _ in range(2)]
+    b = torch.full((F,), 200.0, dtype=torch.float16, device="cuda")
+    out = cet.gated_linear(x, w[0], w[1], None, b, activation="silu")  # gate 0: slope 1/2, act 0; up 200
+    dy = torch.zeros_like(out)
+    dy[5, 3], dy[6, 3] = 800.0, 80.0
+    dx, dwg, dwu = torch.autograd.grad(out, [x, *w], dy)
+    assert float(dx[6, 2]) == 80 * 200 / 2 / 1024
+    if D <= 64:
+        assert float(dx[5, 2]) == 800 * 200 / 2 / 1024
+    else:
+        assert math.isinf(float(dx[5, 2])) and not torch.isfinite(dwg[3]).any()
+    rest = torch.ones(N, dtype=torch.bool, device="cuda")
+    rest[5] = False
+    assert torch.isfinite(dx[rest]).all() and (dwu == 0).all()
+    assert (dwg[[f for f in range(F) if f != 3]] == 0).all()
