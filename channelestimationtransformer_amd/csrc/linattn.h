@@ -92,9 +92,10 @@ __device__ inline int row_count(const Args& a, int b) {
 // as many or fewer as soon as the rows are long: two workgroups (K up to 128) or three buffers then fit a CU's LDS, and
 // one wave holds all of K (2 x 6 heads of 128 x 128, 4096 slots: 59 us; 32 slots, K in halves by two waves and one
 // workgroup of 64 columns per CU 75; 186 heads of 256 x 256, 702 slots: 560 us, by slices of 32 columns 870).
+// Four blocks of K by eight waves too: with 32 slots nine of their 128 registers spilled, at the same times.
 constexpr int OUT_SLOTS = 32, STATE_SLOTS = 64;
-constexpr int chunk_slots(bool bf, bool out, int nk, int wc) {
-  if (out) return bf || nk <= 4 ? 32 : 16;
+constexpr int chunk_slots(bool bf, size_t bytes, bool out, int nk, int wc) {
+  if (out) return bf || nk < 4 || (nk == 4 && !(bytes == 4 && wc == 8)) ? 32 : 16;
   return bf ? 64 : nk > 8 ? 16 : nk > 4 || wc == 8 ? 32 : 64;
 }
 
@@ -249,7 +250,7 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
   typedef Type<IO> Ty;
   typedef typename Ty::Quad Quad;
   typedef typename Ty::Score Score;
-  constexpr int C = chunk_slots(Ty::BF, OUT, NK, WC), NB = C / 16;
+  constexpr int C = chunk_slots(Ty::BF, sizeof(IO), OUT, NK, WC), NB = C / 16;
   constexpr int NW = WC * KH, DK = row_width(NK, sizeof(IO)), NKW = NK / KH, SL = 16 * NV * WC;
   constexpr bool SHARE = NW > 1;  // one wave keeps its scores
   constexpr int BLOCKS = NB * (NB + 1) / 2, MINE = KH == 2 ? 1 : NB;
