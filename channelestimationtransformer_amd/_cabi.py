@@ -22,7 +22,7 @@ EXPORTS = (
     "cet_rnn_blob_size", "cet_rnn_create", "cet_rnn_rollout", "cet_rnn_select", "cet_rnn_rollout_static", "cet_lmmse", "cet_lmmse_direct",
     "cet_lmmse_llr", "cet_lmmse_block", "cet_lmmse_block_llr", "cet_lmmse_grid", "cet_ls_nn", "cet_nmse_sums", "cet_qpsk_bit_errors",
     "cet_linear_attention_states", "cet_linear_attention_workspace", "cet_linear_attention", "cet_linear_attention_backward",
-    "cet_linear_attention_step", "cet_rotary",
+    "cet_linear_attention_step", "cet_linear_attention_step_pool_workspace", "cet_linear_attention_step_pool", "cet_rotary",
     "cet_gated_linear_workspace", "cet_gated_linear", "cet_gated_linear_backward",
 )
 
@@ -115,6 +115,9 @@ def lib():
     L.cet_linear_attention.argtypes = [desc] + [vp] * 10 + [ctypes.c_size_t, vp]
     L.cet_linear_attention_backward.argtypes = [desc] + [vp] * 14 + [ctypes.c_size_t, vp]
     L.cet_linear_attention_step.argtypes = [ip] * 5 + [vp] * 7 + [ctypes.c_float, vp, vp, ip, vp, ip, vp, vp]
+    L.cet_linear_attention_step_pool_workspace.restype = ctypes.c_size_t
+    L.cet_linear_attention_step_pool_workspace.argtypes = [ip] * 2
+    L.cet_linear_attention_step_pool.argtypes = [ip] * 5 + [vp] * 7 + [ctypes.c_float, vp, ip, vp, ip, vp, vp, ctypes.c_size_t, vp]
     L.cet_rotary.argtypes = [ctypes.POINTER(RotaryDesc)] + [vp] * 4 + [ip] + [vp] * 3
     gated = ctypes.POINTER(GatedDesc)
     L.cet_gated_linear_workspace.restype = ctypes.c_size_t

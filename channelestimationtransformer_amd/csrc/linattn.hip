@@ -149,6 +149,7 @@ struct Step {
   const float* in;
   float* out;
   const void* slots;
+  const int* owner;  // first stream of the call in each row of the pool, where a table was made (else nullptr)
   IO* o;
   int B, H, K, V, rows, slots64, nslice;
   float scale;
@@ -156,6 +157,20 @@ struct Step {
 
 __device__ inline long slot_of(const void* slots, int wide, int b) {
   return wide ? static_cast<const long*>(slots)[b] : (long)static_cast<const int*>(slots)[b];
+}
+
+// owner[row] = the first stream of the call whose slot is that row, for the rows that are some stream's. The first
+// launch puts one of them there, the second takes the least; the rest of the table is neither written nor read.
+template <bool CLAIM>
+__global__ __launch_bounds__(256) void claim_rows(const void* __restrict__ slots, int wide, int B, int rows, int* owner) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= B) return;
+  const long row = slot_of(slots, wide, b);
+  if (row < 0 || row >= rows) return;
+  if (CLAIM)
+    atomicMin(owner + row, b);
+  else
+    owner[row] = b;
 }
 
 template <typename IO, int TX, int W>
@@ -174,9 +189,13 @@ __global__ __launch_bounds__(256) void step(const Step<IO> a) {
     row = slot_of(a.slots, a.slots64, b);
     // a slot that an earlier stream of this call has: two workgroups would update one state
     bool twice = false;
-    if (row >= 0)
-      for (int e = tid; e < b; e += 256) twice |= slot_of(a.slots, a.slots64, e) == row;
-    twice = __syncthreads_or(twice);
+    if (a.owner) {
+      twice = row >= 0 && row < a.rows && a.owner[row] != b;
+    } else {
+      if (row >= 0)
+        for (int e = tid; e < b; e += 256) twice |= slot_of(a.slots, a.slots64, e) == row;
+      twice = __syncthreads_or(twice);
+    }
     live = row >= 0 && row < a.rows && !twice;
     if (row >= 0 && !live) idle = __builtin_nanf("");
   }
@@ -416,14 +435,49 @@ void launch_step(const Step<IO>& a0, int cus, hipStream_t s) {
 template <typename IO>
 void run_step(int B, int H, int K, int V, const int64_t* qs, const int64_t* ks, const int64_t* vs, const void* q,
               const void* k, const void* v, const float* log_decay, float scale, const float* in, float* out, int rows,
-              const void* slots, int slots64, void* o, hipStream_t s) {
+              const void* slots, int slots64, const int* owner, void* o, hipStream_t s) {
   const Step<IO> a{static_cast<const IO*>(q), static_cast<const IO*>(k), static_cast<const IO*>(v), qs[0], qs[1], ks[0], ks[1],
-                   vs[0], vs[1], log_decay, in, out, slots, static_cast<IO*>(o), B, H, K, V, rows, slots64, 1, scale};
+                   vs[0], vs[1], log_decay, in, out, slots, owner, static_cast<IO*>(o), B, H, K, V, rows, slots64, 1, scale};
   const bool wide = V % 4 == 0 && ((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   if (wide)
     launch_step<IO, 4>(a, cu_count(), s);
   else
     launch_step<IO, 1>(a, cu_count(), s);
+}
+
+// Streams up to which every workgroup looks for its slot among those before it; for more a table of the rows' owners is
+// made first, by two launches. (Without slots, looking, with the table: 1024 streams of 2 heads of 16 x 16 4.9, 6.3, 8.8 us; 1024 of 8
+// heads of 128 x 128 209, 225, 229; 2048 of 8 of 64 x 64 87, 116, 104; 4096 197, 256, 226; 262,144 of one of 8 x 8 a call 282, 14,490, 366.)
+constexpr int FEW_STREAMS = 1024;
+
+int step_call(int dtype, int B, int H, int K, int V, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+              const void* q, const void* k, const void* v, const float* log_decay, float scale, const float* state_in,
+              float* state_out, int rows, const void* slots, int slots64, int* owner, void* o, hipStream_t s) {
+  if (dtype < CET_F32 || dtype > CET_F16 || B < 0 || H < 0 || K < 1 || V < 1 || rows < 0 || !std::isfinite(scale))
+    return CET_ERR_INVALID_ARG;
+  if (K > 256 || V > 256 || (double)B * H > (1 << 21)) return CET_ERR_UNSUPPORTED;
+  if ((long)B * H == 0) return CET_OK;
+  if (!q_strides || !k_strides || !v_strides || !q || !k || !v || !log_decay || !o) return CET_ERR_INVALID_ARG;
+  if (rows > 0 && (!state_in || !state_out)) return CET_ERR_INVALID_ARG;
+  if (slots ? state_in != state_out : rows < B) return CET_ERR_INVALID_ARG;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(state_in), z = reinterpret_cast<uintptr_t>(state_out);
+  const uintptr_t bytes = (uintptr_t)B * H * K * V * sizeof(float);
+  if (a != z && (a < z ? z - a : a - z) < bytes) return CET_ERR_INVALID_ARG;  // half overlapping
+  if (owner) {
+    const unsigned blocks = (unsigned)((B + 255) / 256);
+    claim_rows<false><<<blocks, 256, 0, s>>>(slots, slots64, B, rows, owner);
+    CET_HIP(hipGetLastError());
+    claim_rows<true><<<blocks, 256, 0, s>>>(slots, slots64, B, rows, owner);
+    CET_HIP(hipGetLastError());
+  }
+  if (dtype == CET_F32)
+    run_step<float>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, owner, o, s);
+  else if (dtype == CET_F16)
+    run_step<_Float16>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, owner, o, s);
+  else
+    run_step<__bf16>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, owner, o, s);
+  CET_HIP(hipGetLastError());
+  return CET_OK;
 }
 
 }  // namespace
@@ -543,25 +597,20 @@ int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64
                               const int64_t* v_strides, const void* q, const void* k, const void* v,
                               const float* log_decay, float scale, const float* state_in, float* state_out, int rows,
                               const void* slots, int slots64, void* o, void* stream) {
-  if (dtype < CET_F32 || dtype > CET_F16 || B < 0 || H < 0 || K < 1 || V < 1 || rows < 0 || !std::isfinite(scale))
-    return CET_ERR_INVALID_ARG;
-  if (K > 256 || V > 256 || (double)B * H > (1 << 21)) return CET_ERR_UNSUPPORTED;
-  if ((long)B * H == 0) return CET_OK;
-  if (!q_strides || !k_strides || !v_strides || !q || !k || !v || !log_decay || !o) return CET_ERR_INVALID_ARG;
-  if (rows > 0 && (!state_in || !state_out)) return CET_ERR_INVALID_ARG;
-  if (slots ? state_in != state_out : rows < B) return CET_ERR_INVALID_ARG;
-  const uintptr_t a = reinterpret_cast<uintptr_t>(state_in), z = reinterpret_cast<uintptr_t>(state_out);
-  const uintptr_t bytes = (uintptr_t)B * H * K * V * sizeof(float);
-  if (a != z && (a < z ? z - a : a - z) < bytes) return CET_ERR_INVALID_ARG;  // half overlapping
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == CET_F32)
-    run_step<float>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, o, s);
-  else if (dtype == CET_F16)
-    run_step<_Float16>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, o, s);
-  else
-    run_step<__bf16>(B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots, slots64, o, s);
-  CET_HIP(hipGetLastError());
-  return CET_OK;
+  return step_call(dtype, B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, state_in, state_out, rows, slots,
+                   slots64, nullptr, o, static_cast<hipStream_t>(stream));
+}
+
+size_t cet_linear_attention_step_pool_workspace(int B, int rows) { return B > FEW_STREAMS && rows > 0 ? align_up((size_t)rows * sizeof(int)) : 0; }
+
+int cet_linear_attention_step_pool(int dtype, int B, int H, int K, int V, const int64_t* q_strides, const int64_t* k_strides,
+                                   const int64_t* v_strides, const void* q, const void* k, const void* v,
+                                   const float* log_decay, float scale, float* states, int rows, const void* slots,
+                                   int slots64, void* o, void* workspace, size_t workspace_bytes, void* stream) {
+  const size_t need = cet_linear_attention_step_pool_workspace(B, rows);
+  if (!slots || need > workspace_bytes || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15)) return CET_ERR_INVALID_ARG;
+  return step_call(dtype, B, H, K, V, q_strides, k_strides, v_strides, q, k, v, log_decay, scale, states, states, rows, slots,
+                   slots64, need ? static_cast<int*>(workspace) : nullptr, o, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

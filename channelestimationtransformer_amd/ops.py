@@ -497,10 +497,18 @@ def _step(q, k, v, log_decay, state, out_state, scale, slots):
     if slots is not None:
         slots, wide = _index("slots", slots, B)
     strides = [_TWO(*t.stride()[:2]) for t in (q, k, v)]
+    L, rows = _cabi.lib(), state.shape[0]
     with _on(dev):
-        rc = _cabi.lib().cet_linear_attention_step(
-            code, B, H, K, V, *strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), scale,
-            state.data_ptr(), out_state.data_ptr(), state.shape[0], _at(slots), wide, o.data_ptr(), _stream(dev))
+        if slots is None:
+            rc = L.cet_linear_attention_step(
+                code, B, H, K, V, *strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), scale,
+                state.data_ptr(), out_state.data_ptr(), rows, None, 0, o.data_ptr(), _stream(dev))
+        else:
+            n = L.cet_linear_attention_step_pool_workspace(B, rows)
+            ws = _workspace(n, dev)
+            rc = L.cet_linear_attention_step_pool(
+                code, B, H, K, V, *strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), scale,
+                state.data_ptr(), rows, slots.data_ptr(), wide, o.data_ptr(), _at(ws), n, _stream(dev))
     _cabi.check(rc, "cet_linear_attention_step")
     return o
 

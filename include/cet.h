@@ -363,6 +363,16 @@ int cet_linear_attention_step(int dtype, int B, int H, int K, int V, const int64
                               const float* state_in, float* state_out, int rows, const void* slots,
                               int slots64, void* o, void* stream);
 
+/* The same on a pool of states (state_in = state_out = states, slots given) with a workspace (16-byte aligned, in use until
+ * the call has run on the stream; its contents need not be kept): of many streams those that share a slot are found in one
+ * pass over a table of the rows, where the call above compares each stream with all before it. */
+size_t cet_linear_attention_step_pool_workspace(int B, int rows);
+int cet_linear_attention_step_pool(int dtype, int B, int H, int K, int V, const int64_t* q_strides,
+                                   const int64_t* k_strides, const int64_t* v_strides, const void* q,
+                                   const void* k, const void* v, const float* log_decay, float scale,
+                                   float* states, int rows, const void* slots, int slots64, void* o,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Rotary positions of queries [B,T,Hq,D] and keys [B,T,Hk,D] (either head count may be 0 with NULL
  * pointers): pair j < pairs of a head is turned by position * inv_freq[j] radians and multiplied by
  * `gain`; the features behind 2 * pairs pass through. Pairs are (j, j + pairs), or (2j, 2j + 1) where
