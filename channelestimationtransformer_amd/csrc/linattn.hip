@@ -510,7 +510,7 @@ int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k
   if (!log_decay || (d->T > 0 && (!q || !k || !v || !o))) return CET_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(initial)) & 15)
     return CET_ERR_INVALID_ARG;
-  const size_t need = cet_linear_attention_workspace(d, q, k, v, nullptr, 0);
+  const size_t need = cet_linear_attention_workspace(d, q, k, v, nullptr, 0) - (states ? cut(*d).states : 0);
   if (need > workspace_bytes || (need && !workspace)) return CET_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -543,7 +543,7 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   if ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(initial) |
        reinterpret_cast<uintptr_t>(d_final)) & 15)
     return CET_ERR_INVALID_ARG;
-  const size_t need = cet_linear_attention_workspace(d, q, k, v, d_o, 1);
+  const size_t need = cet_linear_attention_workspace(d, q, k, v, d_o, 1) - (states ? cut(*d).states : 0);
   if (need > workspace_bytes || (need && !workspace)) return CET_ERR_INVALID_ARG;
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -553,7 +553,7 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   const Cut c = cut(*d);
   const bool columns = by_columns(*d);
   float* const forward = states ? const_cast<float*>(states) : reinterpret_cast<float*>(ws);  // only read where given
-  float* const back = reinterpret_cast<float*>(ws + c.states);
+  float* const back = reinterpret_cast<float*>(ws + (states ? 0 : c.states));
   Args a{};
   a.log_decay = log_decay, a.lengths = lengths, a.lengths64 = d->lengths64;
   a.B = d->B, a.T = d->T, a.H = d->H;

@@ -384,8 +384,9 @@ def run_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     state = torch.empty((d.B, d.H, d.K, d.V), dtype=torch.float32, device=dev)
     L = _cabi.lib()
     with _on(dev):
-        segments = torch.empty((L.cet_linear_attention_states(d) // 4 if keep else 0,), dtype=torch.float32, device=dev)
-        n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), None, 0)
+        kept = L.cet_linear_attention_states(d) if keep else 0
+        segments = torch.empty((kept // 4,), dtype=torch.float32, device=dev)
+        n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), None, 0) - kept
         ws = _workspace(n, dev)
         rc = L.cet_linear_attention(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths), _at(o), _at(state),
                                     _at(segments), _at(ws), n, _stream(dev))
@@ -418,10 +419,12 @@ def run_linear_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     ds = torch.empty((d.B, d.H, d.K, d.V) if want_initial else (0,), dtype=torch.float32, device=dev)
     L = _cabi.lib()
     with _on(dev):
+        kept = 0
         if segments is not None and segments.numel():
             _dev_check(q, segments)
-            segments = _f32("segments", segments, L.cet_linear_attention_states(d) // 4)
-        n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), _at(d_o), 1)
+            kept = L.cet_linear_attention_states(d)
+            segments = _f32("segments", segments, kept // 4)
+        n = L.cet_linear_attention_workspace(d, _at(q), _at(k), _at(v), _at(d_o), 1) - kept
         ws = _workspace(n, dev)
         rc = L.cet_linear_attention_backward(d, _at(q), _at(k), _at(v), _at(log_decay), _at(s0), _at(lengths), _at(segments),
                                              _at(d_o), _at(d_state), _at(dq), _at(dk), _at(dv), _at(ds), _at(ws), n,

@@ -320,7 +320,8 @@ typedef struct cet_linattn_desc {
 
 /* Bytes of workspace that the forward call (backward = 0) or the backward call (1) on these operands
  * needs (they depend on the pointers' alignment: operands whose rows do not start on 16 bytes are copied
- * into it); 0 is a valid answer. d_o may be NULL for the forward call. */
+ * into it); 0 is a valid answer. d_o may be NULL for the forward call. A call that is given `states` needs
+ * cet_linear_attention_states() bytes less. */
 size_t cet_linear_attention_workspace(const cet_linattn_desc* d, const void* q, const void* k, const void* v,
                                       const void* d_o, int backward);
 

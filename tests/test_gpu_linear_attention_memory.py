@@ -1,0 +1,55 @@
+"""What linear attention's calls allocate, and what they read."""
+import pytest
+import torch
+
+import seq_ref as ref
+from channelestimationtransformer_amd import _cabi, ops
+
+
+def descriptor(B, T, H, K, V, code=1):
+    d = _cabi.LinattnDesc(code, B, T, H, K, V, 1, 0.25)
+    d.q[:], d.k[:], d.v[:], d.d_o[:] = (T * H * K, H * K, K), (T * H * K, H * K, K), (T * H * V, H * V, V), (T * H * V, H * V, V)
+    return d
+
+
+def test_workspace_where_the_states_are_given():
+    """The states between segments are in the caller's tensor: no second room for them is asked for."""
+    L, P = _cabi.lib(), 4096
+    d = descriptor(1, 4000, 2, 64, 64)
+    states = L.cet_linear_attention_states(d)
+    assert states >= 2 * 64 * 64 * 4
+    forward, backward = (L.cet_linear_attention_workspace(d, P, P, P, P, b) for b in (0, 1))
+    assert forward == states and backward == 2 * states
+    short = backward - states - 1
+    assert L.cet_linear_attention_backward(d, P, P, P, P, None, None, P, P, None, P, P, P, None, P, short, None) == 1
+    # copies of operands are still asked for
+    odd = L.cet_linear_attention_workspace(d, P + 2, P, P, P, 0) - states
+    assert odd >= 4000 * 2 * 64 * 2
+    assert L.cet_linear_attention(d, P + 2, P, P, P, None, None, P, None, P, P, odd - 1, None) == 1
+
+
+@pytest.mark.gpu
+def test_a_training_call_holds_the_states_once():
+    B, T, H, K = 1, 8192, 2, 128
+    g = torch.Generator().manual_seed(0)
+    q, k, v, d_o = (torch.randn(B, T, H, K, generator=g).bfloat16().cuda() for _ in range(4))
+    decay = ref.geometric(H).cuda()
+    L, d = _cabi.lib(), descriptor(B, T, H, K, K)
+    states = L.cet_linear_attention_states(d)
+    assert states > 1 << 20
+
+    def peak(call):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = call()
+        torch.cuda.synchronize()
+        return out, torch.cuda.max_memory_allocated() - before
+
+    results = B * T * H * K * 2 + B * H * K * K * 4  # o and the last state
+    (o, s, kept), most = peak(lambda: ops.run_linear_attention(q, k, v, decay, 0.1, None, None, True))
+    assert kept.numel() * 4 == states and most < results + 1.5 * states
+    grads, most = peak(lambda: ops.run_linear_attention_backward(q, k, v, decay, 0.1, None, None, kept, d_o, None, False))
+    assert most < 3 * B * T * H * K * 2 + 1.5 * states
+    again = ops.run_linear_attention_backward(q, k, v, decay, 0.1, None, None, None, d_o, None, False)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
