@@ -79,11 +79,13 @@ __device__ inline float pw(float g2, int n) { return n == 0 ? 1.f : exp2f((float
 // the same without denormal results (below 2^-126 they are zero), in one instruction
 __device__ inline float pw_fast(float g2, int n) { return n == 0 ? 1.f : __builtin_amdgcn_exp2f((float)n * g2); }
 
-__device__ inline int row_count(const Args& a, int b) {
-  if (!a.lengths) return a.T;
-  const long n = a.lengths64 ? static_cast<const long*>(a.lengths)[b] : (long)static_cast<const int*>(a.lengths)[b];
-  return n < 0 ? 0 : n > a.T ? a.T : (int)n;
+// slots of sequence b that are in use
+__device__ inline int row_count(const void* lengths, int lengths64, int T, int b) {
+  if (!lengths) return T;
+  const long n = lengths64 ? static_cast<const long*>(lengths)[b] : (long)static_cast<const int*>(lengths)[b];
+  return n < 0 ? 0 : n > T ? T : (int)n;
 }
+__device__ inline int row_count(const Args& a, int b) { return row_count(a.lengths, a.lengths64, a.T, b); }
 
 // The arithmetic of a tensor type. float32 and float16 tensors are multiplied in fp32 (a float16
 // state or score would leave that type's range on long histories), bfloat16 ones in bf16.

@@ -36,14 +36,16 @@ __global__ __launch_bounds__(256) void join_segments(const Args a) {
   }
 }
 
-// [B,T,H,D] with any strides -> contiguous with D rounded up to a multiple of 16 bytes, zeros behind D
+// [B,T,H,D] with any strides -> contiguous with D rounded up to a multiple of 16 bytes, zeros behind D. Slots at and behind a
+// sequence's length are not read, here or by the kernels that take the copy, and nothing is written for them.
 template <typename E>
-__global__ __launch_bounds__(256) void pack_rows(const E* __restrict__ src, Strides s, E* __restrict__ dst, int T, int H,
-                                                 int D, int per_row, long total) {
+__global__ __launch_bounds__(256) void pack_rows(const E* __restrict__ src, Strides s, E* __restrict__ dst, const void* lengths,
+                                                 int lengths64, int T, int H, int D, int per_row, long total) {
   constexpr int VEC = 16 / sizeof(E);
   for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long)gridDim.x * 256) {
     const int c = (int)(at % per_row) * VEC;
     const long row = at / per_row, h = row % H, t = row / H % T, b = row / H / T;
+    if (t >= row_count(lengths, lengths64, T, (int)b)) continue;
     const E* p = src + b * s.b + t * s.t + h * s.h;
     E e[VEC];
 #pragma unroll
@@ -275,15 +277,15 @@ struct Operand {
                       (s.t % vec == 0 || d.T == 1) && (s.h % vec == 0 || d.H == 1);
     if (!wide && !by_columns(d)) copy = align_up((size_t)d.B * d.T * d.H * ((D + vec - 1) / vec) * 16);
   }
-  int pack(const cet_linattn_desc& d, char*& ws, hipStream_t stream) {
+  int pack(const cet_linattn_desc& d, const void* lengths, char*& ws, hipStream_t stream) {
     if (!copy) return CET_OK;
     const int vec = 16 / elem_bytes(d.dtype), per_row = (D + vec - 1) / vec;
     const long total = (long)d.B * d.T * d.H * per_row;
     const unsigned blocks = (unsigned)std::min<long>((total + 255) / 256, 1 << 20);
     if (d.dtype == CET_F32)
-      pack_rows<uint32_t><<<blocks, 256, 0, stream>>>(static_cast<const uint32_t*>(p), s, reinterpret_cast<uint32_t*>(ws), d.T, d.H, D, per_row, total);
+      pack_rows<uint32_t><<<blocks, 256, 0, stream>>>(static_cast<const uint32_t*>(p), s, reinterpret_cast<uint32_t*>(ws), lengths, d.lengths64, d.T, d.H, D, per_row, total);
     else
-      pack_rows<uint16_t><<<blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(p), s, reinterpret_cast<uint16_t*>(ws), d.T, d.H, D, per_row, total);
+      pack_rows<uint16_t><<<blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(p), s, reinterpret_cast<uint16_t*>(ws), lengths, d.lengths64, d.T, d.H, D, per_row, total);
     CET_HIP(hipGetLastError());
     const long row = (long)per_row * vec;
     p = ws;
@@ -516,7 +518,7 @@ int cet_linear_attention(const cet_linattn_desc* d, const void* q, const void* k
   char* ws = static_cast<char*>(workspace);
   Operand oq(q, d->q, d->K, *d), ok(k, d->k, d->K, *d), ov(v, d->v, d->V, *d);
   for (Operand* x : {&oq, &ok, &ov})
-    if (const int rc = x->pack(*d, ws, s)) return rc;
+    if (const int rc = x->pack(*d, lengths, ws, s)) return rc;
   const Cut c = cut(*d);
   const bool columns = by_columns(*d);
   Args a{};
@@ -549,7 +551,7 @@ int cet_linear_attention_backward(const cet_linattn_desc* d, const void* q, cons
   char* ws = static_cast<char*>(workspace);
   Operand oq(q, d->q, d->K, *d), ok(k, d->k, d->K, *d), ov(v, d->v, d->V, *d), og(d_o, d->d_o, d->V, *d);
   for (Operand* x : {&oq, &ok, &ov, &og})
-    if (const int rc = x->pack(*d, ws, s)) return rc;
+    if (const int rc = x->pack(*d, lengths, ws, s)) return rc;
   const Cut c = cut(*d);
   const bool columns = by_columns(*d);
   float* const forward = states ? const_cast<float*>(states) : reinterpret_cast<float*>(ws);  // only read where given

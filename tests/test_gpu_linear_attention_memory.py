@@ -53,3 +53,38 @@ def test_a_training_call_holds_the_states_once():
     assert most < 3 * B * T * H * K * 2 + 1.5 * states
     again = ops.run_linear_attention_backward(q, k, v, decay, 0.1, None, None, None, d_o, None, False)
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code, dtype", [(0, torch.float32), (1, torch.bfloat16), (2, torch.float16)])
+def test_copies_of_operands_stop_at_the_lengths(code, dtype):
+    """Rows that start off 16 bytes are copied into the workspace: only slots in use are, the copy's others stay as they were."""
+    B, T, H, K, V = 5, 50, 2, 17, 23
+    L, d = _cabi.lib(), descriptor(B, T, H, K, V, code)
+    g = torch.Generator().manual_seed(3)
+    q, k = (torch.randn(B, T, H, K, generator=g).to(dtype).cuda() for _ in range(2))
+    v, d_o = (torch.randn(B, T, H, V, generator=g).to(dtype).cuda() for _ in range(2))
+    lengths, decay = torch.tensor([0, 1, 33, 50, 70], device="cuda"), ref.geometric(H).cuda()
+    vec = 16 // q.element_size()
+    rows = [-(-n // vec) * vec for n in (K, K, V, V)]  # values of a row in the copies of q, k, v, d_o
+    o, dq, dk, dv = v.new_empty(B, T, H, V), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    state = torch.empty(B, H, K, V, device="cuda")
+    ptr = [t.data_ptr() for t in (q, k, v)]
+    live = torch.arange(T, device="cuda")[None] < lengths[:, None]
+    for backward in (0, 1):
+        n = L.cet_linear_attention_workspace(d, *ptr, d_o.data_ptr(), backward)
+        ws = torch.full((n,), 0x5A, dtype=torch.uint8, device="cuda")
+        stream = torch.cuda.current_stream().cuda_stream
+        if backward:
+            rc = L.cet_linear_attention_backward(d, *ptr, decay.data_ptr(), None, lengths.data_ptr(), None, d_o.data_ptr(), None, dq.data_ptr(),
+                                                 dk.data_ptr(), dv.data_ptr(), None, ws.data_ptr(), n, stream)
+        else:
+            rc = L.cet_linear_attention(d, *ptr, decay.data_ptr(), None, lengths.data_ptr(), o.data_ptr(), state.data_ptr(), None, ws.data_ptr(), n, stream)
+        assert rc == 0
+        at = 0
+        for width, x in zip(rows[:3 + backward], (q, k, v, d_o)):
+            size = B * T * H * width * q.element_size()
+            copy = ws[at:at + size].view(B, T, H, width * q.element_size())
+            assert (copy[~live] == 0x5A).all()
+            assert torch.equal(copy.contiguous().view(dtype).view(B, T, H, width)[..., :x.shape[3]][live], x[live])
+            at += (size + 255) // 256 * 256
