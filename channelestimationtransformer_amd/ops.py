@@ -37,7 +37,7 @@ def _f32(name, t, *shape):
     if t.shape != shape and (  # (the comparison alone where every size is given)
             t.dim() != len(shape) or any(s is not None and int(d) != int(s) for d, s in zip(t.shape, shape))):
         raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
-    t = t.contiguous()
+    t = t.contiguous() if t.numel() > 1 else t.contiguous().resolve_neg()  # (a single value may carry a flag for its sign)
     return t.clone() if t.data_ptr() % 16 else t  # a slice may start anywhere; the C ABI wants 16 B
 
 
@@ -300,7 +300,15 @@ def _seq_check(name, t, dtype, *shape):
     have = t.shape
     if have != shape and (len(have) != len(shape) or any(s is not None and s != d for s, d in zip(shape, have))):
         raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(have)}")
-    return t if have[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return _rows(t)
+
+
+def _rows(t):
+    """A contiguous last axis, and values as they lie in memory: the imaginary part of a conjugate is a view with a flag that
+    turns its sign (a copy does so, and every view of more than one such value in a row is copied)."""
+    if t.shape[-1] > 1:
+        return t if t.stride(-1) == 1 else t.contiguous()
+    return t.resolve_neg()
 
 
 def _seq_first(name, t, dim):
@@ -308,7 +316,7 @@ def _seq_first(name, t, dim):
     have = t.shape
     if len(have) != dim:
         raise RuntimeError(f"{name} must have shape {[None] * dim}, got {list(have)}")
-    return t if have[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return _rows(t)
 
 
 def _seq_type(t):
@@ -541,7 +549,7 @@ def run_linear_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
         raise RuntimeError(f"q, k, v must be [B, H, features], got {list(q.shape)}, {list(v.shape)}")
     want = (None if slots is not None else q.shape[0], q.shape[1], q.shape[2], v.shape[2])
     if state.dtype != torch.float32 or not state.is_contiguous() or state.dim() != 4 or any(
-            w is not None and s != w for s, w in zip(state.shape, want)):
+            w is not None and s != w for s, w in zip(state.shape, want)) or (state.numel() == 1 and state.is_neg()):
         raise RuntimeError(f"state must be contiguous float32 {list(want)}, got {state.dtype} {list(state.shape)}")
     return _step(q, k, v, log_decay, state, state, scale, slots)
 
