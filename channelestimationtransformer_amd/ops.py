@@ -338,6 +338,8 @@ def _linattn(q, k, v, log_decay, scale, initial_state, lengths, d_o=None):
     code = _seq_type(q)
     q = _seq_first("q", q, 4)
     B, T, H, K = q.shape
+    if T > 1 << 30 or B * H > 1 << 22:  # (the descriptor holds 32 bits of each)
+        raise RuntimeError(f"up to 2^30 slots and 2^22 heads of all sequences are served, got {T} and {B} x {H}")
     k = _seq_check("k", k, q.dtype, B, T, H, K)
     v = _seq_check("v", v, q.dtype, B, T, H, None)
     V = v.shape[3]
@@ -497,6 +499,8 @@ def _step(q, k, v, log_decay, state, out_state, scale, slots):
     code = _seq_type(q)
     q = _seq_first("q", q, 3)
     B, H, K = q.shape
+    if B * H > 1 << 21 or state.shape[0] >= 1 << 31:
+        raise RuntimeError(f"up to 2^21 heads of all streams and 2^31 - 1 states are served, got {B} x {H} and {state.shape[0]}")
     k = _seq_check("k", k, q.dtype, B, H, K)
     v = _seq_check("v", v, q.dtype, B, H, None)
     V = v.shape[2]
@@ -581,6 +585,8 @@ def run_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tens
     if not math.isfinite(gain):
         raise RuntimeError(f"gain must be finite, got {gain}")
     Hk = 0 if k is None else k.shape[2]
+    if B * T > 2 * 10 ** 9 or Hq > 65536 or Hk > 65536:
+        raise RuntimeError(f"up to 2e9 slots and 65536 heads are served, got {B} x {T}, {Hq} and {Hk}")
     if D > 1024:
         raise RuntimeError(f"heads of up to 1024 features are served, got D = {D}")
     d = _cabi.RotaryDesc(code, B, T, Hq, Hk, D, inv_freq.shape[0], int(interleaved), int(positions.dtype == torch.int64), gain)
