@@ -32,6 +32,13 @@ __device__ inline f4 mma4(const f4& a, const f4& b, f4 c) {
   return c;
 }
 
+// What lanes of a wave read of each other in LDS stays behind what they wrote (LDS takes a wave's accesses in order: only the
+// compiler has to be told).
+__device__ inline void between_lanes() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // 16 rows from `row` on as operands (k along the features): lane (i, g) holds features 16 kk + 4 g.. of row i
 template <typename T, int NK>
 __device__ inline void load_rows(f4 (&q)[NK], const void* p, long ld, long row, long rows, int cols, int step, int i, int g) {
@@ -165,7 +172,7 @@ __global__ __launch_bounds__(256, 1) void narrow_backward(const Narrow a) {
       db[f] += dh[f];
       db[NF + f] += dh[NF + f];
     }
-    // both operands of dW with the rows along k: through this wave's own LDS (in order, no other wave involved)
+    // both operands of dW with the rows along k: through this wave's own LDS
 #pragma unroll
     for (int kk = 0; kk < ND; ++kk) *reinterpret_cast<f4*>(xt + i * XLD + 16 * kk + 4 * g) = x[kk];
 #pragma unroll
@@ -189,6 +196,7 @@ __global__ __launch_bounds__(256, 1) void narrow_backward(const Narrow a) {
         if (row < a.N && at < a.D) store4(static_cast<T*>(a.dx) + row * a.D + at, v[d], a.D - at, a.dx_step);
       }
     }
+    between_lanes();
     f4 xq[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -202,6 +210,7 @@ __global__ __launch_bounds__(256, 1) void narrow_backward(const Narrow a) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) dw[f][d] = mma4(xq[d], hq, dw[f][d]);
     }
+    between_lanes();
   }
   if (!a.part) return;
   // sums over the four waves, one after the other, in the space of the weights; lane (i, g) of tile (f, d) holds
