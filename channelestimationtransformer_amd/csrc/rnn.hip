@@ -1060,13 +1060,18 @@ __global__ __launch_bounds__(256) void rnn_mid_kernel(const RArgs a) {
   for (int i = tid; i < (4 * MT * PSTR + NL * MT * HS) / 4; i += 256) st4(smem + 4 * i, f32x4{0, 0, 0, 0});
   for (int i = tid; i < NL * 2 * G * H / 4; i += 256) st4(lbias + 4 * i, ld4(a.bias + 4 * i));
 
-  // decoder rows (features 16 ft + c) x this wave's units, for the whole rollout
-  f32x4 wd[UTW][XB];
+  // Decoder rows (features 16 ft + c) x this wave's units, for the whole rollout where they fit beside the weight ring, the
+  // cell states and the new h. LSTM, 512 units, 3 layers: 256 registers without them; with their 64 the compiler spilled
+  // the ring's lane offset and read it back 800 times a step (4096 sequences 13.6 ms, reading the rows where they are used 9.5).
+  constexpr bool KEEP_DEC = 4 * (D * G + UTW * XB + UTW + (LSTM ? NL * UTW : 0)) <= 300;
+  auto dec_row = [&](int u, int ft) { return ld4(a.dec_w + (size_t)(16 * ft + c) * H + wave * (16 * UTW) + 16 * u + 4 * g); };
+  f32x4 wd[KEEP_DEC ? UTW : 1][XB];
+  if constexpr (KEEP_DEC) {
 #pragma unroll
-  for (int u = 0; u < UTW; ++u)
+    for (int u = 0; u < UTW; ++u)
 #pragma unroll
-    for (int ft = 0; ft < XB; ++ft)
-      wd[u][ft] = ld4(a.dec_w + (size_t)(16 * ft + c) * H + wave * (16 * UTW) + 16 * u + 4 * g);
+      for (int ft = 0; ft < XB; ++ft) wd[u][ft] = dec_row(u, ft);
+  }
   f32x4 bd[XB];
 #pragma unroll
   for (int ft = 0; ft < XB; ++ft) bd[ft] = ld4(a.dec_b + 16 * ft + 4 * g);
@@ -1146,9 +1151,15 @@ __global__ __launch_bounds__(256) void rnn_mid_kernel(const RArgs a) {
         // decoder Linear partial over this tile's units, straight from the registers
         if (l == NL - 1 && decode) {
 #pragma unroll
-          for (int ft = 0; ft < XB; ++ft)
+          for (int ft = 0; ft < XB; ++ft) {
+            f32x4 w;
+            if constexpr (KEEP_DEC)
+              w = wd[u][ft];
+            else
+              w = dec_row(u, ft);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dec_acc[ft] = mfma16(wd[u][ft][i], hnew[u][i], dec_acc[ft]);
+            for (int i = 0; i < 4; ++i) dec_acc[ft] = mfma16(w[i], hnew[u][i], dec_acc[ft]);
+          }
         }
       }
       __syncthreads();  // every wave has finished reading the old h of this layer
