@@ -132,11 +132,17 @@ __device__ inline f4 mma32(const bf4& a0, const bf4& a1, const bf4& b0, const bf
   const bf8 b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
-__device__ inline bf4 to_bf(const f4& v) { return bf4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]}; }
-__device__ inline f4 to_f(const bf4& v) { return f4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
+__device__ inline bf4 to_bf(const f4& v) { return __builtin_convertvector(v, bf4); }
+// (whole vectors one way and bits the other: of single conversions the compiler made the packed values and each by itself)
+__device__ inline f4 to_f(const bf4& v) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 w = __builtin_bit_cast(u2, v);
+  return f4{__builtin_bit_cast(float, w[0] << 16), __builtin_bit_cast(float, w[0] & 0xffff0000u), __builtin_bit_cast(float, w[1] << 16),
+            __builtin_bit_cast(float, w[1] & 0xffff0000u)};
+}
 // An fp32 operand of bf16 products in two terms, 2^-16 of it at most left out: scores and states are sums in fp32, and
 // rounded to one term they made the outputs' error 1.4 times that of their own rounding. (8 x 16 heads x 2048 slots of
-// 128 x 128: 134 us forward and 308 for the gradients, with one term 119 and 271; 96 heads of 256 x 256: 276, 229.)
+// 128 x 128: 126 us forward and 293 for the gradients, with one term 119 and 271; 96 heads of 256 x 256: 255, 229.)
 __device__ inline bf8 two_terms(const f4& v) {
   const bf4 hi = to_bf(v);
   return __builtin_shufflevector(hi, to_bf(v - to_f(hi)), 0, 1, 2, 3, 4, 5, 6, 7);
