@@ -300,15 +300,13 @@ def _seq_check(name, t, dtype, *shape):
     have = t.shape
     if have != shape and (len(have) != len(shape) or any(s is not None and s != d for s, d in zip(shape, have))):
         raise RuntimeError(f"{name} must have shape {list(shape)}, got {list(have)}")
-    return _rows(t)
+    return t if have[-1] > 1 and t.stride(-1) == 1 else _rows(t)
 
 
 def _rows(t):
     """A contiguous last axis, and values as they lie in memory: the imaginary part of a conjugate is a view with a flag that
     turns its sign (a copy does so, and every view of more than one such value in a row is copied)."""
-    if t.shape[-1] > 1:
-        return t if t.stride(-1) == 1 else t.contiguous()
-    return t.resolve_neg()
+    return t.contiguous() if t.shape[-1] > 1 else t.resolve_neg()
 
 
 def _seq_first(name, t, dim):
@@ -316,7 +314,7 @@ def _seq_first(name, t, dim):
     have = t.shape
     if len(have) != dim:
         raise RuntimeError(f"{name} must have shape {[None] * dim}, got {list(have)}")
-    return _rows(t)
+    return t if have[-1] > 1 and t.stride(-1) == 1 else _rows(t)
 
 
 def _seq_type(t):
@@ -491,7 +489,7 @@ class LinearAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_state, _):
-        return _linattn_backward(ctx, d_o, d_state, None, run_linear_attention_backward if direct(d_o, d_state) else linear_attention_backward)
+        return _linattn_backward(ctx, d_o, d_state, None, run_linear_attention_backward if direct_gradient(d_o, d_state) else linear_attention_backward)
 
 
 def _step(q, k, v, log_decay, state, out_state, scale, slots):
@@ -499,25 +497,27 @@ def _step(q, k, v, log_decay, state, out_state, scale, slots):
     code = _seq_type(q)
     q = _seq_first("q", q, 3)
     B, H, K = q.shape
-    if B * H > 1 << 21 or state.shape[0] >= 1 << 31:
-        raise RuntimeError(f"up to 2^21 heads of all streams and 2^31 - 1 states are served, got {B} x {H} and {state.shape[0]}")
+    if B * H > 1 << 21:
+        raise RuntimeError(f"up to 2^21 heads of all streams are served, got {B} x {H}")
     k = _seq_check("k", k, q.dtype, B, H, K)
     v = _seq_check("v", v, q.dtype, B, H, None)
     V = v.shape[2]
     if not (1 <= K <= 256 and 1 <= V <= 256):
         raise RuntimeError(f"head sizes from 1 to 256 are served, got K = {K}, V = {V}")
     log_decay = _f32("log_decay", log_decay, H)
-    o = q.new_empty((B, H, V))
-    wide = 0
     if slots is not None:
         slots, wide = _index("slots", slots, B)
+        rows = state.shape[0]
+        if rows >= 1 << 31:
+            raise RuntimeError(f"pools of up to 2^31 - 1 states are served, got {rows}")
+    o = q.new_empty((B, H, V))
     strides = [_TWO(*t.stride()[:2]) for t in (q, k, v)]
-    L, rows = _cabi.lib(), state.shape[0]
+    L = _cabi.lib()
     with _on(dev):
         if slots is None:
             rc = L.cet_linear_attention_step(
                 code, B, H, K, V, *strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), scale,
-                state.data_ptr(), out_state.data_ptr(), rows, None, 0, o.data_ptr(), _stream(dev))
+                state.data_ptr(), out_state.data_ptr(), B, None, 0, o.data_ptr(), _stream(dev))
         else:
             n = L.cet_linear_attention_step_pool_workspace(B, rows)
             ws = _workspace(n, dev)
@@ -645,7 +645,7 @@ class Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        return _rotary_backward(ctx, dq, dk, direct_rotary if direct(dq, dk) else rotary)
+        return _rotary_backward(ctx, dq, dk, direct_rotary if direct_gradient(dq, dk) else rotary)
 
 
 def direct_rotary(q, k, *rest):
@@ -755,7 +755,7 @@ class GatedLinear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        return _gated_backward(ctx, dy, run_gated_linear_backward if direct(dy) else gated_linear_backward)
+        return _gated_backward(ctx, dy, run_gated_linear_backward if direct_gradient(dy) else gated_linear_backward)
 
 
 _PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
@@ -768,21 +768,33 @@ def step_in_place(q, k, v, log_decay, state, scale, slots):
     return o
 
 
+_compiling, _tracing = torch.compiler.is_compiling, torch._C._is_tracing
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+
+
 def _modes():
     """Whether a mode wants to see the calls (a default device does not)."""
     return any(not isinstance(torch._C._get_function_stack_at(n), torch.utils._device.DeviceContext)
-               for n in range(torch._C._len_torch_function_stack()))
+               for n in range(_function_modes()))
 
 
 def direct(*tensors):
     """Whether a call may pass the dispatcher by: eager, on plain tensors, with no tracer and no mode active (they
     would see the allocations of the results and not what fills them)."""
-    if torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._len_torch_dispatch_stack():
-        return False
-    if torch._C._len_torch_function_stack() and _modes():
+    if _compiling() or _tracing() or _dispatch_modes() or (_function_modes() and _modes()):
         return False
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("forward-mode differentiation is not supported")  # the tangents would be dropped in silence
+    for t in tensors:
+        if type(t) not in _PLAIN:
+            return False
+    return True
+
+
+def direct_gradient(*tensors):
+    """The same for gradients on their way back, in fewer questions (the engine's thread takes twice as long for each)."""
+    if _dispatch_modes() or _function_modes() or _tracing():
+        return False
     for t in tensors:
         if type(t) not in _PLAIN:
             return False
