@@ -2,7 +2,7 @@
 // fit one CU, so that a pass over the rows does everything. Waves are persistent; each takes 16 rows at a time
 // straight into registers. Multiplied in fp32 whatever the tensors' type: what bounds these sizes is memory
 // (102,400 rows of 64 to 64 in fp32: 52 MB, 11 us at the rate of a large copy) and the fp32 matrix rate (11 us)
-// alike. Forward takes 33 us and backward 78; the tiled products took 40 and 375, most of it in passes over dh and
+// alike. Forward takes 34 us and backward 79; the tiled products took 40 and 375, most of it in passes over dh and
 // in launches.
 //
 //   forward:  the weights stay in a wave's registers; D tiles hold 4 neighbouring features of a row per lane.

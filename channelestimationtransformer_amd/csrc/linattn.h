@@ -281,9 +281,10 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, kh = wave / WC;
   // Workgroups go to the 8 XCDs in turn: the slices and passes of a segment, which read the same rows, are given to
-  // one, and share its L2 (the three gradients of 8 x 16 heads of 128 x 128, 2048 slots, bf16: 234 us, one after the
-  // other 251); the segments of a sequence are spread over all, so that long ones keep no XCD busy alone (32
-  // sequences, the first four full and the others of 64 slots, 16 heads, bf16: 200 us, by runs of workgroups 263).
+  // one, and share its L2 (the three gradients of 8 x 16 heads of 128 x 128, 2048 slots, bf16: 543 MB fetched, 700 in the
+  // order of the ids, in the same time; the whole backward call 255 us, with a launch for each gradient 281); the segments of
+  // a sequence are spread over all, so that long ones keep no XCD busy alone (32 sequences, the first four full and the
+  // others of 64 slots, 16 heads, bf16: 220 us forward and 256 for the gradients, by runs of workgroups 286 and 763).
   const int inner = passes.n * passes.a[0].nslice;
   unsigned id = blockIdx.x;
   int slice;
@@ -668,9 +669,10 @@ __global__ __launch_bounds__(64 * WC * KH, WC == 8 && NK <= 8 ? 4 : WC * KH == 1
 
 // Columns of V that a workgroup takes: 16 (one wave, as long as that wave can bring in the rows of K in few
 // instructions), else 64 or, from 65 on, 128: in bf16 up to K = 128 by four waves that hold their state in 64 registers
-// each, otherwise by eight. (bf16, 128 x 128, 8 x 16 heads x 2048 slots: 82 us a pass; 64 columns by eight waves, two to
-// the K of a column, 101 us, and 119 us with one workgroup per CU and no segments. bf16, 256 x 256, 16 x 6 heads x
-// 2048 slots: 241 us, by slices of 64 columns 320. fp32, 40 x 72, 16 x 6 heads of up to 777 slots: 35 us, by 64 50.)
+// each, otherwise by eight. (Forward and gradients in us, bf16, 128 x 128, 16 heads x 2048 slots, 32 sequences: 300 and 820,
+// by 64 columns with eight waves, two to the K of a column, 370 and 1015; 8 sequences 128 and 255, 124 and 288; 12 sequences, where
+// the coarser slices leave a round half empty, 197 and 389, 164 and 403. 256 x 256, 16 x 6 heads: 255 and 727, 328 and 803.
+// fp32, 40 x 72, 16 x 6 heads of up to 777 slots, a pass: 35, 50.)
 inline int slice_columns(int K, int V) {
   if (V <= 16 && K <= 64) return 16;
   return V > 64 ? 128 : 64;

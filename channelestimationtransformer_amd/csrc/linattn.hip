@@ -297,9 +297,9 @@ struct Operand {
 
 // How the time axis is cut: into segments where heads, sequences and slices alone are fewer than two workgroups
 // per CU, none shorter than 128 slots, as many as make the workgroups' rounds over the chip times the length of a
-// segment least (12 x 16 heads x 2048 slots, bf16, 128 x 128: two segments in one round 190 us with the states
-// between them, three in two rounds 206). Forward and backward cut it alike, and share the segments' states. (Three
-// or four workgroups per CU cost the bf16 training pass of 8 x 16 heads 20 to 25 %.)
+// segment least (forward and gradients in us, bf16, 128 x 128, 16 heads x 2048 slots, 12 sequences: two segments in one round 197 and
+// 389, three in two rounds 210 and 372; 8 sequences: 128 and 255, three 137 and 267, as for four workgroups per CU 158 and
+// 290). Forward and backward cut it alike, and share the segments' states.
 struct Cut {
   int nseg, seg_len;
   size_t states;  // bytes of the states between segments, K x V per head
