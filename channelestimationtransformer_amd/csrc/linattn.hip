@@ -162,7 +162,7 @@ __device__ inline long slot_of(const void* slots, int wide, int b) {
 }
 
 // owner[row] = the first stream of the call whose slot is that row, for the rows that are some stream's. The first
-// launch puts one of them there, the second takes the least; the rest of the table is neither written nor read.
+// launch clears these, the second takes the least; the rest of the table is neither written nor read.
 template <bool CLAIM>
 __global__ __launch_bounds__(256) void claim_rows(const void* __restrict__ slots, int wide, int B, int rows, int* owner) {
   const int b = blockIdx.x * 256 + threadIdx.x;
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256) void claim_rows(const void* __restrict__ slots
   if (CLAIM)
     atomicMin(owner + row, b);
   else
-    owner[row] = b;
+    owner[row] = 0x7fffffff;
 }
 
 template <typename IO, int TX, int W>
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256) void step(const Step<IO> a) {
     if (a.owner) {
       twice = row >= 0 && row < a.rows && a.owner[row] != b;
     } else {
-      if (row >= 0)
+      if (row >= 0 && row < a.rows)
         for (int e = tid; e < b; e += 256) twice |= slot_of(a.slots, a.slots64, e) == row;
       twice = __syncthreads_or(twice);
     }
